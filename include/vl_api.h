@@ -79,6 +79,8 @@ extern "C" {
 #define VL_STATUS_BAD_ID 1      /* token id outside [0, vocab)              */
 #define VL_STATUS_BAD_AUDIO 2   /* more audio placeholders than audio rows  */
 #define VL_STATUS_BAD_SLOT 4    /* KV slot >= num_slots                      */
+#define VL_STATUS_BAD_PAGE 8    /* page id, length or parent out of range    */
+#define VL_STATUS_TIMEOUT 16    /* a bounded wait inside a kernel ran out    */
 
 /* Whisper/GLM-ASR log-mel geometry (native/asr/src/mel_frontend.h:34-42). */
 #define VL_MEL_BINS 128
@@ -552,6 +554,177 @@ VL_EXPORT int vl_argmax_eos(const void* logits, int64_t rows, int64_t vocab, int
                             int64_t out_stride, const int32_t* positions,
                             const int64_t* prompt_length, const int64_t* eos_ids, int n_eos,
                             int64_t freeze_id, int dtype, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged KV cache and beam search                                            */
+/* ------------------------------------------------------------------------ */
+/*
+ * The reference decodes greedily over one contiguous cache per chunk
+ * (native/asr/src/decoder.cu:1372-1800).  The four calls below are what a
+ * beam search needs instead: a cache in pages that sequences can share,
+ * attention of one or many new tokens per sequence through the pages, the
+ * selection of the best continuations, and the reordering of the page tables
+ * after it.  They have no counterpart in the reference.
+ *
+ * Common arguments
+ *   caches      k_cache and v_cache: num_pages pages of [page_size][n_kv_heads]
+ *               [head_dim], consecutive pages page_stride elements apart (so a
+ *               layer of a [layers][pages]... or [pages][layers]... buffer can
+ *               be passed).  page_size is a power of two in [16, 256].
+ *   q_start     int32 [batch + 1], ascending: sequence b's new tokens are the
+ *               rows q_start[b] .. q_start[b+1] - 1 of q / k / v / out.  Rows
+ *               from q_start[batch] on (a padded batch) are neither read nor
+ *               written.
+ *   kv_len      int32 [batch]: positions of the sequence once its new tokens
+ *               are counted; the new tokens are the last ones, so token i of
+ *               n sits at position kv_len - n + i.
+ *   page_table  int32 [batch][table_stride], max_pages used: position p of
+ *               sequence b is row p % page_size of page
+ *               page_table[b][p / page_size].
+ * All three live in device memory, so that a captured graph serves changing
+ * lengths.  They cannot be checked on the host; what is out of range is
+ * skipped, and VL_STATUS_BAD_PAGE is OR-ed into *status (if given).  No call
+ * here allocates, synchronises or keeps anything between calls; calls on
+ * different streams are independent as long as their buffers are.
+ */
+
+/*
+ * Rotary embedding of q and k and the append of k and v to the pages.
+ * For every token at position p, with angle p * position_scale *
+ * base^(-2d/rotary_dim) for pair d < rotary_dim / 2 (formed and reduced in
+ * fp64, then fp32 sincosf):
+ *   x1' = x1*cos - x2*sin,  x2' = x2*cos + x1*sin     (fp32, one rounding)
+ * over the pairs (d, d + rotary_dim/2) of every head, or with interleaved != 0
+ * over the pairs (2d, 2d + 1).  Dims from rotary_dim on are copied.
+ *   q_out[t] = rotated q[t]   (q_out may be q itself; else it must not overlap)
+ *   cache rows of the position = rotated k[t], v[t]; k and v are only read.
+ * q may be NULL with n_q_heads 0.  rotary_dim 0 copies without rotation.
+ * position_scale < 1 compresses positions for contexts beyond the trained
+ * length (linear interpolation); a changed base does the rest.
+ * A token whose position is negative, beyond the table or in a page id
+ * outside [0, num_pages) is not cached and sets VL_STATUS_BAD_PAGE; its q
+ * row is still rotated.  f32 / f16 / bf16.  Two tokens of one call must not
+ * share a cache row.
+ */
+VL_EXPORT int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_out,
+                                   void* k_cache, void* v_cache, const int32_t* q_start,
+                                   const int32_t* kv_len, const int32_t* page_table,
+                                   int64_t tokens, int64_t batch, int64_t max_pages,
+                                   int64_t table_stride, int n_q_heads, int n_kv_heads,
+                                   int head_dim, int rotary_dim, int interleaved, double base,
+                                   double position_scale, int64_t q_row_stride,
+                                   int64_t k_row_stride, int64_t v_row_stride,
+                                   int64_t q_out_row_stride, int64_t num_pages, int page_size,
+                                   int64_t page_stride, int dtype, int32_t* status,
+                                   void* stream);
+
+/* Workspace bytes of vl_paged_attention (0 for arguments it refuses). */
+VL_EXPORT size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batch,
+                                                    int64_t max_q_len, int n_q_heads,
+                                                    int n_kv_heads, int head_dim, int dtype);
+
+/*
+ * Causal attention of each sequence's new tokens over its pages (which hold
+ * the new tokens' k and v already): token i of n, query head h:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  j <= kv_len - n + i
+ * with kv head h / (n_q_heads / n_kv_heads); scale 0 means 1/sqrt(head_dim).
+ * Scores, softmax and sums in fp32, one rounding of the output; in f16 / bf16
+ * at head_dim 64 or 128 the probabilities are rounded to the storage type
+ * before the second product.  A token that sees no position (kv_len < n)
+ * gives a zero row.
+ * max_q_len bounds the new tokens of any sequence and chooses the kernel
+ * (single tokens and a few tokens stream the cache once; longer chunks run
+ * on the tcgen05 tensor cores); a sequence with more gives zero rows and
+ * VL_STATUS_BAD_PAGE, as does a kv_len outside [0, max_pages * page_size].
+ * out may be q itself; else it must overlap neither q nor a cache.
+ * A page id outside [0, num_pages) reads as rows of zeros and sets the bit.
+ * Cache rows at and beyond kv_len may hold anything.  A non-finite k or v
+ * below kv_len may reach the output of any query of its sequence.
+ * f32 / f16 / bf16; head_dim a multiple of 32 up to 256.
+ * workspace: vl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ * no initialisation; calls that may overlap on the GPU need their own.
+ * flags: 0 or VL_LAUNCH_PDL (the kernel before it in the stream must not
+ * write q_start, kv_len or page_table).
+ */
+VL_EXPORT int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                                 const int32_t* q_start, const int32_t* kv_len,
+                                 const int32_t* page_table, int64_t tokens, int64_t batch,
+                                 int64_t max_q_len, int64_t max_pages, int64_t table_stride,
+                                 int n_q_heads, int n_kv_heads, int head_dim, float scale,
+                                 int64_t q_row_stride, int64_t out_row_stride,
+                                 int64_t num_pages, int page_size, int64_t page_stride,
+                                 void* out, int dtype, void* workspace,
+                                 size_t workspace_bytes, int32_t* status, int flags,
+                                 void* stream);
+
+/* Workspace bytes of vl_beam_select (0 for arguments it refuses). */
+VL_EXPORT size_t vl_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab);
+
+/*
+ * One step's selection of beam search.  logits [batch * beams][row_stride]
+ * (vocab used), scores [batch][beams] the beams' summed log-probabilities.
+ * A live beam b offers every token v with value
+ *   scores[b] + logits[b][v] - log(sum_v exp(logits[b][v]));
+ * a finished beam (finished given and non-zero) offers pad_id with its own
+ * score and nothing else.  The `beams` best values of an entry, in
+ * descending order, ties going to the lower b * vocab + v:
+ *   tokens   int64 [batch][beams]   the token (pad_id in an empty place)
+ *   parents  int32 [batch][beams]   the beam it continues (its own index there)
+ *   scores_out  f32, finished_out u8: the value, and whether the parent was
+ *               finished or the token is one of eos_ids (a HOST array, n_eos <= 8).
+ * Candidates whose value is NaN or -inf are none: logits of -inf or NaN are
+ * never taken, a row with a +inf logit or without a finite sum offers
+ * nothing, nor does a beam whose score is -inf (start with scores 0, -inf,
+ * -inf, ...).  Places without a candidate get value -inf and are finished.
+ * scores_out may be scores and finished_out may be finished; finished_out may
+ * be NULL.  Sums in fp32 per thread and fp64 across threads, values in fp64,
+ * rounded to f32 once.  beams <= 32, vocab <= 2^24, f32 / f16 / bf16; any
+ * vocab and row_stride.  workspace as in vl_paged_attention.
+ */
+#define VL_BEAM_MAX 32
+VL_EXPORT int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
+                             int64_t row_stride, const float* scores, const uint8_t* finished,
+                             const int64_t* eos_ids, int n_eos, int64_t pad_id,
+                             int64_t* tokens, int32_t* parents, float* scores_out,
+                             uint8_t* finished_out, int dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Page tables after a selection: row (e, i) of the new tables continues row
+ * (e, parents[e][i]) of the old ones, with its length L = kv_len there.
+ *   - the L / page_size whole pages are shared with the parent (and with
+ *     whatever else holds them);
+ *   - the page of position L, which the next append writes, becomes the
+ *     row's own.  With L % page_size == 0 it is a fresh page.  Else the
+ *     parent's part-filled page is kept by the lowest row that takes it, if
+ *     it lies in the entry's own range and no row of the entry reads it as
+ *     a whole page; the other rows get a fresh page, and the filled rows are
+ *     copied into it in every layer of k_cache and v_cache;
+ *   - entries behind it are -1.  Nothing is allocated when L has reached
+ *     max_pages * page_size.
+ * Fresh pages come from the entry's range pool_start[e] .. + pool_pages - 1:
+ * those that no new row holds, lowest first, in row order.  Pages that no row
+ * holds any more are free again without further notice.  Pages outside the
+ * range (a shared prompt) are never written.  With the shared prompt outside
+ * it, beams * (pages of a row behind the prompt's whole pages) pages suffice.
+ * A parent outside [0, beams), a bad length, page id or range, or an
+ * exhausted range leaves -1 (and for the first two length 0) and sets
+ * VL_STATUS_BAD_PAGE.
+ * table_out and kv_len_out must not overlap the inputs.  caches:
+ * [layers][num_pages] pages of page_bytes bytes (row_bytes * page_size),
+ * layer_stride_bytes and page_stride_bytes apart; layers 0 moves no cache.
+ * Ranges of different entries must not overlap.  beams <= 32,
+ * beams * pool_pages and pool_pages <= 16384, max_pages <= 4096.
+ */
+VL_EXPORT int vl_paged_beam_reorder(const int32_t* page_table, const int32_t* parents,
+                                    const int32_t* kv_len, const int32_t* pool_start,
+                                    int64_t pool_pages, int64_t batch, int beams,
+                                    int64_t max_pages, int64_t table_stride, int32_t* table_out,
+                                    int64_t table_out_stride, int32_t* kv_len_out,
+                                    void* k_cache, void* v_cache, int64_t layers,
+                                    int64_t num_pages, int page_size, int64_t row_bytes,
+                                    int64_t page_stride_bytes, int64_t layer_stride_bytes,
+                                    int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

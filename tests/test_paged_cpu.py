@@ -1,0 +1,216 @@
+"""CPU: what the paged-cache and beam-search entry points refuse, before any
+CUDA call, and the plain statements the GPU tests compare with, against
+independent small cases."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref
+import vlasr
+from vlasr import _lib
+
+FAKE = 0x10000
+FAR = 0x100000000     # bases far enough apart not to overlap
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return vlasr.load()
+
+
+def _err(lib) -> str:
+    return lib.vl_last_error().decode()
+
+
+def test_append_rejects(lib):
+    def call(q=FAR, k=2 * FAR, v=3 * FAR, qo=4 * FAR, kc=5 * FAR, vc=6 * FAR, qst=FAKE, kvl=FAKE,
+             tab=FAKE, tokens=4, batch=2, max_pages=8, ts=8, nq=16, nkv=4, hd=128, rot=128,
+             inter=0, base=1e4, scale=1.0, qs=2048, ks=512, vs=512, os_=2048, pages=64, ps=16,
+             stride=16 * 512, dtype=2):
+        return lib.vl_paged_rope_append(q, k, v, qo, kc, vc, qst, kvl, tab, tokens, batch,
+                                        max_pages, ts, nq, nkv, hd, rot, inter, base, scale, qs,
+                                        ks, vs, os_, pages, ps, stride, dtype, None, None)
+
+    assert call(k=None) == 2 and "null" in _err(lib)
+    assert call(kc=None) == 2 and "null" in _err(lib)
+    assert call(tab=None) == 2 and "null" in _err(lib)
+    assert call(q=None) == 2 and "n_q_heads" in _err(lib)
+    assert call(dtype=5) == 2 and "dtype" in _err(lib)
+    assert call(tokens=-1) == 2 and "shape" in _err(lib)
+    assert call(nkv=0) == 2 and "shape" in _err(lib)
+    for ps in (0, 8, 24, 512):
+        assert call(ps=ps, stride=1 << 20) == 2 and "page_size" in _err(lib)
+    assert call(pages=0) == 2 and "num_pages" in _err(lib)
+    assert call(ts=7) == 2 and "table_stride" in _err(lib)
+    assert call(stride=100) == 2 and "page_stride" in _err(lib)
+    assert call(rot=130) == 2 and "rotary_dim" in _err(lib)
+    assert call(rot=63) == 2 and "rotary_dim" in _err(lib)
+    assert call(inter=2) == 2 and "interleaved" in _err(lib)
+    assert call(base=0.0) == 2 and "base" in _err(lib)
+    assert call(scale=math.inf) == 2 and "position_scale" in _err(lib)
+    assert call(qs=100) == 2 and "strides" in _err(lib)
+    assert call(qo=FAR + 64) == 2 and "overlaps" in _err(lib)
+    # disjoint columns of one buffer are not an overlap; nothing to do is not an error
+    assert call(tokens=0, qo=FAR + 4096, qs=6144, os_=6144) == 0
+    assert call(batch=0) == 0
+
+
+def test_attention_rejects(lib):
+    def call(q=FAR, kc=2 * FAR, vc=3 * FAR, qst=FAKE, kvl=FAKE, tab=FAKE, tokens=4, batch=4,
+             mq=1, max_pages=8, ts=8, nq=16, nkv=4, hd=128, scale=0.0, qs=2048, os_=2048,
+             pages=64, ps=16, stride=16 * 512, out=4 * FAR, dtype=2, ws=5 * FAR, wsb=1 << 30,
+             flags=0):
+        return lib.vl_paged_attention(q, kc, vc, qst, kvl, tab, tokens, batch, mq, max_pages, ts,
+                                      nq, nkv, hd, scale, qs, os_, pages, ps, stride, out, dtype,
+                                      ws, wsb, None, flags, None)
+
+    assert call(q=None) == 2 and "null" in _err(lib)
+    assert call(kvl=None) == 2 and "null" in _err(lib)
+    assert call(dtype=9) == 2 and "dtype" in _err(lib)
+    assert call(flags=4) == 2 and "flags" in _err(lib)
+    assert call(nq=14) == 2 and "heads" in _err(lib)
+    assert call(nq=1024, nkv=4, qs=1 << 17, os_=1 << 17) == 2 and "heads" in _err(lib)
+    assert call(hd=72, nkv=4) == 2 and "head_dim" in _err(lib)
+    assert call(hd=288, stride=1 << 20) == 2 and "head_dim" in _err(lib)
+    assert call(mq=0) == 2 and "max_q_len" in _err(lib)
+    assert call(scale=math.nan) == 2 and "scale" in _err(lib)
+    assert call(scale=-1.0) == 2 and "scale" in _err(lib)
+    assert call(os_=100) == 2 and "strides" in _err(lib)
+    assert call(qs=2052) == 2 and "multiples" in _err(lib)
+    assert call(stride=16 * 512 + 4) == 2 and "multiples" in _err(lib)
+    assert call(out=4 * FAR + 2) == 2 and "aligned" in _err(lib)
+    assert call(ps=48) == 2 and "page_size" in _err(lib)
+    assert call(wsb=8) == 2 and "workspace" in _err(lib)
+    assert call(ws=None) == 2 and "workspace" in _err(lib)
+    assert call(out=2 * FAR) == 2 and "overlaps" in _err(lib)
+    assert call(out=FAR + 2048) == 2 and "overlaps" in _err(lib)
+    assert call(tokens=0) == 0 and call(batch=0) == 0
+    ws = lib.vl_paged_attention_workspace_bytes
+    assert ws(4, 4, 1, 16, 4, 128, 2) > 0
+    assert ws(4, 4, 1, 15, 4, 128, 2) == 0 and ws(4, 4, 0, 16, 4, 128, 2) == 0
+    assert ws(4, 4, 1, 16, 4, 100, 2) == 0 and ws(-1, 4, 1, 16, 4, 128, 2) == 0
+
+
+def test_select_rejects(lib):
+    eos = (ctypes.c_int64 * 2)(1, 2)
+
+    def call(lg=FAR, batch=2, beams=4, vocab=1000, rs=1000, sc=FAKE, fin=None, n_eos=2, pad=0,
+             tok=2 * FAR, par=3 * FAR, so=4 * FAR, fo=5 * FAR, dtype=2, ws=6 * FAR, wsb=1 << 30):
+        return lib.vl_beam_select(lg, batch, beams, vocab, rs, sc, fin, eos, n_eos, pad, tok, par,
+                                  so, fo, dtype, ws, wsb, None)
+
+    assert call(lg=None) == 2 and "null" in _err(lib)
+    assert call(so=None) == 2 and "null" in _err(lib)
+    assert call(dtype=3) == 2 and "dtype" in _err(lib)
+    for beams in (0, 33):
+        assert call(beams=beams) == 2 and "beams" in _err(lib)
+    assert call(batch=20000) == 2 and "batch" in _err(lib)
+    assert call(vocab=0) == 2 and "vocab" in _err(lib)
+    assert call(vocab=(1 << 24) + 1, rs=1 << 25) == 2 and "vocab" in _err(lib)
+    assert call(rs=999) == 2 and "stride" in _err(lib)
+    assert call(lg=FAR + 1) == 2 and "aligned" in _err(lib)
+    assert call(n_eos=9) == 2 and "n_eos" in _err(lib)
+    assert call(pad=1000) == 2 and "pad_id" in _err(lib)
+    assert call(so=FAKE + 4) == 2 and "overlaps" in _err(lib)
+    assert call(fin=5 * FAR + 1) == 2 and "overlaps" in _err(lib)
+    assert call(wsb=16) == 2 and "workspace" in _err(lib)
+    assert call(batch=0) == 0
+    ws = lib.vl_beam_select_workspace_bytes
+    assert ws(2, 4, 1000) > 0 and ws(0, 4, 1000) == 0 and ws(2, 33, 1000) == 0
+
+
+def test_reorder_rejects(lib):
+    def call(tab=FAR, par=FAKE, kvl=2 * FAR, first=FAKE, pool=32, batch=2, beams=4, mp=8, ts=8,
+             out=3 * FAR, os_=8, ko=4 * FAR, kc=5 * FAR, vc=6 * FAR, layers=2, pages=64, ps=16,
+             row=1024, pstride=16 * 1024, lstride=64 * 16 * 1024):
+        return lib.vl_paged_beam_reorder(tab, par, kvl, first, pool, batch, beams, mp, ts, out,
+                                         os_, ko, kc, vc, layers, pages, ps, row, pstride,
+                                         lstride, None, None)
+
+    assert call(par=None) == 2 and "null" in _err(lib)
+    assert call(kc=None) == 2 and "null" in _err(lib)
+    assert call(beams=33) == 2 and "beams" in _err(lib)
+    assert call(mp=4097, ts=5000, os_=5000) == 2 and "max_pages" in _err(lib)
+    assert call(os_=7) == 2 and "strides" in _err(lib)
+    assert call(pool=16385) == 2 and "pool_pages" in _err(lib)
+    assert call(ps=17) == 2 and "page_size" in _err(lib)
+    assert call(layers=-1) == 2 and "layers" in _err(lib)
+    assert call(row=1023) == 2 and "row_bytes" in _err(lib)
+    assert call(pstride=1024) == 2 and "page_stride_bytes" in _err(lib)
+    assert call(out=FAR) == 2 and "overlap" in _err(lib)
+    assert call(ko=2 * FAR + 4) == 2 and "overlap" in _err(lib)
+    assert call(batch=0) == 0
+
+
+def test_wrappers_refuse_cpu_tensors():
+    x = torch.zeros(4, 8)
+    with pytest.raises(vlasr.VlasrInputError, match="CUDA"):
+        vlasr.beam_select(x, torch.zeros(2, 2))
+    with pytest.raises(vlasr.VlasrInputError, match="CUDA"):
+        vlasr.paged_attention(x, x, x, x, x, x, max_q_len=1)
+    with pytest.raises(vlasr.VlasrInputError, match="CUDA"):
+        vlasr.paged_rope_append(None, x, x, x, x, x, x, x)
+    with pytest.raises(vlasr.VlasrInputError, match="CUDA"):
+        vlasr.paged_beam_reorder(x, x, x, x, 1, x, x)
+
+
+# ---------------------------------------------------------------------------
+# the plain statements themselves
+# ---------------------------------------------------------------------------
+
+def test_plain_rotation_turns_pairs():
+    x = np.array([[1.0, 0.0, 0.0, 0.0, 7.0]])
+    half = paged_ref.rotate(x, 3, 4, 100.0, False, 0.5)
+    assert np.allclose(half, [[math.cos(1.5), 0, math.sin(1.5), 0, 7.0]])
+    inter = paged_ref.rotate(x, 3, 4, 100.0, True, 0.5)
+    assert np.allclose(inter, [[math.cos(1.5), math.sin(1.5), 0, 0, 7.0]])
+    second = paged_ref.rotate(np.array([[0, 1.0, 0, 0]]), 3, 4, 100.0, False, 1.0)
+    assert np.allclose(second, [[0, math.cos(0.3), 0, math.sin(0.3)]])
+
+
+def test_plain_attention_matches_softmax():
+    rng = np.random.default_rng(0)
+    kc, vc = rng.normal(size=(3, 16, 1, 4)), rng.normal(size=(3, 16, 1, 4))
+    q = rng.normal(size=(2, 2, 4))
+    table = np.array([[2, 0]])
+    out, _ = paged_ref.attention(q, kc, vc, [0, 2], [18], table, 0.5, np.zeros((2, 2, 4)), 0.0)
+    K = np.concatenate([kc[2], kc[0]])[:18, 0]
+    V = np.concatenate([vc[2], vc[0]])[:18, 0]
+    s = torch.softmax(torch.from_numpy(q[1] @ K.T * 0.5), -1).numpy()
+    assert np.allclose(out[1], s @ V)
+    s = torch.softmax(torch.from_numpy(q[0] @ K[:17].T * 0.5), -1).numpy()
+    assert np.allclose(out[0], s @ V[:17])
+
+
+def test_plain_select_matches_topk():
+    rng = np.random.default_rng(1)
+    lg = rng.normal(size=(6, 50))
+    sc = -rng.random((2, 3))
+    tok, par, val, _, _ = paged_ref.select(lg, sc, None, (), 0, 3)
+    x = torch.log_softmax(torch.from_numpy(lg), -1).view(2, 3, 50) + torch.from_numpy(sc)[..., None]
+    top = x.view(2, -1).topk(3, -1)
+    assert np.allclose(val, top.values.numpy())
+    assert np.array_equal(par * 50 + tok, top.indices.numpy())
+
+
+def test_plain_reorder_keeps_copies_and_frees():
+    # one entry, three beams, pages of 16; page 0 is the shared prompt
+    kc = np.arange(8 * 16, dtype=np.float64).reshape(1, 8, 16, 1, 1)
+    table = np.array([[0, 3, -1], [0, 4, -1], [0, 5, -1]], np.int32)
+    out, lens, kc2, _, bad = paged_ref.reorder(table, np.array([[1, 1, 0]], np.int32),
+                                               np.array([20, 20, 20], np.int32),
+                                               np.array([3], np.int32), 4, kc, kc)
+    assert out.tolist() == [[0, 4, -1], [0, 5, -1], [0, 3, -1]] and not bad
+    assert lens.tolist() == [20, 20, 20]
+    assert np.array_equal(kc2[0, 5, :4], kc[0, 4, :4])       # the copy
+    assert np.array_equal(kc2[0, 5, 4:], kc[0, 5, 4:])
+    out, _, kc3, _, _ = paged_ref.reorder(table, np.array([[0, 0, 0]], np.int32),
+                                          np.array([16, 16, 16], np.int32),
+                                          np.array([3], np.int32), 4, kc, kc)
+    assert out[:, 1].tolist() == [3, 4, 5] and np.array_equal(kc3, kc)   # fresh pages, no copies

@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -716,6 +717,339 @@ int vl_argmax_eos(const void* logits, int64_t rows, int64_t vocab, int64_t row_s
   a.freeze_id = freeze_id;
   a.status = status;
   return exec_status(vl::launch_argmax_eos(a, dtype, static_cast<cudaStream_t>(stream)), op);
+}
+
+
+// ---------------------------------------------------------------------------
+// paged KV cache and beam search
+// ---------------------------------------------------------------------------
+static bool pow2_in(int64_t x, int64_t lo, int64_t hi) {
+  return x >= lo && x <= hi && (x & (x - 1)) == 0;
+}
+
+// Whether rows of `width` bytes at two row strides share memory, other than
+// by being the same rows.
+static bool rows_clash(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
+                       int64_t rows, int64_t width) {
+  if (rows == 0 || (x == y && x_stride == y_stride)) return false;
+  if (!overlaps(x, (rows - 1) * x_stride + width, y, (rows - 1) * y_stride + width)) return false;
+  if (x_stride != y_stride) return true;
+  // equal strides: apart if they are disjoint columns of one buffer
+  const int64_t off = std::llabs(static_cast<const char*>(x) - static_cast<const char*>(y)) %
+                      x_stride;
+  return off < width || x_stride - off < width;
+}
+
+static int check_pages(const char* op, const void* k_cache, const void* v_cache,
+                       const int32_t* q_start, const int32_t* kv_len, const int32_t* page_table,
+                       int64_t tokens, int64_t batch, int64_t max_pages, int64_t table_stride,
+                       int n_kv_heads, int head_dim, int64_t num_pages, int page_size,
+                       int64_t page_stride) {
+  if (k_cache == nullptr || v_cache == nullptr || q_start == nullptr || kv_len == nullptr ||
+      page_table == nullptr)
+    return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (tokens < 0 || tokens > 0x7fffffff || batch < 0 || batch > (1 << 24) || n_kv_heads <= 0 ||
+      n_kv_heads > 65535 || head_dim <= 0)
+    return fail(VL_ERR_INVALID, "%s: bad shape tokens=%lld batch=%lld kv_heads=%d head_dim=%d", op,
+                static_cast<long long>(tokens), static_cast<long long>(batch), n_kv_heads,
+                head_dim);
+  if (!pow2_in(page_size, 16, 256))
+    return fail(VL_ERR_INVALID, "%s: page_size must be a power of two in [16, 256], got %d", op,
+                page_size);
+  if (num_pages <= 0 || num_pages > 0x7ffffffe || max_pages <= 0 || table_stride < max_pages ||
+      max_pages * page_size > 0x7fffffff)
+    return fail(VL_ERR_INVALID, "%s: bad pages num_pages=%lld max_pages=%lld table_stride=%lld", op,
+                static_cast<long long>(num_pages), static_cast<long long>(max_pages),
+                static_cast<long long>(table_stride));
+  if (page_stride < static_cast<int64_t>(page_size) * n_kv_heads * head_dim)
+    return fail(VL_ERR_INVALID, "%s: page_stride must cover a page", op);
+  return VL_OK;
+}
+
+int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                         void* v_cache, const int32_t* q_start, const int32_t* kv_len,
+                         const int32_t* page_table, int64_t tokens, int64_t batch,
+                         int64_t max_pages, int64_t table_stride, int n_q_heads, int n_kv_heads,
+                         int head_dim, int rotary_dim, int interleaved, double base,
+                         double position_scale, int64_t q_row_stride, int64_t k_row_stride,
+                         int64_t v_row_stride, int64_t q_out_row_stride, int64_t num_pages,
+                         int page_size, int64_t page_stride, int dtype, int32_t* status,
+                         void* stream) {
+  const char* op = "vl_paged_rope_append";
+  const int st = check_pages(op, k_cache, v_cache, q_start, kv_len, page_table, tokens, batch,
+                             max_pages, table_stride, n_kv_heads, head_dim, num_pages, page_size,
+                             page_stride);
+  if (st != VL_OK) return st;
+  if (k == nullptr || v == nullptr) return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
+  if (n_q_heads < 0 || (q == nullptr) != (n_q_heads == 0) ||
+      (q_out == nullptr) != (n_q_heads == 0))
+    return fail(VL_ERR_INVALID, "%s: q and q_out must be null exactly when n_q_heads is 0", op);
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim || rotary_dim > 256)
+    return fail(VL_ERR_INVALID,
+                "%s: rotary_dim must be even, in [0, min(head_dim, 256)] (head_dim=%d "
+                "rotary_dim=%d)", op, head_dim, rotary_dim);
+  if (interleaved != 0 && interleaved != 1)
+    return fail(VL_ERR_INVALID, "%s: interleaved must be 0 or 1", op);
+  if (!(base > 0.0) || !std::isfinite(base) || !(position_scale > 0.0) ||
+      !std::isfinite(position_scale))
+    return fail(VL_ERR_INVALID, "%s: base and position_scale must be finite and > 0", op);
+  const int64_t qw = static_cast<int64_t>(n_q_heads) * head_dim;
+  const int64_t kw = static_cast<int64_t>(n_kv_heads) * head_dim;
+  if (q_row_stride < qw || q_out_row_stride < qw || k_row_stride < kw || v_row_stride < kw)
+    return fail(VL_ERR_INVALID, "%s: row strides must cover heads * head_dim", op);
+  const int64_t es = dtype_size(dtype);
+  if (n_q_heads > 0 &&
+      rows_clash(q_out, q_out_row_stride * es, q, q_row_stride * es, tokens, qw * es))
+    return fail(VL_ERR_INVALID, "%s: q_out overlaps q without being equal to it", op);
+  if (tokens == 0 || batch == 0) return ok();
+  vl::PagedAppendArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.q_start = q_start;
+  a.kv_len = kv_len;
+  a.page_table = page_table;
+  a.tokens = tokens;
+  a.batch = static_cast<int>(batch);
+  a.max_pages = static_cast<int>(max_pages);
+  a.table_stride = table_stride;
+  a.n_q_heads = n_q_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.interleaved = interleaved != 0;
+  a.base = base;
+  a.position_scale = position_scale;
+  a.q_row_stride = q_row_stride;
+  a.k_row_stride = k_row_stride;
+  a.v_row_stride = v_row_stride;
+  a.q_out_row_stride = q_out_row_stride;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.page_stride = page_stride;
+  a.status = status;
+  return exec_status(vl::launch_paged_append(a, dtype, static_cast<cudaStream_t>(stream)), op);
+}
+
+static bool paged_attention_shape(int64_t tokens, int64_t batch, int64_t max_q_len, int n_q_heads,
+                                  int n_kv_heads, int head_dim, int dtype) {
+  return tokens >= 0 && tokens <= 0x7fffffff && batch >= 0 && batch <= (1 << 24) &&
+         max_q_len > 0 && max_q_len <= 0x7fffffff / 2 && n_kv_heads > 0 && n_kv_heads <= 65535 &&
+         n_q_heads > 0 && n_q_heads <= 65535 && n_q_heads % n_kv_heads == 0 &&
+         n_q_heads / n_kv_heads <= 128 && head_dim > 0 && head_dim <= 256 && head_dim % 32 == 0 &&
+         valid_dtype(dtype);
+}
+
+size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
+                                          int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
+  if (!paged_attention_shape(tokens, batch, max_q_len, n_q_heads, n_kv_heads, head_dim, dtype))
+    return 0;
+  return vl::paged_attention_workspace_bytes(tokens, batch, max_q_len, n_q_heads, n_kv_heads,
+                                             head_dim, dtype);
+}
+
+int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* q_start, const int32_t* kv_len, const int32_t* page_table,
+                       int64_t tokens, int64_t batch, int64_t max_q_len, int64_t max_pages,
+                       int64_t table_stride, int n_q_heads, int n_kv_heads, int head_dim,
+                       float scale, int64_t q_row_stride, int64_t out_row_stride,
+                       int64_t num_pages, int page_size, int64_t page_stride, void* out, int dtype,
+                       void* workspace, size_t workspace_bytes, int32_t* status, int flags,
+                       void* stream) {
+  const char* op = "vl_paged_attention";
+  const int st = check_pages(op, k_cache, v_cache, q_start, kv_len, page_table, tokens, batch,
+                             max_pages, table_stride, n_kv_heads, head_dim, num_pages, page_size,
+                             page_stride);
+  if (st != VL_OK) return st;
+  if (q == nullptr || out == nullptr) return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
+  if ((flags & ~VL_LAUNCH_PDL) != 0)
+    return fail(VL_ERR_INVALID, "%s: unknown flags 0x%x", op, flags);
+  if (!paged_attention_shape(tokens, batch, max_q_len, n_q_heads, n_kv_heads, head_dim, dtype))
+    return fail(VL_ERR_INVALID,
+                "%s: unsupported shape: heads %d / %d (a multiple, at most 128 per kv head), "
+                "head_dim %d (a multiple of 32 up to 256), max_q_len %lld", op, n_q_heads,
+                n_kv_heads, head_dim, static_cast<long long>(max_q_len));
+  if (!std::isfinite(scale) || scale < 0.0f)
+    return fail(VL_ERR_INVALID, "%s: scale must be finite and >= 0", op);
+  const int64_t qw = static_cast<int64_t>(n_q_heads) * head_dim;
+  const int64_t E = 16 / dtype_size(dtype);
+  if (q_row_stride < qw || out_row_stride < qw)
+    return fail(VL_ERR_INVALID, "%s: row strides must cover heads * head_dim", op);
+  if (q_row_stride % E || out_row_stride % E || page_stride % E)
+    return fail(VL_ERR_INVALID, "%s: row and page strides must be multiples of %lld elements", op,
+                static_cast<long long>(E));
+  if (!vl::aligned16(q) || !vl::aligned16(out) || !vl::aligned16(k_cache) ||
+      !vl::aligned16(v_cache))
+    return fail(VL_ERR_INVALID, "%s: q, out and the caches must be 16-byte aligned", op);
+  if (tokens == 0 || batch == 0) return ok();
+  const size_t need = vl::paged_attention_workspace_bytes(tokens, batch, max_q_len, n_q_heads,
+                                                          n_kv_heads, head_dim, dtype);
+  if (workspace == nullptr || workspace_bytes < need || !vl::aligned16(workspace))
+    return fail(VL_ERR_INVALID, "%s: workspace of %zu bytes (16-byte aligned) required", op, need);
+  const int64_t es = dtype_size(dtype);
+  const int64_t out_bytes = ((tokens - 1) * out_row_stride + qw) * es;
+  const int64_t cache_bytes =
+      ((num_pages - 1) * page_stride + static_cast<int64_t>(page_size) * n_kv_heads * head_dim) *
+      es;
+  if (overlaps(out, out_bytes, k_cache, cache_bytes) ||
+      overlaps(out, out_bytes, v_cache, cache_bytes) ||
+      rows_clash(out, out_row_stride * es, q, q_row_stride * es, tokens, qw * es))
+    return fail(VL_ERR_INVALID, "%s: out overlaps a cache, or q without being equal to it", op);
+  vl::PagedAttnArgs a{};
+  a.q = q;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.q_start = q_start;
+  a.kv_len = kv_len;
+  a.page_table = page_table;
+  a.out = out;
+  a.tokens = tokens;
+  a.batch = static_cast<int>(batch);
+  a.max_q_len = static_cast<int>(max_q_len);
+  a.max_pages = static_cast<int>(max_pages);
+  a.table_stride = table_stride;
+  a.n_q_heads = n_q_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.head_dim = head_dim;
+  a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(head_dim));
+  a.q_row_stride = q_row_stride;
+  a.out_row_stride = out_row_stride;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.page_stride = page_stride;
+  a.status = status;
+  return exec_status(vl::launch_paged_attention(a, dtype, workspace, (flags & VL_LAUNCH_PDL) != 0,
+                                                static_cast<cudaStream_t>(stream)),
+                     op);
+}
+
+static bool beam_select_shape(int64_t batch, int beams, int64_t vocab) {
+  return batch >= 0 && beams >= 1 && beams <= VL_BEAM_MAX && batch * beams <= 65535 &&
+         vocab >= 1 && vocab <= (int64_t(1) << 24);
+}
+
+size_t vl_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab) {
+  if (batch > 65535 || !beam_select_shape(batch, beams, vocab) || batch == 0) return 0;
+  return vl::beam_select_workspace_bytes(batch, beams, vocab);
+}
+
+int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
+                   int64_t row_stride, const float* scores, const uint8_t* finished,
+                   const int64_t* eos_ids, int n_eos, int64_t pad_id, int64_t* tokens,
+                   int32_t* parents, float* scores_out, uint8_t* finished_out, int dtype,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "vl_beam_select";
+  if (logits == nullptr || scores == nullptr || tokens == nullptr || parents == nullptr ||
+      scores_out == nullptr)
+    return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
+  if (batch > 65535 || !beam_select_shape(batch, beams, vocab))
+    return fail(VL_ERR_INVALID,
+                "%s: beams must be in [1, %d], batch * beams at most 65535, vocab in [1, 2^24] "
+                "(batch=%lld beams=%d vocab=%lld)", op, VL_BEAM_MAX,
+                static_cast<long long>(batch), beams, static_cast<long long>(vocab));
+  if (row_stride < vocab) return fail(VL_ERR_INVALID, "%s: bad row stride", op);
+  const int64_t es = dtype_size(dtype);
+  if (reinterpret_cast<uintptr_t>(logits) % es != 0)
+    return fail(VL_ERR_INVALID, "%s: logits must be aligned to their type", op);
+  if (n_eos < 0 || n_eos > 8 || (n_eos > 0 && eos_ids == nullptr))
+    return fail(VL_ERR_INVALID, "%s: n_eos must be in [0, 8] with eos_ids given", op);
+  if (pad_id < 0 || pad_id >= vocab)
+    return fail(VL_ERR_INVALID, "%s: pad_id must be in [0, vocab)", op);
+  if (batch == 0) return ok();
+  const int64_t n = batch * beams;
+  if ((scores_out != scores && overlaps(scores_out, n * 4, scores, n * 4)) ||
+      (finished_out != nullptr && finished != nullptr && finished_out != finished &&
+       overlaps(finished_out, n, finished, n)))
+    return fail(VL_ERR_INVALID, "%s: an output overlaps its input without being equal to it", op);
+  const size_t need = vl::beam_select_workspace_bytes(batch, beams, vocab);
+  if (workspace == nullptr || workspace_bytes < need || !vl::aligned16(workspace))
+    return fail(VL_ERR_INVALID, "%s: workspace of %zu bytes (16-byte aligned) required", op, need);
+  vl::BeamSelectArgs a{};
+  a.logits = logits;
+  a.batch = batch;
+  a.beams = beams;
+  a.vocab = vocab;
+  a.row_stride = row_stride;
+  a.scores = scores;
+  a.finished = finished;
+  for (int e = 0; e < n_eos; ++e) a.eos[e] = eos_ids[e];
+  a.n_eos = n_eos;
+  a.pad_id = pad_id;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.scores_out = scores_out;
+  a.finished_out = finished_out;
+  return exec_status(
+      vl::launch_beam_select(a, dtype, workspace, static_cast<cudaStream_t>(stream)), op);
+}
+
+int vl_paged_beam_reorder(const int32_t* page_table, const int32_t* parents,
+                          const int32_t* kv_len, const int32_t* pool_start, int64_t pool_pages,
+                          int64_t batch, int beams, int64_t max_pages, int64_t table_stride,
+                          int32_t* table_out, int64_t table_out_stride, int32_t* kv_len_out,
+                          void* k_cache, void* v_cache, int64_t layers, int64_t num_pages,
+                          int page_size, int64_t row_bytes, int64_t page_stride_bytes,
+                          int64_t layer_stride_bytes, int32_t* status, void* stream) {
+  const char* op = "vl_paged_beam_reorder";
+  if (page_table == nullptr || parents == nullptr || kv_len == nullptr || pool_start == nullptr ||
+      table_out == nullptr || kv_len_out == nullptr ||
+      (layers > 0 && (k_cache == nullptr || v_cache == nullptr)))
+    return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (batch < 0 || batch > 65535 || beams < 1 || beams > VL_BEAM_MAX)
+    return fail(VL_ERR_INVALID, "%s: beams must be in [1, %d] and batch at most 65535", op,
+                VL_BEAM_MAX);
+  if (max_pages <= 0 || max_pages > 4096 || table_stride < max_pages ||
+      table_out_stride < max_pages || pool_pages < 0 || pool_pages > 16384)
+    return fail(VL_ERR_INVALID, "%s: max_pages must be in [1, 4096], pool_pages in [0, 16384], "
+                "the table strides at least max_pages", op);
+  if (!pow2_in(page_size, 16, 256))
+    return fail(VL_ERR_INVALID, "%s: page_size must be a power of two in [16, 256], got %d", op,
+                page_size);
+  if (layers < 0 || layers > (1 << 16) || num_pages <= 0 || num_pages > 0x7ffffffe)
+    return fail(VL_ERR_INVALID, "%s: bad caches layers=%lld num_pages=%lld", op,
+                static_cast<long long>(layers), static_cast<long long>(num_pages));
+  if (layers > 0 && (row_bytes <= 0 || row_bytes % 2 != 0 || row_bytes > (1 << 26) ||
+                     page_stride_bytes < page_size * row_bytes || page_stride_bytes % 2 != 0 ||
+                     layer_stride_bytes < 0 || layer_stride_bytes % 2 != 0 ||
+                     reinterpret_cast<uintptr_t>(k_cache) % 2 != 0 ||
+                     reinterpret_cast<uintptr_t>(v_cache) % 2 != 0))
+    return fail(VL_ERR_INVALID, "%s: row_bytes must be even, page_stride_bytes cover a page", op);
+  if (batch == 0) return ok();
+  const int64_t rows = batch * beams;
+  const int64_t in_bytes = ((rows - 1) * table_stride + max_pages) * 4;
+  const int64_t out_bytes = ((rows - 1) * table_out_stride + max_pages) * 4;
+  if (overlaps(table_out, out_bytes, page_table, in_bytes) ||
+      overlaps(kv_len_out, rows * 4, kv_len, rows * 4))
+    return fail(VL_ERR_INVALID, "%s: the new tables and lengths must not overlap the old", op);
+  vl::BeamReorderArgs a{};
+  a.page_table = page_table;
+  a.parents = parents;
+  a.kv_len = kv_len;
+  a.pool_start = pool_start;
+  a.pool_pages = static_cast<int>(pool_pages);
+  a.batch = batch;
+  a.beams = beams;
+  a.max_pages = static_cast<int>(max_pages);
+  a.table_stride = table_stride;
+  a.table_out = table_out;
+  a.table_out_stride = table_out_stride;
+  a.kv_len_out = kv_len_out;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.layers = layers;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.row_bytes = row_bytes;
+  a.page_stride_bytes = page_stride_bytes;
+  a.layer_stride_bytes = layer_stride_bytes;
+  a.status = status;
+  return exec_status(vl::launch_beam_reorder(a, static_cast<cudaStream_t>(stream)), op);
 }
 
 }  // extern "C"

@@ -178,6 +178,119 @@ struct DecodeRowsArgs {
 };
 cudaError_t launch_decode_rows(const DecodeRowsArgs& args, int dtype, cudaStream_t stream);
 
+// Paged KV cache (vl_paged_append.cu, vl_paged_attn.cu, vl_paged_attn_tc.cu).
+struct PagedAppendArgs {
+  const void* q;               // [tokens][q_row_stride] or nullptr
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* q_start;      // [batch + 1]
+  const int32_t* kv_len;       // [batch]
+  const int32_t* page_table;   // [batch][table_stride]
+  int64_t tokens;
+  int batch;
+  int max_pages;
+  int64_t table_stride;
+  int n_q_heads;
+  int n_kv_heads;
+  int head_dim;
+  int rotary_dim;
+  bool interleaved;
+  double base;
+  double position_scale;
+  int64_t q_row_stride;
+  int64_t k_row_stride;
+  int64_t v_row_stride;
+  int64_t q_out_row_stride;
+  int64_t num_pages;
+  int page_size;
+  int64_t page_stride;
+  int32_t* status;
+};
+cudaError_t launch_paged_append(const PagedAppendArgs& args, int dtype, cudaStream_t stream);
+
+struct PagedAttnArgs {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  const int32_t* page_table;
+  void* out;
+  int64_t tokens;
+  int batch;
+  int max_q_len;
+  int max_pages;
+  int64_t table_stride;
+  int n_q_heads;
+  int n_kv_heads;
+  int head_dim;
+  float scale;
+  int64_t q_row_stride;
+  int64_t out_row_stride;
+  int64_t num_pages;
+  int page_size;
+  int64_t page_stride;
+  int32_t* status;
+};
+size_t paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
+                                       int n_q_heads, int n_kv_heads, int head_dim, int dtype);
+cudaError_t launch_paged_attention(const PagedAttnArgs& args, int dtype, void* workspace,
+                                   bool pdl, cudaStream_t stream);
+// The tcgen05 kernel of long chunks (vl_paged_attn_tc.cu).
+size_t paged_attention_tc_workspace_bytes(int64_t tokens, int64_t batch, int n_q_heads,
+                                          int n_kv_heads, int head_dim);
+cudaError_t launch_paged_attention_tc(const PagedAttnArgs& args, int dtype, void* workspace,
+                                      bool pdl, cudaStream_t stream);
+
+// Beam search (vl_beam.cu).
+struct BeamSelectArgs {
+  const void* logits;
+  int64_t batch;
+  int beams;
+  int64_t vocab;
+  int64_t row_stride;
+  const float* scores;
+  const uint8_t* finished;
+  int64_t eos[8];
+  int n_eos;
+  int64_t pad_id;
+  int64_t* tokens;
+  int32_t* parents;
+  float* scores_out;
+  uint8_t* finished_out;
+};
+size_t beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab);
+cudaError_t launch_beam_select(const BeamSelectArgs& args, int dtype, void* workspace,
+                               cudaStream_t stream);
+
+struct BeamReorderArgs {
+  const int32_t* page_table;
+  const int32_t* parents;
+  const int32_t* kv_len;
+  const int32_t* pool_start;
+  int pool_pages;
+  int64_t batch;
+  int beams;
+  int max_pages;
+  int64_t table_stride;
+  int32_t* table_out;
+  int64_t table_out_stride;
+  int32_t* kv_len_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t layers;
+  int64_t num_pages;
+  int page_size;
+  int64_t row_bytes;
+  int64_t page_stride_bytes;
+  int64_t layer_stride_bytes;
+  int32_t* status;
+};
+cudaError_t launch_beam_reorder(const BeamReorderArgs& args, cudaStream_t stream);
+
 // Peer-memory plumbing of the sharded pipeline (vl_peer.cu).
 cudaError_t ipc_export(const void* ptr, void* handle_out, uint64_t* offset_out);
 cudaError_t ipc_open(const void* handle, void** base_out);

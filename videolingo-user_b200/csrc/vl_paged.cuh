@@ -1,0 +1,57 @@
+// Lookups shared by the paged-cache kernels: which sequence a packed row
+// belongs to, and whether a sequence's device-side lengths are usable.
+#pragma once
+
+#include "vl_common.cuh"
+#include "vl_kernels.h"
+
+namespace vl {
+
+__device__ __forceinline__ int ilog2(int pow2) { return 31 - __clz(pow2); }
+
+// The largest b in [0, batch) with q_start[b] <= row, or 0: the sequence of
+// a packed row if any holds it.  Called by a whole warp; 32 probes a round.
+__device__ __forceinline__ int find_sequence(const int32_t* __restrict__ q_start, int batch,
+                                             int64_t row, int lane) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int p = lo + (lane + 1) * step;
+    const bool at_or_before = p < hi && static_cast<int64_t>(q_start[p]) <= row;
+    const int n = __popc(__ballot_sync(0xffffffffu, at_or_before));
+    lo += n * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// A sequence of a ragged batch as the attention kernels see it.
+struct SeqView {
+  int start;   // first packed row
+  int rows;    // new tokens (0: nothing to do)
+  int len;     // cached positions, new tokens included (0: zero output rows)
+  bool bad;    // lengths out of range
+};
+
+__device__ __forceinline__ SeqView sequence_view(const PagedAttnArgs& a, int b, int page_shift) {
+  SeqView s;
+  const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
+  const int len = a.kv_len[b];
+  s.start = q0;
+  s.rows = q1 - q0;
+  s.len = len;
+  s.bad = false;
+  if (q0 < 0 || q1 < q0 || static_cast<int64_t>(q1) > a.tokens) {
+    s.start = 0;   // no rows that could be told to be this sequence's
+    s.rows = 0;
+    s.len = 0;
+    s.bad = true;
+  } else if (len < 0 || static_cast<int64_t>(len) > (static_cast<int64_t>(a.max_pages) << page_shift) ||
+             s.rows > a.max_q_len) {
+    s.len = 0;
+    s.bad = true;
+  }
+  return s;
+}
+
+}  // namespace vl

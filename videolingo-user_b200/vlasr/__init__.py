@@ -6,13 +6,15 @@ the first op call (or by `vlasr.load()`), and fails loudly when it is absent.
 """
 
 from ._lib import (VL_BF16, VL_F16, VL_F32, VL_STATUS_BAD_AUDIO, VL_STATUS_BAD_ID,
-                   VL_STATUS_BAD_SLOT, SIGNATURES, VlasrError, VlasrExecutionError,
-                   VlasrInputError, load)
+                   VL_STATUS_BAD_PAGE, VL_STATUS_BAD_SLOT, VL_STATUS_TIMEOUT, SIGNATURES,
+                   VlasrError, VlasrExecutionError, VlasrInputError, load)
 from .ops import (CHUNK_SAMPLES, MEL_BINS, MEL_FRAMES, add_layernorm, add_rmsnorm,
                   argmax_eos, decode_attention, decode_attention_workspace_bytes, decode_linear,
                   decode_rows,
                   embed_gather, gelu_erf, init,
                   kv_append, logmel, logmel_workspace_bytes, rope_, rope_kv_append, swiglu)
+from .paged import (beam_select, beam_select_workspace_bytes, paged_attention,
+                    paged_attention_workspace_bytes, paged_beam_reorder, paged_rope_append)
 
 __all__ = [
     "VL_BF16", "VL_F16", "VL_F32", "VL_STATUS_BAD_AUDIO", "VL_STATUS_BAD_ID", "VL_STATUS_BAD_SLOT",
@@ -20,5 +22,7 @@ __all__ = [
     "CHUNK_SAMPLES", "MEL_BINS", "MEL_FRAMES", "add_layernorm", "add_rmsnorm", "argmax_eos",
     "decode_attention", "decode_attention_workspace_bytes", "decode_linear", "decode_rows", "embed_gather",
     "gelu_erf", "init", "kv_append", "logmel", "logmel_workspace_bytes", "rope_", "rope_kv_append",
-    "swiglu",
+    "swiglu", "VL_STATUS_BAD_PAGE", "VL_STATUS_TIMEOUT", "beam_select",
+    "beam_select_workspace_bytes", "paged_attention", "paged_attention_workspace_bytes",
+    "paged_beam_reorder", "paged_rope_append",
 ]

@@ -19,6 +19,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libvlasr.so"
 VL_OK, VL_ERR_EXEC, VL_ERR_INVALID = 0, 1, 2
 VL_F32, VL_F16, VL_BF16 = 0, 1, 2
 VL_STATUS_BAD_ID, VL_STATUS_BAD_AUDIO, VL_STATUS_BAD_SLOT = 1, 2, 4
+VL_STATUS_BAD_PAGE, VL_STATUS_TIMEOUT = 8, 16
 VL_IPC_HANDLE_BYTES = 64
 
 # Every symbol the header declares, with (restype, argtypes).
@@ -70,6 +71,21 @@ SIGNATURES = {
                                     c_float, c_int64, c_int64, c_int64, c_int64, c_int64,
                                     c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p,
                                     c_int, c_void_p]),
+    "vl_paged_rope_append": (c_int, [c_void_p] * 9 + [c_int64] * 4 + [c_int] * 5
+                             + [c_double] * 2 + [c_int64] * 5
+                             + [c_int, c_int64, c_int, c_void_p, c_void_p]),
+    "vl_paged_attention_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 4),
+    "vl_paged_attention": (c_int, [c_void_p] * 6 + [c_int64] * 5 + [c_int] * 3 + [c_float]
+                           + [c_int64] * 3 + [c_int, c_int64, c_void_p, c_int, c_void_p,
+                                              c_size_t, c_void_p, c_int, c_void_p]),
+    "vl_beam_select_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
+    "vl_beam_select": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p,
+                               ctypes.POINTER(c_int64), c_int, c_int64, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "vl_paged_beam_reorder": (c_int, [c_void_p] * 4 + [c_int64, c_int64, c_int, c_int64, c_int64,
+                                                       c_void_p, c_int64, c_void_p, c_void_p,
+                                                       c_void_p, c_int64, c_int64, c_int]
+                              + [c_int64] * 3 + [c_void_p, c_void_p]),
 }
 
 
