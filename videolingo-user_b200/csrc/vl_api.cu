@@ -889,6 +889,8 @@ int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
   if (tokens == 0 || batch == 0) return ok();
   const size_t need = vl::paged_attention_workspace_bytes(tokens, batch, max_q_len, n_q_heads,
                                                           n_kv_heads, head_dim, dtype);
+  if (need == 0)
+    return fail(VL_ERR_INVALID, "%s: batch * max_q_len is too large", op);
   if (workspace == nullptr || workspace_bytes < need || !vl::aligned16(workspace))
     return fail(VL_ERR_INVALID, "%s: workspace of %zu bytes (16-byte aligned) required", op, need);
   const int64_t es = dtype_size(dtype);

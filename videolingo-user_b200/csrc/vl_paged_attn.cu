@@ -740,11 +740,14 @@ cudaError_t any_launch(const PagedAttnArgs& a, bool pdl, cudaStream_t stream) {
                        dim3(kAnyWarps * 32), 0, stream, pdl, a);
 }
 
-enum class Kind { kFew, kAny };
+enum class Kind { kFew, kChunk, kAny };
 
+// 16 rows fill two 8-wide MMA columns of the few-token kernel, which
+// streams the cache at HBM's rate; from there on the tcgen05 kernel's 128-row
+// blocks re-read it less often.
 Kind paged_kind(int64_t max_q_len, int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
   if (dtype == kDtypeF32 || (head_dim != 64 && head_dim != 128)) return Kind::kAny;
-  return max_q_len * (n_q_heads / n_kv_heads) <= kFewRows ? Kind::kFew : Kind::kAny;
+  return max_q_len * (n_q_heads / n_kv_heads) <= kFewRows ? Kind::kFew : Kind::kChunk;
 }
 
 }  // namespace
@@ -790,9 +793,13 @@ bool encode_rows_map(CUtensorMap* map, const void* rows, bool bf16, int head_dim
 
 size_t paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
                                        int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
-  if (paged_kind(max_q_len, n_q_heads, n_kv_heads, head_dim, dtype) == Kind::kFew)
-    return few_workspace(batch, head_dim);
-  return 16;
+  switch (paged_kind(max_q_len, n_q_heads, n_kv_heads, head_dim, dtype)) {
+    case Kind::kFew: return few_workspace(batch, head_dim);
+    case Kind::kChunk:
+      return paged_attention_tc_workspace_bytes(tokens, batch, max_q_len, n_q_heads, n_kv_heads,
+                                                head_dim);
+    default: return 16;
+  }
 }
 
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, void* workspace, bool pdl,
@@ -802,6 +809,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, void* work
     case Kind::kFew:
       return dtype == kDtypeBF16 ? few_typed<__nv_bfloat16>(a, workspace, pdl, stream)
                                  : few_typed<__half>(a, workspace, pdl, stream);
+    case Kind::kChunk: return launch_paged_attention_tc(a, dtype, workspace, pdl, stream);
     default:
       if (dtype == kDtypeF32) return any_launch<float>(a, pdl, stream);
       return dtype == kDtypeF16 ? any_launch<__half>(a, pdl, stream)
