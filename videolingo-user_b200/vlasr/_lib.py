@@ -108,6 +108,8 @@ _lib: ctypes.CDLL | None = None
 def load(path: Path | str | None = None) -> ctypes.CDLL:
     """Load libvlasr.so (once) and attach the prototypes."""
     global _lib
+    if path is None and _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -26,8 +26,8 @@ VL_STATUS_BAD_PAGE in `status` (an int32 tensor), if given.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -38,42 +38,71 @@ from .ops import LAUNCH_PDL
 BEAM_MAX = 32
 
 _CODES = {torch.float32: VL_F32, torch.float16: VL_F16, torch.bfloat16: VL_BF16}
+_I32, _I64, _F32, _BOOL, _U8 = (torch.int32, torch.int64, torch.float32, torch.bool, torch.uint8)
+
+# A decode step makes these calls once per layer, so the checks are written to
+# cost as few tensor-attribute reads as they can.
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:      # a build of torch without them
+    def _raw_stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
+
+    _current_device = torch.cuda.current_device
 
 
-def _code(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor):
-        raise VlasrInputError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+def _operator(fn):
+    """Launches go to the tensors' device, whatever the current one is (the
+    first CUDA tensor among the arguments names it), and an argument that is
+    no tensor is an input error."""
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        try:
+            return fn(*args, **kwargs)
+        except _OtherDevice as e:
+            with torch.cuda.device(e.device):
+                return fn(*args, **kwargs)
+        except AttributeError as e:
+            raise VlasrInputError(f"{fn.__name__}: an argument is not a torch.Tensor ({e})") from e
+    return call
+
+
+class _OtherDevice(Exception):
+    def __init__(self, device: int):
+        self.device = device
+
+
+def _lead(t: torch.Tensor, name: str) -> tuple[int, torch.dtype, int]:
+    """dtype code, dtype and device of the tensor the others must match."""
+    dev = t.get_device()
+    if dev < 0:
         raise VlasrInputError(f"{name} must be a CUDA tensor (there is no CPU path)")
-    code = _CODES.get(t.dtype)
+    dt = t.dtype
+    code = _CODES.get(dt)
     if code is None:
-        raise VlasrInputError(f"unsupported dtype {t.dtype}; expected float32/float16/bfloat16")
-    return code
+        raise VlasrInputError(f"unsupported dtype {dt}; expected float32/float16/bfloat16")
+    if dev != _current_device():
+        raise _OtherDevice(dev)
+    return code, dt, dev
 
 
-def _like(ref: torch.Tensor, t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != ref.dtype or t.device != ref.device:
-        raise VlasrInputError(f"{name} must match dtype/device {ref.dtype}/{ref.device}")
+def _like(t: torch.Tensor, dt: torch.dtype, dev: int, name: str) -> None:
+    if t.dtype is not dt or t.get_device() != dev:
+        raise VlasrInputError(f"{name} must match dtype/device {dt}/cuda:{dev}")
 
 
-def _ints(ref: torch.Tensor, t: torch.Tensor, name: str, dtype=torch.int32) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != ref.device:
-        raise VlasrInputError(f"{name} must be {dtype} on {ref.device}")
+def _packed(t: torch.Tensor, dt: torch.dtype, dev: int, name: str) -> None:
+    if t.dtype is not dt or t.get_device() != dev:
+        raise VlasrInputError(f"{name} must be {dt} on cuda:{dev}")
     if not t.is_contiguous():
         raise VlasrInputError(f"{name} must be contiguous")
 
 
-def _on(device: torch.device):
-    """Launches go to the tensors' device, whatever the current one is."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _status_ptr(ref: torch.Tensor, status: torch.Tensor | None) -> int | None:
+def _status_ptr(status: torch.Tensor | None, dev: int) -> int | None:
     if status is None:
         return None
-    _ints(ref, status, "status")
+    _packed(status, _I32, dev, "status")
     if status.numel() < 1:
         raise VlasrInputError("status must hold one int32")
     return status.data_ptr()
@@ -82,18 +111,19 @@ def _status_ptr(ref: torch.Tensor, status: torch.Tensor | None) -> int | None:
 def _head_rows(t: torch.Tensor, head_dim: int, name: str) -> tuple[int, int, int]:
     """[tokens, heads, head_dim] or [tokens, heads * head_dim] -> tokens, heads, row stride."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 3:
-        if shape[2] != head_dim or stride[2] != 1 or (stride[1] != head_dim and shape[1] != 1):
-            raise VlasrInputError(f"{name} must be [tokens, heads, {head_dim}] with packed heads")
-        tokens, heads = shape[0], shape[1]
-    elif len(shape) == 2:
-        if shape[1] % head_dim or stride[1] != 1:
+    if len(shape) == 2:
+        tokens, width = shape
+        if width % head_dim or stride[1] != 1:
             raise VlasrInputError(f"{name} must be [tokens, heads * {head_dim}] with contiguous rows")
-        tokens, heads = shape[0], shape[1] // head_dim
+    elif len(shape) == 3:
+        tokens, heads, hd = shape
+        if hd != head_dim or stride[2] != 1 or (stride[1] != head_dim and heads != 1):
+            raise VlasrInputError(f"{name} must be [tokens, heads, {head_dim}] with packed heads")
+        width = heads * hd
     else:
         raise VlasrInputError(f"{name} must be [tokens, heads, head_dim] or [tokens, heads * head_dim]")
     # one row may carry any stride
-    return tokens, heads, stride[0] if tokens > 1 else max(stride[0], heads * head_dim)
+    return tokens, width // head_dim, stride[0] if tokens > 1 else max(stride[0], width)
 
 
 def _cache_pages(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int, int]:
@@ -109,22 +139,23 @@ def _cache_pages(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int
         stride[0], page_size * heads * hd)
 
 
-def _batch(ref, q_start, kv_len, page_table) -> tuple[int, int, int]:
+def _batch(dev, q_start, kv_len, page_table) -> tuple[int, int, int]:
     """batch, max_pages and row stride of the page table."""
-    _ints(ref, q_start, "q_start")
-    _ints(ref, kv_len, "kv_len")
+    _packed(q_start, _I32, dev, "q_start")
+    _packed(kv_len, _I32, dev, "kv_len")
     batch = kv_len.numel()
-    if kv_len.dim() != 1 or q_start.dim() != 1 or q_start.numel() != batch + 1:
+    if q_start.numel() != batch + 1 or kv_len.dim() != 1 or q_start.dim() != 1:
         raise VlasrInputError("q_start must be [batch + 1] and kv_len [batch]")
-    if (not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32
-            or page_table.device != ref.device or page_table.dim() != 2
-            or page_table.shape[0] != batch or page_table.stride(1) != 1):
+    shape = page_table.shape
+    if (page_table.dtype is not _I32 or page_table.get_device() != dev or len(shape) != 2
+            or shape[0] != batch or page_table.stride(1) != 1):
         raise VlasrInputError("page_table must be int32 [batch, max_pages] with contiguous rows")
-    max_pages = page_table.shape[1]
+    max_pages = shape[1]
     return batch, max_pages, page_table.stride(0) if batch > 1 else max(page_table.stride(0),
                                                                         max_pages)
 
 
+@_operator
 def paged_rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
                       k_cache: torch.Tensor, v_cache: torch.Tensor, q_start: torch.Tensor,
                       kv_len: torch.Tensor, page_table: torch.Tensor, *,
@@ -141,9 +172,10 @@ def paged_rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     (0: none) in pairs (d, d + rotary_dim/2), or (2d, 2d + 1) with interleaved,
     by position * position_scale * base^(-2d/rotary_dim).  q None only
     appends."""
-    code = _code(k, "k")
-    for name, t in (("v", v), ("k_cache", k_cache), ("v_cache", v_cache)):
-        _like(k, t, name)
+    code, dt, dev = _lead(k, "k")
+    _like(v, dt, dev, "v")
+    _like(k_cache, dt, dev, "k_cache")
+    _like(v_cache, dt, dev, "v_cache")
     num_pages, page_size, kvh, hd, page_stride = _cache_pages(k_cache, v_cache)
     if head_dim is not None and head_dim != hd:
         raise VlasrInputError(f"head_dim {head_dim} is not the cache's ({hd})")
@@ -151,31 +183,30 @@ def paged_rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     vt, vh, vs = _head_rows(v, hd, "v")
     if kh != kvh or vh != kvh or vt != tokens:
         raise VlasrInputError("k and v must have one row per token and the cache's heads")
-    batch, max_pages, table_stride = _batch(k, q_start, kv_len, page_table)
+    batch, max_pages, table_stride = _batch(dev, q_start, kv_len, page_table)
     nq = qs = os_ = 0
     q_ptr = out_ptr = None
     if q is not None:
-        _like(k, q, "q")
+        _like(q, dt, dev, "q")
         qt, nq, qs = _head_rows(q, hd, "q")
         if q_out is None:
-            q_out = torch.empty((tokens, nq * hd), dtype=q.dtype, device=q.device)
-        _like(k, q_out, "q_out")
+            q_out = torch.empty((tokens, nq * hd), dtype=dt, device=q.device)
+        else:
+            _like(q_out, dt, dev, "q_out")
         ot, oh, os_ = _head_rows(q_out, hd, "q_out")
         if qt != tokens or ot != tokens or oh != nq:
             raise VlasrInputError("q and q_out must have one row per token and the same heads")
         q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise VlasrInputError("q_out needs q")
-    if rotary_dim is None:
-        rotary_dim = hd
-    with _on(k.device):
-        check(_lib.load().vl_paged_rope_append(
-            q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
-            q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), tokens, batch,
-            max_pages, table_stride, nq, kvh, hd, rotary_dim, 1 if interleaved else 0, base,
-            position_scale, qs, ks, vs, os_, num_pages, page_size, page_stride, code,
-            _status_ptr(k, status), torch.cuda.current_stream().cuda_stream),
-            "vl_paged_rope_append")
+    rc = _lib.load().vl_paged_rope_append(
+        q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
+        q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), tokens, batch, max_pages,
+        table_stride, nq, kvh, hd, hd if rotary_dim is None else rotary_dim,
+        1 if interleaved else 0, base, position_scale, qs, ks, vs, os_, num_pages, page_size,
+        page_stride, code, _status_ptr(status, dev), _raw_stream(dev))
+    if rc:
+        check(rc, "vl_paged_rope_append")
     return q_out
 
 
@@ -186,17 +217,18 @@ def paged_attention_workspace_bytes(tokens: int, batch: int, max_q_len: int, n_q
         tokens, batch, max_q_len, n_q_heads, n_kv_heads, head_dim, _CODES[dtype]))
 
 
-def _workspace(ref: torch.Tensor, workspace: torch.Tensor | None, need: int) -> torch.Tensor:
-    """The caller's workspace, or one of the call's own from the allocator
-    (stream-ordered, and inside a capture the graph's)."""
+def _workspace(device: torch.device, dev: int, workspace: torch.Tensor | None,
+               need: int) -> tuple[torch.Tensor, int]:
+    """The caller's workspace and its bytes, or one of the call's own from the
+    allocator (stream-ordered, and inside a capture the graph's)."""
     if workspace is None:
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=ref.device)
-    if (not isinstance(workspace, torch.Tensor) or workspace.device != ref.device
-            or not workspace.is_contiguous()):
-        raise VlasrInputError(f"workspace must be a contiguous tensor on {ref.device}")
-    return workspace
+        return torch.empty(max(need, 16), dtype=_U8, device=device), need
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise VlasrInputError(f"workspace must be a contiguous tensor on cuda:{dev}")
+    return workspace, workspace.numel() * workspace.element_size()
 
 
+@_operator
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, *,
                     max_q_len: int, scale: float = 0.0, out: torch.Tensor | None = None,
@@ -212,29 +244,31 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the call takes its own.  pdl=True launches it as a programmatic dependent
     of the previous kernel on the stream (VL_LAUNCH_PDL): that kernel must
     not write q_start, kv_len or page_table."""
-    code = _code(q, "q")
-    _like(q, k_cache, "k_cache")
-    _like(q, v_cache, "v_cache")
+    code, dt, dev = _lead(q, "q")
+    _like(k_cache, dt, dev, "k_cache")
+    _like(v_cache, dt, dev, "v_cache")
     num_pages, page_size, kvh, hd, page_stride = _cache_pages(k_cache, v_cache)
     tokens, nq, qs = _head_rows(q, hd, "q")
-    batch, max_pages, table_stride = _batch(q, q_start, kv_len, page_table)
+    batch, max_pages, table_stride = _batch(dev, q_start, kv_len, page_table)
+    device = q.device
     if out is None:
-        out = torch.empty((tokens, nq * hd), dtype=q.dtype, device=q.device)
-    _like(q, out, "out")
+        out = torch.empty((tokens, nq * hd), dtype=dt, device=device)
+    else:
+        _like(out, dt, dev, "out")
     ot, oh, os_ = _head_rows(out, hd, "out")
     if ot != tokens or oh != nq:
         raise VlasrInputError("out must have q's rows and heads")
     lib = _lib.load()
-    with _on(q.device):
-        need = lib.vl_paged_attention_workspace_bytes(tokens, batch, max_q_len, nq, kvh, hd, code)
-        ws = _workspace(q, workspace, need)
-        check(lib.vl_paged_attention(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(),
-            kv_len.data_ptr(), page_table.data_ptr(), tokens, batch, max_q_len, max_pages,
-            table_stride, nq, kvh, hd, scale, qs, os_, num_pages, page_size, page_stride,
-            out.data_ptr(), code, ws.data_ptr(), ws.numel() * ws.element_size(),
-            _status_ptr(q, status), LAUNCH_PDL if pdl else 0,
-            torch.cuda.current_stream().cuda_stream), "vl_paged_attention")
+    ws, ws_bytes = _workspace(device, dev, workspace, lib.vl_paged_attention_workspace_bytes(
+        tokens, batch, max_q_len, nq, kvh, hd, code))
+    rc = lib.vl_paged_attention(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(),
+        kv_len.data_ptr(), page_table.data_ptr(), tokens, batch, max_q_len, max_pages,
+        table_stride, nq, kvh, hd, scale, qs, os_, num_pages, page_size, page_stride,
+        out.data_ptr(), code, ws.data_ptr(), ws_bytes, _status_ptr(status, dev),
+        LAUNCH_PDL if pdl else 0, _raw_stream(dev))
+    if rc:
+        check(rc, "vl_paged_attention")
     return out
 
 
@@ -242,6 +276,7 @@ def beam_select_workspace_bytes(batch: int, beams: int, vocab: int) -> int:
     return int(_lib.load().vl_beam_select_workspace_bytes(batch, beams, vocab))
 
 
+@_operator
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
                 finished: torch.Tensor | None = None, eos_ids=(), pad_id: int = 0,
                 tokens: torch.Tensor | None = None, parents: torch.Tensor | None = None,
@@ -258,50 +293,50 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
     beam * vocab + token.  Returns (tokens int64, parents int32, scores
     float32, finished bool), each [batch, beams]; scores_out may be scores and
     finished_out may be finished."""
-    code = _code(logits, "logits")
+    code, _, dev = _lead(logits, "logits")
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise VlasrInputError("logits must be a 2-D tensor with contiguous rows")
-    _ints(logits, scores, "scores", torch.float32)
-    if scores.dim() != 2:
-        raise VlasrInputError("scores must be [batch, beams]")
+    _packed(scores, _F32, dev, "scores")
     shape = scores.shape
+    if len(shape) != 2:
+        raise VlasrInputError("scores must be [batch, beams]")
     batch, beams = shape
     rows, vocab = logits.shape
     if rows != batch * beams:
         raise VlasrInputError("logits must have batch * beams rows")
-    dev = logits.device
+    device = logits.device
 
     def place(t, name, dtype):
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=dev)
-        if dtype is torch.bool and isinstance(t, torch.Tensor) and t.dtype == torch.uint8:
-            dtype = torch.uint8
-        _ints(logits, t, name, dtype)
+            return torch.empty(shape, dtype=dtype, device=device)
+        _packed(t, _U8 if dtype is _BOOL and t.dtype is _U8 else dtype, dev, name)
         if t.shape != shape:
             raise VlasrInputError(f"{name} must be [batch, beams]")
         return t
 
     if finished is not None:
-        place(finished, "finished", torch.bool)
-    tokens = place(tokens, "tokens", torch.int64)
-    parents = place(parents, "parents", torch.int32)
-    scores_out = place(scores_out, "scores_out", torch.float32)
-    finished_out = place(finished_out, "finished_out", torch.bool)
+        place(finished, "finished", _BOOL)
+    tokens = place(tokens, "tokens", _I64)
+    parents = place(parents, "parents", _I32)
+    scores_out = place(scores_out, "scores_out", _F32)
+    finished_out = place(finished_out, "finished_out", _BOOL)
     n_eos = len(eos_ids)
     eos = (ctypes.c_int64 * max(n_eos, 1))(*eos_ids)
     lib = _lib.load()
-    with _on(dev):
-        ws = _workspace(logits, workspace, lib.vl_beam_select_workspace_bytes(batch, beams, vocab))
-        check(lib.vl_beam_select(
-            logits.data_ptr(), batch, beams, vocab,
-            logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
-            None if finished is None else finished.data_ptr(), eos, n_eos, pad_id,
-            tokens.data_ptr(), parents.data_ptr(), scores_out.data_ptr(),
-            finished_out.data_ptr(), code, ws.data_ptr(), ws.numel() * ws.element_size(),
-            torch.cuda.current_stream().cuda_stream), "vl_beam_select")
+    ws, ws_bytes = _workspace(device, dev, workspace,
+                              lib.vl_beam_select_workspace_bytes(batch, beams, vocab))
+    rc = lib.vl_beam_select(
+        logits.data_ptr(), batch, beams, vocab,
+        logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
+        None if finished is None else finished.data_ptr(), eos, n_eos, pad_id,
+        tokens.data_ptr(), parents.data_ptr(), scores_out.data_ptr(), finished_out.data_ptr(),
+        code, ws.data_ptr(), ws_bytes, _raw_stream(dev))
+    if rc:
+        check(rc, "vl_beam_select")
     return tokens, parents, scores_out, finished_out
 
 
+@_operator
 def paged_beam_reorder(page_table: torch.Tensor, parents: torch.Tensor, kv_len: torch.Tensor,
                        pool_start: torch.Tensor, pool_pages: int, k_cache: torch.Tensor,
                        v_cache: torch.Tensor, *, out: torch.Tensor | None = None,
@@ -318,56 +353,58 @@ def paged_beam_reorder(page_table: torch.Tensor, parents: torch.Tensor, kv_len: 
     pool_start[e] .. + pool_pages - 1 with the rows so far copied in every
     layer.  The old tables are only read; `out` and `kv_len_out` must be other
     tensors."""
-    _code(k_cache, "k_cache")
-    _like(k_cache, v_cache, "v_cache")
+    _, dt, dev = _lead(k_cache, "k_cache")
+    _like(v_cache, dt, dev, "v_cache")
     shape, stride = k_cache.shape, k_cache.stride()
-    if len(shape) == 4:
-        shape, stride = (1,) + tuple(shape), (0,) + tuple(stride)
-    if len(shape) != 5 or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+    if v_cache.shape != shape or v_cache.stride() != stride or len(shape) not in (4, 5):
         raise VlasrInputError("k_cache and v_cache must be [layers, num_pages, page_size, "
                               "kv_heads, head_dim] of the same shape and strides")
+    if len(shape) == 4:
+        shape, stride = (1, *shape), (0, *stride)
     layers, num_pages, page_size, kvh, hd = shape
     row = kvh * hd
     if stride[4] != 1 or (stride[3] != hd and kvh != 1) or stride[2] != row:
         raise VlasrInputError("the rows of a cache page must be contiguous")
-    _ints(k_cache, parents, "parents")
+    _packed(parents, _I32, dev, "parents")
     if parents.dim() != 2:
         raise VlasrInputError("parents must be [batch, beams]")
     batch, beams = parents.shape
     rows = batch * beams
-    _ints(k_cache, kv_len, "kv_len")
-    _ints(k_cache, pool_start, "pool_start")
+    _packed(kv_len, _I32, dev, "kv_len")
+    _packed(pool_start, _I32, dev, "pool_start")
     if kv_len.numel() != rows or pool_start.numel() != batch:
         raise VlasrInputError("kv_len must be [batch * beams] and pool_start [batch]")
 
-    def table(t, name):
-        if (not isinstance(t, torch.Tensor) or t.dtype != torch.int32
-                or t.device != k_cache.device or t.dim() != 2 or t.shape[0] != rows
+    def row_stride(t, name):
+        if (t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 or t.shape[0] != rows
                 or t.stride(1) != 1):
             raise VlasrInputError(f"{name} must be int32 [batch * beams, max_pages] with "
                                   "contiguous rows")
         return t.stride(0) if rows > 1 else max(t.stride(0), t.shape[1])
 
-    table_stride = table(page_table, "page_table")
+    table_stride = row_stride(page_table, "page_table")
     max_pages = page_table.shape[1]
+    device = k_cache.device
     if out is None:
-        out = torch.empty((rows, max_pages), dtype=torch.int32, device=k_cache.device)
-    out_stride = table(out, "out")
-    if out.shape[1] != max_pages:
-        raise VlasrInputError("out must have page_table's shape")
+        out, out_stride = torch.empty((rows, max_pages), dtype=_I32, device=device), max_pages
+    else:
+        out_stride = row_stride(out, "out")
+        if out.shape[1] != max_pages:
+            raise VlasrInputError("out must have page_table's shape")
     if kv_len_out is None:
-        kv_len_out = torch.empty(rows, dtype=torch.int32, device=k_cache.device)
-    _ints(k_cache, kv_len_out, "kv_len_out")
-    if kv_len_out.numel() != rows:
-        raise VlasrInputError("kv_len_out must be [batch * beams]")
+        kv_len_out = torch.empty(rows, dtype=_I32, device=device)
+    else:
+        _packed(kv_len_out, _I32, dev, "kv_len_out")
+        if kv_len_out.numel() != rows:
+            raise VlasrInputError("kv_len_out must be [batch * beams]")
     es = k_cache.element_size()
     page_stride = stride[1] if num_pages > 1 else max(stride[1], page_size * row)
-    with _on(k_cache.device):
-        check(_lib.load().vl_paged_beam_reorder(
-            page_table.data_ptr(), parents.data_ptr(), kv_len.data_ptr(), pool_start.data_ptr(),
-            pool_pages, batch, beams, max_pages, table_stride, out.data_ptr(), out_stride,
-            kv_len_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), layers, num_pages,
-            page_size, row * es, page_stride * es, stride[0] * es,
-            _status_ptr(k_cache, status), torch.cuda.current_stream().cuda_stream),
-            "vl_paged_beam_reorder")
+    rc = _lib.load().vl_paged_beam_reorder(
+        page_table.data_ptr(), parents.data_ptr(), kv_len.data_ptr(), pool_start.data_ptr(),
+        pool_pages, batch, beams, max_pages, table_stride, out.data_ptr(), out_stride,
+        kv_len_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), layers, num_pages,
+        page_size, row * es, page_stride * es, stride[0] * es, _status_ptr(status, dev),
+        _raw_stream(dev))
+    if rc:
+        check(rc, "vl_paged_beam_reorder")
     return out, kv_len_out
