@@ -247,9 +247,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
   Cursor c = few_locate(a, shift, lane, before, u0);
 
   if (warp == kFewWarps) {
-    // ---- producer: lane l fetches the l-th (page, column) box of K and V ----
+    // ---- producer ----
     const int box_rows = 1 << box_shift;
-    const int boxes_k = kFewTile >> box_shift;        // page pieces of a tile
     int stage = 0;
     uint32_t phase = 0;
     int64_t issued = 0;
@@ -257,15 +256,13 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       while (u >= c.base + static_cast<int64_t>(c.tiles) * a.n_kv_heads) few_next(a, shift, c);
       const int local = static_cast<int>(u - c.base);
       const int h = local / c.tiles, tile = local - h * c.tiles;
-      const int need = (min(kFewTile, c.s.len - tile * kFewTile) + box_rows - 1) >> box_shift;
-      // page ids before the wait for the stage
-      const int piece = lane / kHalves, half = lane % kHalves;
-      int page = -1, row = 0;
-      if (piece < need && piece < boxes_k) {
-        const int64_t p = static_cast<int64_t>(tile) * kFewTile + (static_cast<int64_t>(piece) << box_shift);
-        page = a.page_table[c.b * a.table_stride + (p >> shift)];
-        row = static_cast<int>(p) & (a.page_size - 1);
-        if (page < 0 || page >= a.num_pages) {        // read as rows of zeros
+      const int pos0 = tile * kFewTile;
+      const int need = (min(kFewTile, c.s.len - pos0) + box_rows - 1) >> box_shift;
+      // lane l looks up the l-th box's page, before the wait for the stage
+      int page = 0;
+      if (lane < need) {
+        page = a.page_table[c.b * a.table_stride + ((pos0 + (lane << box_shift)) >> shift)];
+        if (page < 0 || page >= a.num_pages) {          // read as rows of zeros
           page = static_cast<int>(a.num_pages);
           if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
         }
@@ -274,13 +271,22 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
         if (lane == 0) atomicExch(&sm.bad, 1);
         break;
       }
-      if (lane == 0)
+      if (elect_lane())
         mbarrier_expect(&sm.full[stage], static_cast<uint32_t>(need) * box_rows * 128 * kHalves * 2);
       __syncwarp();
-      if (page >= 0) {
-        const uint32_t dst = ring + stage * kStage + half * kColumn + piece * box_rows * 128;
-        tma_load_4d(dst, &kmap, half * 64, h, row, page, &sm.full[stage]);
-        tma_load_4d(dst + kMatrix, &vmap, half * 64, h, row, page, &sm.full[stage]);
+      for (int j = 0; j < need; ++j) {
+        const int pj = __shfl_sync(0xffffffffu, page, j);
+        const uint32_t dst = ring + stage * kStage + j * box_rows * 128;
+        const int row = (pos0 + (j << box_shift)) & (a.page_size - 1);
+        if (elect_lane()) {
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+            tma_load_4d(dst + half * kColumn, &kmap, half * 64, h, row, pj, &sm.full[stage]);
+            tma_load_4d(dst + half * kColumn + kMatrix, &vmap, half * 64, h, row, pj,
+                        &sm.full[stage]);
+          }
+        }
+        __syncwarp();
       }
       ++issued;
       if (++stage == kFewStages) {

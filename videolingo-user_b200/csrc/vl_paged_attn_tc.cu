@@ -66,7 +66,7 @@ struct Shape {
 struct Bars {
   uint64_t q_full, q_empty;
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_ready[2], o_done[2];
+  uint64_t s_full[2], p_half[2], p_ready[2], o_done[2];
   uint64_t end;
   uint32_t tmem;
   int bad;
@@ -207,13 +207,32 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
       "r"(r[30]), "r"(r[31]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
 // Loads issued so far have arrived; ties the registers to the wait, so that
 // no use of them moves above it.
 template <int N>
-__device__ __forceinline__ void tmem_load_wait(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_tie(uint32_t* r) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_load_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  tmem_tie<N>(r);
+}
+// Scores from `seen` on become -inf.
+template <int N>
+__device__ __forceinline__ void hide(uint32_t* r, int seen) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i >= seen) r[i] = 0xff800000u;
 }
 __device__ __forceinline__ void tmem_store_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -221,6 +240,39 @@ __device__ __forceinline__ void tmem_store_wait() {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;"
+      : "=f"(y)
+      : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return y;
+}
+// two floats in one 64-bit register, for the packed adds and multiply-adds
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ float2 halves_of(uint64_t x) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
   return y;
 }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
@@ -258,7 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&bars.s_full[i], 1);
-      mbarrier_init(&bars.p_ready[i], kSoftThreads / 64);   // a block's warps
+      mbarrier_init(&bars.p_half[i], kSoftThreads / 64);    // a block's warps
+      mbarrier_init(&bars.p_ready[i], kSoftThreads / 64);
       mbarrier_init(&bars.o_done[i], 1);
     }
     mbarrier_init(&bars.end, 1);
@@ -284,18 +337,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- copies: Q of a piece, then its K and V tiles in turn ----
     const int box_rows = 1 << box_shift;
     uint32_t tile = 0, item = 0;          // tiles and pieces so far
-    const int part = lane / L::kHalves, half = lane % L::kHalves;
     bool ok = true;
     for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
       const Piece p = piece_of(a, w, index, shift, G);
       const int n = max(p.count[0], p.count[1]);
       if (n == 0) continue;
       if (item > 0 && !wait_or_bad(&bars.q_empty, (item - 1) & 1, &bars.bad)) break;
-      if (lane == 0) {
+      if (elect_lane()) {
         const uint32_t bytes = L::kHalves * 128 * G * p.rows_tok;
         mbarrier_expect(&bars.q_full, bytes * ((p.count[0] > 0) + (p.count[1] > 0)));
+#pragma unroll
         for (int i = 0; i < 2; ++i)
           if (p.count[i] > 0)
+#pragma unroll
             for (int c = 0; c < L::kHalves; ++c)
               tma_load_3d(base + L::kQ + i * L::kMatrix + c * L::kColumn, &qmap, c * 64, p.h * G,
                           p.s.start + p.tok0 + i * p.rows_tok, &bars.q_full);
@@ -305,11 +359,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int jj = 0; jj < n; ++jj, ++tile) {
         const int pos0 = (p.j0 + jj) * kTile;
         const int need = (min(kTile, p.s.len - pos0) + box_rows - 1) >> box_shift;
-        int page = -1, row = 0;
-        if (part < need) {
-          const int pos = pos0 + (part << box_shift);
-          page = a.page_table[p.b * a.table_stride + (pos >> shift)];
-          row = pos & (a.page_size - 1);
+        // lane l looks up the l-th box's page, all before the waits
+        int page = 0;
+        if (lane < need) {
+          page = a.page_table[p.b * a.table_stride + ((pos0 + (lane << box_shift)) >> shift)];
           if (page < 0 || page >= a.num_pages) {       // read as rows of zeros
             page = static_cast<int>(a.num_pages);
             if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
@@ -318,23 +371,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = tile % kStages;
         const uint32_t parity = ((tile / kStages) & 1) ^ 1;
         const uint32_t bytes = static_cast<uint32_t>(need) * box_rows * 128 * L::kHalves;
-        const uint32_t at = st * L::kMatrix + half * L::kColumn + part * box_rows * 128;
+        auto fetch = [&](uint32_t matrix, const CUtensorMap* map, uint64_t* full) {
+          if (elect_lane()) mbarrier_expect(full, bytes);
+          __syncwarp();
+          for (int j = 0; j < need; ++j) {
+            const int pj = __shfl_sync(0xffffffffu, page, j);
+            const uint32_t dst = matrix + st * L::kMatrix + j * box_rows * 128;
+            const int row = (pos0 + (j << box_shift)) & (a.page_size - 1);
+            if (elect_lane()) {
+#pragma unroll
+              for (int c = 0; c < L::kHalves; ++c)
+                tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pj, full);
+            }
+            __syncwarp();
+          }
+        };
         if (tile >= kStages && !wait_or_bad(&bars.k_empty[st], parity, &bars.bad)) {
           ok = false;
           break;
         }
-        if (lane == 0) mbarrier_expect(&bars.k_full[st], bytes);
-        __syncwarp();
-        if (page >= 0)
-          tma_load_4d(base + L::kK + at, &kmap, half * 64, p.h, row, page, &bars.k_full[st]);
+        fetch(base + L::kK, &kmap, &bars.k_full[st]);
         if (tile >= kStages && !wait_or_bad(&bars.v_empty[st], parity, &bars.bad)) {
           ok = false;
           break;
         }
-        if (lane == 0) mbarrier_expect(&bars.v_full[st], bytes);
-        __syncwarp();
-        if (page >= 0)
-          tma_load_4d(base + L::kV + at, &vmap, half * 64, p.h, row, page, &bars.v_full[st]);
+        fetch(base + L::kV, &vmap, &bars.v_full[st]);
       }
     }
     if (*reinterpret_cast<volatile int*>(&bars.bad)) {
@@ -348,13 +409,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---- products: one thread ----
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = instruction<T>(kTile, false);
-      constexpr uint32_t kIdescO = instruction<T>(HD, true);
-      uint32_t tile = 0, item = 0, used[2] = {0, 0};
-      auto scores = [&](int i, int st) {               // S_i = Q_i K^T
-        const uint32_t q = base + L::kQ + i * L::kMatrix, k = base + L::kK + st * L::kMatrix;
+    // ---- products: the warp waits, an elected lane issues ----
+    constexpr uint32_t kIdescS = instruction<T>(kTile, false);
+    constexpr uint32_t kIdescO = instruction<T>(HD, true);
+    uint32_t tile = 0, item = 0, used[2] = {0, 0};
+    auto scores = [&](int i, int st) {                 // S_i = Q_i K^T
+      const uint32_t q = base + L::kQ + i * L::kMatrix, k = base + L::kK + st * L::kMatrix;
+      if (elect_lane()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = (kk >> 2) * L::kColumn + (kk & 3) * 32;
@@ -362,62 +423,80 @@ __global__ void __launch_bounds__(kThreads, 1)
                  kk > 0);
         }
         commit(&bars.s_full[i]);
-      };
-      auto values = [&](int i, int st, bool first) {   // O_i (+)= P_i V
-        const uint32_t v = base + L::kV + st * L::kMatrix;
+      }
+      __syncwarp();
+    };
+    // O_i (+)= P_i V over one half of the tile's positions
+    auto values = [&](int i, int st, int half, bool first) {
+      const uint32_t v = base + L::kV + st * L::kMatrix + half * (kTile / 2) * 128;
+      const uint32_t p = tmem + i * kTile + kTile / 2 + half * (kTile / 4);
+      if (elect_lane()) {
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_ts(tmem + 2 * kTile + i * HD, tmem + i * kTile + kk * 8,
-                 desc(v + kk * 2048, L::kColumn, 1024), kIdescO, !first || kk > 0);
-      };
-      bool ok = true;
-      for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
-        const Piece p = piece_of(a, w, index, shift, G);
-        const int n = max(p.count[0], p.count[1]);
-        if (n == 0) continue;
-        ok = wait_or_bad(&bars.q_full, item & 1, &bars.bad) &&
-             wait_or_bad(&bars.k_full[tile % kStages], (tile / kStages) & 1, &bars.bad);
-        if (!ok) break;
-        fence_after();
-        for (int i = 0; i < 2; ++i)
-          if (p.count[i] > 0) scores(i, tile % kStages);
-        commit(&bars.k_empty[tile % kStages]);
-        if (n == 1) commit(&bars.q_empty);
-        for (int jj = 0; ok && jj < n; ++jj, ++tile) {
-          const int st = tile % kStages;
-          const uint32_t next = tile + 1;
-          ok = wait_or_bad(&bars.v_full[st], (tile / kStages) & 1, &bars.bad);
-          for (int i = 0; ok && i < 2; ++i) {
-            if (jj < p.count[i]) {
-              if (!(ok = wait_or_bad(&bars.p_ready[i], used[i] & 1, &bars.bad))) break;
+        for (int kk = 0; kk < kTile / 32; ++kk)
+          mma_ts(tmem + 2 * kTile + i * HD, p + kk * 8, desc(v + kk * 2048, L::kColumn, 1024),
+                 kIdescO, !first || kk > 0);
+      }
+      __syncwarp();
+    };
+    auto signal = [&](uint64_t* bar) {                 // when the products so far are done
+      if (elect_lane()) commit(bar);
+      __syncwarp();
+    };
+    bool ok = true;
+    for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
+      const Piece p = piece_of(a, w, index, shift, G);
+      const int n = max(p.count[0], p.count[1]);
+      if (n == 0) continue;
+      ok = wait_or_bad(&bars.q_full, item & 1, &bars.bad) &&
+           wait_or_bad(&bars.k_full[tile % kStages], (tile / kStages) & 1, &bars.bad);
+      if (!ok) break;
+      fence_after();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (p.count[i] > 0) scores(i, tile % kStages);
+      signal(&bars.k_empty[tile % kStages]);
+      if (n == 1) signal(&bars.q_empty);
+      for (int jj = 0; ok && jj < n; ++jj, ++tile) {
+        const int st = tile % kStages;
+        const uint32_t next = tile + 1;
+        ok = wait_or_bad(&bars.v_full[st], (tile / kStages) & 1, &bars.bad);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (ok && jj < p.count[i]) {
+            ok = wait_or_bad(&bars.p_half[i], used[i] & 1, &bars.bad);
+            if (ok) {
+              fence_after();
+              values(i, st, 1, jj == 0);
+              ok = wait_or_bad(&bars.p_ready[i], used[i] & 1, &bars.bad);
+            }
+            if (ok) {
               ++used[i];
               fence_after();
-              values(i, st, jj == 0);
-              if (jj + 1 == p.count[i]) commit(&bars.o_done[i]);
+              values(i, st, 0, false);
+              if (jj + 1 == p.count[i]) signal(&bars.o_done[i]);
             }
-            if (jj + 1 < p.count[i]) {
-              if (!(ok = wait_or_bad(&bars.k_full[next % kStages], (next / kStages) & 1,
-                                     &bars.bad)))
-                break;
+          }
+          if (ok && jj + 1 < p.count[i]) {
+            ok = wait_or_bad(&bars.k_full[next % kStages], (next / kStages) & 1, &bars.bad);
+            if (ok) {
               fence_after();
               scores(i, next % kStages);
             }
           }
-          if (!ok) break;
-          commit(&bars.v_empty[st]);
-          if (jj + 1 < n) {
-            commit(&bars.k_empty[next % kStages]);
-            if (jj + 2 == n) commit(&bars.q_empty);
-          }
         }
-        ++item;
+        if (!ok) break;
+        signal(&bars.v_empty[st]);
+        if (jj + 1 < n) {
+          signal(&bars.k_empty[next % kStages]);
+          if (jj + 2 == n) signal(&bars.q_empty);
+        }
       }
-      // every MMA has ended, and with it the arrivals that it owes
-      commit(&bars.end);
-      (void)mbarrier_wait(&bars.end, 0);
+      ++item;
     }
-    __syncwarp();
-  } else {
+    // every MMA has ended, and with it the arrivals that it owes
+    signal(&bars.end);
+    (void)mbarrier_wait(&bars.end, 0);
+  } else if (warp < kProducerWarp) {
     // ---- softmax: a thread per row ----
     const int i = warp >> 2;                           // block
     const int r = tid & (kRows - 1);
@@ -449,18 +528,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++used;
         fence_after();
         const int pos0 = (p.j0 + jj) * kTile;
-        uint32_t x[kTile];
-#pragma unroll
-        for (int c = 0; c < kTile; c += 32) tmem_load32(ts + c, x + c);
-        tmem_load_wait<kTile>(x);
-        if (pos0 + kTile > see) {
-#pragma unroll
-          for (int c = 0; c < kTile; ++c)
-            if (pos0 + c >= see) x[c] = 0xff800000u;   // -inf
+        // The row in two halves.  P takes the columns of the upper one, so
+        // that the lower can wait in tensor memory while the upper's
+        // exponentials are taken: a thread then holds 64 to 96 scores, not
+        // 128 and what it makes of them.
+        uint32_t lo[kTile / 2], hi[kTile / 2];
+        tmem_load32(ts, lo);
+        tmem_load32(ts + 32, lo + 32);
+        tmem_load32(ts + 64, hi);
+        tmem_load32(ts + 96, hi + 32);
+        tmem_load_wait<kTile / 2>(lo);
+        tmem_tie<kTile / 2>(hi);
+        const bool cut = pos0 + kTile > see;
+        if (cut) {
+          hide<kTile / 2>(lo, see - pos0);
+          hide<kTile / 2>(hi, see - pos0 - kTile / 2);
         }
-        float mx = __uint_as_float(x[0]);
+        float mx = max3(lo[0], hi[0], lo[1]), my = max3(lo[2], hi[2], hi[1]);
 #pragma unroll
-        for (int c = 1; c < kTile; ++c) mx = fmaxf(mx, __uint_as_float(x[c]));
+        for (int c = 3; c + 1 < kTile / 2; c += 2) {
+          mx = max3(__float_as_uint(mx), lo[c], lo[c + 1]);
+          my = max3(__float_as_uint(my), hi[c], hi[c + 1]);
+        }
+        mx = max3(__float_as_uint(mx), lo[kTile / 2 - 1], hi[kTile / 2 - 1]);
+        mx = fmaxf(mx, my);
         mx *= scale;
         if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
           const float m_new = fmaxf(m, mx);
@@ -481,21 +572,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float off = m == -INFINITY ? 0.0f : -m;
-        // P rounds to the storage type, as its tensor-core operand: half a
-        // step per weight, against a sum that stays in fp32
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint32_t pk[kTile / 2];
-#pragma unroll
-        for (int c = 0; c < kTile; c += 2) {
-          const float e0 = ex2(fmaf(__uint_as_float(x[c]), scale, off));
-          const float e1 = ex2(fmaf(__uint_as_float(x[c + 1]), scale, off));
-          sum[(c >> 1) & 3] += e0 + e1;
-          pk[c / 2] = pack16(e0, e1, T());
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_store32(ts, pk);
-        tmem_store32(ts + 32, pk + 32);
         if (pos0 + kTile > p.s.len) {
           // rows of V past the end hold anything: their weights are 0, and so
           // must they be
@@ -512,10 +588,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        tmem_store_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbarrier_arrive(&bars.p_ready[i]);
+        const float off = m == -INFINITY ? 0.0f : -m;
+        const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
+        // P rounds to the storage type, as its tensor-core operand: half a
+        // step per weight, against a sum that stays in fp32
+        uint64_t sum[2] = {0, 0};
+        auto weights = [&](const uint32_t* x, int part) {   // 32 positions of the tile
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 z = halves_of(fma2(pair_of(x[e], x[e + 1]), scale2, off2));
+            const float e0 = ex2(z.x), e1 = ex2(z.y);
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair_of(e0, e1));
+            pk[e / 2] = pack16(e0, e1, T());
+          }
+          tmem_store16(ts + kTile / 2 + part * 16, pk);
+        };
+        auto publish = [&](uint64_t* bar) {                 // products over them may start
+          tmem_store_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbarrier_arrive(bar);
+        };
+        tmem_load32(ts, lo);
+        weights(hi, 2);
+        weights(hi + 32, 3);
+        tmem_load_wait<32>(lo);
+        publish(&bars.p_half[i]);
+        tmem_load32(ts + 32, lo + 32);
+        if (cut) hide<32>(lo, see - pos0);
+        weights(lo, 0);
+        tmem_load_wait<32>(lo + 32);
+        if (cut) hide<32>(lo + 32, see - pos0 - 32);
+        weights(lo + 32, 1);
+        publish(&bars.p_ready[i]);
+        const float2 s0 = halves_of(add2(sum[0], sum[1]));
+        l += s0.x + s0.y;
       }
       tile += max(p.count[0], p.count[1]);
       if (!ok) break;

@@ -33,6 +33,19 @@ __device__ __forceinline__ bool mbarrier_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// One lane of a converged warp.  MMAs and TMA copies take their operands from
+// uniform registers: issued one lane at a time behind a lane test they cost
+// about 200 cycles each, behind an elected lane of a converged warp what the
+// hardware needs (64 for a 128 x 128 x 16 MMA).
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t on;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(on));
+  return on != 0;
+}
 // Waits for the phase of the given parity, a few seconds at most: false then.
 __device__ __forceinline__ bool mbarrier_wait(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 22); ++i)
