@@ -848,8 +848,8 @@ size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t
                                           int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
   if (!paged_attention_shape(tokens, batch, max_q_len, n_q_heads, n_kv_heads, head_dim, dtype))
     return 0;
-  return vl::paged_attention_workspace_bytes(tokens, batch, max_q_len, n_q_heads, n_kv_heads,
-                                             head_dim, dtype);
+  return vl::paged_attention_workspace_bytes(batch, max_q_len, n_q_heads, n_kv_heads, head_dim,
+                                             dtype);
 }
 
 int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -887,10 +887,8 @@ int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
       !vl::aligned16(v_cache))
     return fail(VL_ERR_INVALID, "%s: q, out and the caches must be 16-byte aligned", op);
   if (tokens == 0 || batch == 0) return ok();
-  const size_t need = vl::paged_attention_workspace_bytes(tokens, batch, max_q_len, n_q_heads,
-                                                          n_kv_heads, head_dim, dtype);
-  if (need == 0)
-    return fail(VL_ERR_INVALID, "%s: batch * max_q_len is too large", op);
+  const size_t need = vl::paged_attention_workspace_bytes(batch, max_q_len, n_q_heads, n_kv_heads,
+                                                          head_dim, dtype);
   if (workspace == nullptr || workspace_bytes < need || !vl::aligned16(workspace))
     return fail(VL_ERR_INVALID, "%s: workspace of %zu bytes (16-byte aligned) required", op, need);
   const int64_t es = dtype_size(dtype);

@@ -235,14 +235,12 @@ struct PagedAttnArgs {
   int64_t page_stride;
   int32_t* status;
 };
-size_t paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
-                                       int n_q_heads, int n_kv_heads, int head_dim, int dtype);
+size_t paged_attention_workspace_bytes(int64_t batch, int64_t max_q_len, int n_q_heads,
+                                       int n_kv_heads, int head_dim, int dtype);
 cudaError_t launch_paged_attention(const PagedAttnArgs& args, int dtype, void* workspace,
                                    bool pdl, cudaStream_t stream);
 // The tcgen05 kernel of long chunks (vl_paged_attn_tc.cu).
-// 0 workspace bytes: more cells than the kernel counts.
-size_t paged_attention_tc_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
-                                          int n_q_heads, int n_kv_heads, int head_dim);
+size_t paged_attention_tc_workspace_bytes(int head_dim);
 cudaError_t launch_paged_attention_tc(const PagedAttnArgs& args, int dtype, void* workspace,
                                       bool pdl, cudaStream_t stream);
 

@@ -797,13 +797,11 @@ bool encode_rows_map(CUtensorMap* map, const void* rows, bool bf16, int head_dim
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-size_t paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
-                                       int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
+size_t paged_attention_workspace_bytes(int64_t batch, int64_t max_q_len, int n_q_heads,
+                                       int n_kv_heads, int head_dim, int dtype) {
   switch (paged_kind(max_q_len, n_q_heads, n_kv_heads, head_dim, dtype)) {
     case Kind::kFew: return few_workspace(batch, head_dim);
-    case Kind::kChunk:
-      return paged_attention_tc_workspace_bytes(tokens, batch, max_q_len, n_q_heads, n_kv_heads,
-                                                head_dim);
+    case Kind::kChunk: return paged_attention_tc_workspace_bytes(head_dim);
     default: return 16;
   }
 }

@@ -48,7 +48,9 @@ constexpr int kStages = 2;                // of K and of V
 constexpr int kSoftThreads = 256;         // two blocks' warps
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kPlanWarp = 10;
+constexpr int kThreads = 352;
+constexpr int kPlans = 4;                 // pieces that the walk is ahead
 constexpr float kRescaleLog2 = 8.0f;
 
 template <int HD>
@@ -59,80 +61,205 @@ struct Shape {
   static constexpr int kQ = 0;                         // two blocks
   static constexpr int kK = 2 * kMatrix;
   static constexpr int kV = kK + kStages * kMatrix;
-  static constexpr int kBars = kV + kStages * kMatrix;
-  static constexpr int kBytes = kBars + 256 + 1024;    // barriers, and the ring's alignment
+  static constexpr int kOut = kV + kStages * kMatrix;  // 32 rows x 64 dims a softmax warp
+  static constexpr int kBars = kOut + 8 * 4096;
+  static constexpr int kBytes = kBars + 1024 + 1024;    // barriers, and the ring's alignment
+};
+
+// A piece of work as the walk hands it to the others.
+struct Plan {
+  int row0;           // packed row of its first token
+  int tokens;         // tokens from there to the sequence's end
+  int seen0;          // positions that the first token sees, less one
+  int len;            // positions of the sequence
+  int h, b;           // kv head, sequence
+  int j0, j1;         // tiles of positions
+  int count[2];       // tiles of each block
+  int whole;          // all tiles of its cell
+  int last;           // no piece: the run is over
 };
 
 struct Bars {
-  uint64_t q_full, q_empty;
+  uint64_t q_full[2], q_empty[2];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], p_half[2], p_ready[2], o_done[2];
+  uint64_t plan_full[kPlans], plan_empty[kPlans];
   uint64_t end;
+  Plan plan[kPlans];
   uint32_t tmem;
   int bad;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+static_assert(sizeof(Bars) <= 1024, "barrier block");
 
 struct TcWork {
-  float* part;        // split: [cell * splits + s][256 rows][HD], then [..][256] (max, sum)
-  float2* ml;
-  int splits;
-  int tiles;          // q tiles of a sequence, at most
-  int cells;          // tiles * batch * kv heads
+  float* part;        // [2 * grid][256 rows][HD]: a CTA's cut pieces
+  float2* ml;         // [2 * grid][256] their (max, sum)
 };
 
-// One piece of work: a block pair of a sequence and kv head, and a run of
-// position tiles.
-struct Piece {
-  int b, h;
+// A cell is a pair of blocks of one sequence and kv head against the n tiles
+// of positions that they see.  All cells lie on one line, (sequence, head,
+// pair) in order, each as long as the positions it sees plus what a cell
+// costs by itself, so that places are sums in closed form; CTAs take equal
+// runs of the line.  Where a run ends inside a cell the cell is cut, at a
+// whole tile, if both ends are worth a piece; else it goes to the side that
+// has more of it.
+constexpr int kCellCost = 2 * kTile;      // of a cell by itself, in positions
+constexpr int kMinPiece = 4;              // tiles
+
+// Where a walk along the line stands.
+struct Walk {
+  int b;              // sequence (batch: past the end)
   SeqView s;
-  int tok0;           // first token of the pair
-  int j0;             // first position tile
-  int count[2];       // tiles of each block
+  int past;           // positions before the new tokens
+  int h, t;           // kv head, pair of blocks
+  int pairs;          // of the sequence
+  int64_t at, size;   // the cell's place on the line
+  int n;              // its tiles
   int rows_tok;       // tokens of a block
-  int tiles;          // block pairs of the sequence
-  int k;              // this one, from the sequence's end
-  bool lead;          // the sequence's first piece
+  int j0, j1;         // this CTA's tiles of it
 };
 
-__device__ __forceinline__ Piece piece_of(const PagedAttnArgs& a, const TcWork& w, int index,
-                                          int shift, int group) {
-  Piece p;
-  const int cell = index / w.splits, split = index - cell * w.splits;
-  const int per = a.batch * a.n_kv_heads;
-  const int rest = cell % per;
-  p.k = cell / per;
-  p.b = rest / a.n_kv_heads;
-  p.h = rest - p.b * a.n_kv_heads;
-  p.rows_tok = kRows / group;
-  p.s = sequence_view(a, p.b, shift);
-  const int pair = 2 * p.rows_tok;
-  p.tiles = (p.s.rows + pair - 1) / pair;
-  p.tok0 = (p.tiles - 1 - p.k) * pair;
-  p.lead = p.k == 0 && p.h == 0 && split == 0;
-  int n[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = p.tok0 + i * p.rows_tok;
-    const int last = min(p.s.rows, first + p.rows_tok);
-    const int see = p.s.len - p.s.rows + last;         // positions of the block's last token
-    n[i] = p.k < p.tiles && first < p.s.rows && see > 0 && p.s.len > 0 ? (see + kTile - 1) / kTile : 0;
-  }
-  const int all = max(n[0], n[1]);
-  p.j0 = static_cast<int>(static_cast<int64_t>(all) * split / w.splits);
-  const int j1 = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / w.splits);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) p.count[i] = max(0, min(j1, n[i]) - p.j0);
-  return p;
+__device__ __forceinline__ int cut_at(int64_t x, const Walk& w) {
+  const int64_t into = x - w.at;
+  if (into <= 0) return 0;
+  if (into >= w.size) return w.n;
+  if (w.n < 2 * kMinPiece) return 2 * into >= w.size ? w.n : 0;
+  const int j = into < kCellCost ? 0 : static_cast<int>((into - kCellCost) / kTile);
+  return j < kMinPiece ? 0 : (w.n - j < kMinPiece ? w.n : j);
 }
 
-__device__ __forceinline__ bool wait_or_bad(uint64_t* bar, uint32_t parity, int* bad) {
-  for (uint32_t i = 0; i < (1u << 22); ++i) {
+__device__ __forceinline__ int tiles_seen(const SeqView& s, int last_token) {
+  const int see = s.len - s.rows + last_token;         // positions of that token
+  return s.len > 0 && see > 0 ? (see + kTile - 1) / kTile : 0;
+}
+// A head's first t cells on the line, none of them the sequence's last.
+__device__ __forceinline__ int64_t cells_before(int past, int t, int pair) {
+  return t * (static_cast<int64_t>(past) + kCellCost) +
+         static_cast<int64_t>(t) * (t + 1) / 2 * pair;
+}
+__device__ __forceinline__ int64_t head_size(const SeqView& s, int pair) {
+  if (s.rows == 0) return 0;
+  const int past = max(0, s.len - s.rows), pairs = (s.rows + pair - 1) / pair;
+  return cells_before(past, pairs - 1, pair) + past + s.rows + kCellCost;
+}
+
+// The line's length; before: where the sequences that this lane adds up
+// begin (a whole warp, the l-th 32nd of them each).
+__device__ __forceinline__ int64_t line_length(const PagedAttnArgs& a, int shift, int pair,
+                                               int lane, int64_t* before, bool* bad) {
+  const int each = (a.batch + 31) / 32;
+  const int b0 = min(a.batch, lane * each), b1 = min(a.batch, b0 + each);
+  int64_t mine = 0;
+  *bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const SeqView s = sequence_view(a, b, shift);
+    *bad |= s.bad;
+    mine += head_size(s, pair) * a.n_kv_heads;
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += n;
+  }
+  *before = upto - mine;
+  return __shfl_sync(0xffffffffu, upto, 31);
+}
+
+__device__ __forceinline__ void enter_cell(int pair, Walk& w) {
+  const int last = min(w.s.rows, (w.t + 1) * pair);
+  w.n = tiles_seen(w.s, last);
+  w.size = static_cast<int64_t>(w.past) + last + kCellCost;
+}
+// The next sequence from w.b on that has rows.
+__device__ __forceinline__ void enter_sequence(const PagedAttnArgs& a, int shift, int pair,
+                                               Walk& w) {
+  for (; w.b < a.batch; ++w.b) {
+    w.s = sequence_view(a, w.b, shift);
+    if (w.s.rows > 0) break;
+  }
+  w.h = w.t = 0;
+  if (w.b == a.batch) return;
+  w.past = max(0, w.s.len - w.s.rows);
+  w.pairs = (w.s.rows + pair - 1) / pair;
+  enter_cell(pair, w);
+}
+__device__ __forceinline__ void next_cell(const PagedAttnArgs& a, int shift, int pair, Walk& w) {
+  w.at += w.size;
+  if (++w.t == w.pairs) {
+    w.t = 0;
+    if (++w.h == a.n_kv_heads) {
+      ++w.b;
+      enter_sequence(a, shift, pair, w);
+      return;
+    }
+  }
+  enter_cell(pair, w);
+}
+// The cell that holds place x.
+__device__ __forceinline__ Walk find_cell(const PagedAttnArgs& a, int shift, int pair,
+                                          int64_t before, int64_t x) {
+  const int owner = 31 - __clz(__ballot_sync(0xffffffffu, before <= x));
+  Walk w;
+  w.b = owner * ((a.batch + 31) / 32);
+  w.at = __shfl_sync(0xffffffffu, before, owner);
+  w.rows_tok = pair / 2;
+  enter_sequence(a, shift, pair, w);
+  while (w.b < a.batch) {
+    const int64_t head = head_size(w.s, pair), into = x - w.at;
+    if (into < head * a.n_kv_heads) {
+      w.h = static_cast<int>(into / head);
+      w.at += w.h * head;
+      int hi = w.pairs;                   // the last cell of the head that begins at or before x
+      while (hi - w.t > 1) {
+        const int mid = (w.t + hi) / 2;
+        if (w.at + cells_before(w.past, mid, pair) <= x) w.t = mid;
+        else hi = mid;
+      }
+      w.at += cells_before(w.past, w.t, pair);
+      enter_cell(pair, w);
+      break;
+    }
+    w.at += head * a.n_kv_heads;
+    ++w.b;
+    enter_sequence(a, shift, pair, w);
+  }
+  return w;
+}
+
+// This CTA's run, cell by cell.
+struct Run {
+  int64_t x0, x1;
+  int shift, pair;
+};
+__device__ __forceinline__ bool settle(const PagedAttnArgs& a, const Run& r, Walk& w) {
+  for (; w.b < a.batch && w.at < r.x1; next_cell(a, r.shift, r.pair, w)) {
+    w.j0 = cut_at(r.x0, w);
+    w.j1 = cut_at(r.x1, w);
+    if (w.j1 > w.j0) return true;
+    if (w.n == 0 && w.at >= r.x0) return true;
+  }
+  return false;
+}
+// Tiles of block i within the piece.
+__device__ __forceinline__ int block_tiles(const Walk& w, int i) {
+  const int first = w.t * 2 * w.rows_tok + i * w.rows_tok;
+  if (first >= w.s.rows) return 0;
+  return max(0, min(w.j1, tiles_seen(w.s, min(w.s.rows, first + w.rows_tok))) - w.j0);
+}
+
+// The slow side of a wait: bounded, and given up when another has run out.
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, int* bad) {
+  for (uint32_t i = 0; i < kWaitPolls; ++i) {
     if (mbarrier_test(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(bad)) return false;
   }
   atomicExch(bad, 1);
   return false;
+}
+__device__ __forceinline__ bool wait_or_bad(uint64_t* bar, uint32_t parity, int* bad) {
+  const uint32_t at = smem_addr(bar);
+  return mbarrier_test(at, parity) || wait_longer(at, parity, bad);
 }
 
 __device__ __forceinline__ void fence_before() {
@@ -275,6 +402,28 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
   return y;
 }
+// 2^x of two values on the multiply-add pipe, beside the exponential unit:
+// x = n + f with |f| <= 1/2, a degree-5 polynomial of f fitted to the least
+// relative error (2.2e-7), n added to the exponent.  Values below -126 give
+// about 1e-38.
+__device__ __forceinline__ float2 ex2_pair(float2 z) {
+  const uint64_t t = pair_of(fmaxf(z.x, -126.0f), fmaxf(z.y, -126.0f));
+  constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: the sum's low bits are n
+  const uint64_t r = add2(t, pair_of(kRound, kRound));
+  const uint64_t f = fma2(add2(r, pair_of(-kRound, -kRound)), pair_of(-1.0f, -1.0f), t);
+  uint64_t p = fma2(pair_of(0.0013276471f, 0.0013276471f), f, pair_of(0.009675541f, 0.009675541f));
+  p = fma2(p, f, pair_of(0.05550713f, 0.05550713f));
+  p = fma2(p, f, pair_of(0.2402212f, 0.2402212f));
+  p = fma2(p, f, pair_of(0.69314694f, 0.69314694f));
+  p = fma2(p, f, pair_of(1.0000001f, 1.0000001f));
+  const float2 pf = halves_of(p), rf = halves_of(r);
+  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(rf.x) << 23)),
+                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(rf.y) << 23)));
+}
+// Which of the 32 pairs of half a row go that way: three of eight, spread.
+__device__ constexpr bool by_polynomial(int pair) {
+  return pair % 8 == 1 || pair % 8 == 4 || pair % 8 == 6;
+}
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
   return pack_bf16x2(lo, hi);
 }
@@ -297,11 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = ilog2(a.page_size);
   const int G = a.n_q_heads / a.n_kv_heads;
-  const int pieces = w.cells * w.splits;
 
   if (tid == 0) {
-    mbarrier_init(&bars.q_full, 1);
-    mbarrier_init(&bars.q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
       mbarrier_init(&bars.k_full[s], 1);
       mbarrier_init(&bars.k_empty[s], 1);
@@ -309,10 +455,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbarrier_init(&bars.v_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbarrier_init(&bars.q_full[i], 1);
+      mbarrier_init(&bars.q_empty[i], 1);
       mbarrier_init(&bars.s_full[i], 1);
       mbarrier_init(&bars.p_half[i], kSoftThreads / 64);    // a block's warps
       mbarrier_init(&bars.p_ready[i], kSoftThreads / 64);
       mbarrier_init(&bars.o_done[i], 1);
+    }
+    for (int k = 0; k < kPlans; ++k) {
+      mbarrier_init(&bars.plan_full[k], 1);
+      mbarrier_init(&bars.plan_empty[k], 2 + kSoftThreads / 32);   // every reader's warp
     }
     mbarrier_init(&bars.end, 1);
     bars.bad = 0;
@@ -330,35 +482,94 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = bars.tmem;
-  pdl_wait();
-  pdl_release();
 
-  if (warp == kProducerWarp) {
-    // ---- copies: Q of a piece, then its K and V tiles in turn ----
-    const int box_rows = 1 << box_shift;
-    uint32_t tile = 0, item = 0;          // tiles and pieces so far
-    bool ok = true;
-    for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
-      const Piece p = piece_of(a, w, index, shift, G);
-      const int n = max(p.count[0], p.count[1]);
-      if (n == 0) continue;
-      if (item > 0 && !wait_or_bad(&bars.q_empty, (item - 1) & 1, &bars.bad)) break;
-      if (elect_lane()) {
-        const uint32_t bytes = L::kHalves * 128 * G * p.rows_tok;
-        mbarrier_expect(&bars.q_full, bytes * ((p.count[0] > 0) + (p.count[1] > 0)));
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (p.count[i] > 0)
-#pragma unroll
-            for (int c = 0; c < L::kHalves; ++c)
-              tma_load_3d(base + L::kQ + i * L::kMatrix + c * L::kColumn, &qmap, c * 64, p.h * G,
-                          p.s.start + p.tok0 + i * p.rows_tok, &bars.q_full);
+  // Pieces as they come, for the producer, the MMA warp and the softmax warps.
+  uint32_t piece = 0;
+  bool ok = true;
+  auto take = [&](Plan& p) {
+    ok = wait_or_bad(&bars.plan_full[piece % kPlans], (piece / kPlans) & 1, &bars.bad);
+    if (!ok) return false;
+    p = bars.plan[piece % kPlans];
+    __syncwarp();
+    if (lane == 0) mbarrier_arrive(&bars.plan_empty[piece % kPlans]);
+    ++piece;
+    return p.last == 0;
+  };
+
+  if (warp == kPlanWarp) {
+    // ---- the walk; lengths and tables are not written by the kernel before
+    // this one ----
+    Run run;
+    run.shift = shift;
+    run.pair = 2 * (kRows / G);
+    int64_t before;
+    bool bad_lengths;
+    const int64_t total = line_length(a, shift, run.pair, lane, &before, &bad_lengths);
+    if (bad_lengths && blockIdx.x == 0 && a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
+    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    run.x0 = min(total, blockIdx.x * share);
+    run.x1 = min(total, run.x0 + share);
+    Walk at;
+    at.b = a.batch;
+    if (run.x0 < run.x1) at = find_cell(a, shift, run.pair, before, run.x0);
+    for (bool more = true; more; ++piece) {
+      more = settle(a, run, at);
+      const int slot = piece % kPlans;
+      if (piece >= kPlans &&
+          !wait_or_bad(&bars.plan_empty[slot], ((piece / kPlans) & 1) ^ 1, &bars.bad))
+        break;
+      if (lane == 0) {
+        Plan p{};
+        p.last = !more;
+        if (more) {
+          const int tok0 = 2 * at.t * at.rows_tok;
+          p.row0 = at.s.start + tok0;
+          p.tokens = at.s.rows - tok0;
+          p.seen0 = at.s.len - at.s.rows + tok0;
+          p.len = at.s.len;
+          p.h = at.h;
+          p.b = at.b;
+          p.j0 = at.j0;
+          p.j1 = at.j1;
+          p.count[0] = block_tiles(at, 0);
+          p.count[1] = block_tiles(at, 1);
+          p.whole = at.j0 == 0 && at.j1 == at.n;
+        }
+        bars.plan[slot] = p;
+        mbarrier_arrive(&bars.plan_full[slot]);
       }
       __syncwarp();
-      ++item;
-      for (int jj = 0; jj < n; ++jj, ++tile) {
-        const int pos0 = (p.j0 + jj) * kTile;
-        const int need = (min(kTile, p.s.len - pos0) + box_rows - 1) >> box_shift;
+      if (more) next_cell(a, shift, run.pair, at);
+    }
+    // the last ones have been read before this block goes
+    for (uint32_t k = piece < kPlans ? 0 : piece - kPlans; k < piece; ++k)
+      if (!wait_or_bad(&bars.plan_empty[k % kPlans], (k / kPlans) & 1, &bars.bad)) break;
+  } else if (warp == kProducerWarp) {
+    // ---- copies: Q of a piece, then its K and V tiles in turn ----
+    pdl_wait();
+    pdl_release();
+    const int box_rows = 1 << box_shift, rows_tok = kRows / G;
+    uint32_t tile = 0, asked[2] = {0, 0};              // tiles and Q blocks so far
+    Plan p;
+    while (ok && take(p)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!ok || p.count[i] == 0) continue;
+        if (asked[i] > 0) ok = wait_or_bad(&bars.q_empty[i], (asked[i] - 1) & 1, &bars.bad);
+        if (!ok) continue;
+        ++asked[i];
+        if (elect_lane()) {
+          mbarrier_expect(&bars.q_full[i], L::kHalves * 128 * G * rows_tok);
+#pragma unroll
+          for (int c = 0; c < L::kHalves; ++c)
+            tma_load_3d(base + L::kQ + i * L::kMatrix + c * L::kColumn, &qmap, c * 64, p.h * G,
+                        p.row0 + i * rows_tok, &bars.q_full[i]);
+        }
+        __syncwarp();
+      }
+      for (int j = p.j0; ok && j < p.j1; ++j, ++tile) {
+        const int pos0 = j * kTile;
+        const int need = (min(kTile, p.len - pos0) + box_rows - 1) >> box_shift;
         // lane l looks up the l-th box's page, all before the waits
         int page = 0;
         if (lane < need) {
@@ -374,186 +585,195 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto fetch = [&](uint32_t matrix, const CUtensorMap* map, uint64_t* full) {
           if (elect_lane()) mbarrier_expect(full, bytes);
           __syncwarp();
-          for (int j = 0; j < need; ++j) {
-            const int pj = __shfl_sync(0xffffffffu, page, j);
-            const uint32_t dst = matrix + st * L::kMatrix + j * box_rows * 128;
-            const int row = (pos0 + (j << box_shift)) & (a.page_size - 1);
+          for (int k = 0; k < need; ++k) {
+            const int pk = __shfl_sync(0xffffffffu, page, k);
+            const uint32_t dst = matrix + st * L::kMatrix + k * box_rows * 128;
+            const int row = (pos0 + (k << box_shift)) & (a.page_size - 1);
             if (elect_lane()) {
 #pragma unroll
               for (int c = 0; c < L::kHalves; ++c)
-                tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pj, full);
+                tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pk, full);
             }
             __syncwarp();
           }
         };
-        if (tile >= kStages && !wait_or_bad(&bars.k_empty[st], parity, &bars.bad)) {
-          ok = false;
-          break;
-        }
+        if (tile >= kStages) ok = wait_or_bad(&bars.k_empty[st], parity, &bars.bad);
+        if (!ok) break;
         fetch(base + L::kK, &kmap, &bars.k_full[st]);
-        if (tile >= kStages && !wait_or_bad(&bars.v_empty[st], parity, &bars.bad)) {
-          ok = false;
-          break;
-        }
+        if (tile >= kStages) ok = wait_or_bad(&bars.v_empty[st], parity, &bars.bad);
+        if (!ok) break;
         fetch(base + L::kV, &vmap, &bars.v_full[st]);
       }
     }
     if (*reinterpret_cast<volatile int*>(&bars.bad)) {
       // leave no copy in flight (each wait is bounded; what was never asked
-      // for lets them run out)
-      if (item > 0) (void)mbarrier_wait(&bars.q_full, (item - 1) & 1);
+      // for lets it run out)
+      auto drain = [&](uint64_t* bar, uint32_t parity) {
+        for (int i = 0; i < 1000 && !mbarrier_test(bar, parity); ++i) {}
+      };
+      for (int i = 0; i < 2; ++i)
+        if (asked[i] > 0) drain(&bars.q_full[i], (asked[i] - 1) & 1);
       for (uint32_t t = tile < kStages ? 0 : tile - kStages; t <= tile; ++t) {
-        const uint32_t parity = (t / kStages) & 1;
-        for (int i = 0; i < 1000 && !mbarrier_test(&bars.k_full[t % kStages], parity); ++i) {}
-        for (int i = 0; i < 1000 && !mbarrier_test(&bars.v_full[t % kStages], parity); ++i) {}
+        drain(&bars.k_full[t % kStages], (t / kStages) & 1);
+        drain(&bars.v_full[t % kStages], (t / kStages) & 1);
       }
     }
   } else if (warp == kMmaWarp) {
-    // ---- products: the warp waits, an elected lane issues ----
-    constexpr uint32_t kIdescS = instruction<T>(kTile, false);
-    constexpr uint32_t kIdescO = instruction<T>(HD, true);
-    uint32_t tile = 0, item = 0, used[2] = {0, 0};
-    auto scores = [&](int i, int st) {                 // S_i = Q_i K^T
-      const uint32_t q = base + L::kQ + i * L::kMatrix, k = base + L::kK + st * L::kMatrix;
-      if (elect_lane()) {
+    // ---- products: one thread ----
+    // Each block is a stream of tiles of its own, across cells: S of its next
+    // tile is issued behind P V of the last, whatever the other block does.
+    // This thread's own steps are on every tile's critical path, so
+    // descriptors are made once and only their low words move.
+    if (elect_lane()) {
+      constexpr uint32_t kIdescS = instruction<T>(kTile, false);
+      constexpr uint32_t kIdescO = instruction<T>(HD, true);
+      uint64_t qd[2], kd[kStages], vd[kStages];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) qd[i] = desc(base + L::kQ + i * L::kMatrix, 16, 1024);
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) {
+        kd[i] = desc(base + L::kK + i * L::kMatrix, 16, 1024);
+        vd[i] = desc(base + L::kV + i * L::kMatrix, L::kColumn, 1024);
+      }
+      uint32_t tile = 0, heads[2] = {0, 0}, used[2] = {0, 0};
+      auto wait = [&](uint64_t& bar, uint32_t parity) {
+        ok = ok && wait_or_bad(&bar, parity & 1, &bars.bad);
+      };
+      auto ask = [&](int i, uint32_t t, bool first, bool last) {   // S_i = Q_i K^T of tile t
+        if (first) wait(bars.q_full[i], heads[i]++);
+        wait(bars.k_full[t % kStages], t / kStages);
+        if (!ok) return;
+        fence_after();
+        const uint64_t k = kd[t % kStages];
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * L::kColumn + (kk & 3) * 32;
-          mma_ss(tmem + i * kTile, desc(q + off, 16, 1024), desc(k + off, 16, 1024), kIdescS,
-                 kk > 0);
+          const uint32_t off = ((kk >> 2) * L::kColumn + (kk & 3) * 32) >> 4;
+          mma_ss(tmem + i * kTile, qd[i] + off, k + off, kIdescS, kk > 0);
         }
         commit(&bars.s_full[i]);
-      }
-      __syncwarp();
-    };
-    // O_i (+)= P_i V over one half of the tile's positions
-    auto values = [&](int i, int st, int half, bool first) {
-      const uint32_t v = base + L::kV + st * L::kMatrix + half * (kTile / 2) * 128;
-      const uint32_t p = tmem + i * kTile + kTile / 2 + half * (kTile / 4);
-      if (elect_lane()) {
+        if (last) commit(&bars.q_empty[i]);
+      };
+      // O_i (+)= P_i V over one half of the tile's positions
+      auto values = [&](int i, int half, bool first) {
+        const uint64_t v = vd[tile % kStages] + half * (kTile / 2 * 128 >> 4);
+        const uint32_t p = tmem + i * kTile + half * (kTile / 4);
+        fence_after();
 #pragma unroll
         for (int kk = 0; kk < kTile / 32; ++kk)
-          mma_ts(tmem + 2 * kTile + i * HD, p + kk * 8, desc(v + kk * 2048, L::kColumn, 1024),
-                 kIdescO, !first || kk > 0);
-      }
-      __syncwarp();
-    };
-    auto signal = [&](uint64_t* bar) {                 // when the products so far are done
-      if (elect_lane()) commit(bar);
-      __syncwarp();
-    };
-    bool ok = true;
-    for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
-      const Piece p = piece_of(a, w, index, shift, G);
-      const int n = max(p.count[0], p.count[1]);
-      if (n == 0) continue;
-      ok = wait_or_bad(&bars.q_full, item & 1, &bars.bad) &&
-           wait_or_bad(&bars.k_full[tile % kStages], (tile / kStages) & 1, &bars.bad);
-      if (!ok) break;
-      fence_after();
+          mma_ts(tmem + 2 * kTile + i * HD, p + kk * 8, v + kk * (2048 >> 4), kIdescO,
+                 !first || kk > 0);
+      };
+      // tiles of a piece, and of its blocks (a piece without tiles is not ours)
+      struct Count {
+        int all, of[2];
+      };
+      auto next_piece = [&](Count& c) {
+        for (;;) {
+          wait(bars.plan_full[piece % kPlans], piece / kPlans);
+          if (!ok) return false;
+          const Plan& p = bars.plan[piece % kPlans];
+          const bool over = p.last != 0;
+          c.all = p.j1 - p.j0;
+          c.of[0] = p.count[0];
+          c.of[1] = p.count[1];
+          mbarrier_arrive(&bars.plan_empty[piece % kPlans]);
+          ++piece;
+          if (over) return false;
+          if (c.all > 0) return true;
+        }
+      };
+      Count now, then;
+      bool more = next_piece(now);
+      if (more) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (p.count[i] > 0) scores(i, tile % kStages);
-      signal(&bars.k_empty[tile % kStages]);
-      if (n == 1) signal(&bars.q_empty);
-      for (int jj = 0; ok && jj < n; ++jj, ++tile) {
-        const int st = tile % kStages;
-        const uint32_t next = tile + 1;
-        ok = wait_or_bad(&bars.v_full[st], (tile / kStages) & 1, &bars.bad);
+        for (int i = 0; i < 2; ++i)
+          if (now.of[i] > 0) ask(i, 0, true, now.of[i] == 1);
+        commit(&bars.k_empty[0]);
+      }
+      int jj = 0;
+      while (ok && more) {
+        const bool ends = jj + 1 == now.all;
+        int jn = jj + 1;
+        then = now;
+        if (ends) {
+          more = next_piece(then);
+          jn = 0;
+          if (!more) then.of[0] = then.of[1] = 0;
+        }
+        wait(bars.v_full[tile % kStages], tile / kStages);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (ok && jj < p.count[i]) {
-            ok = wait_or_bad(&bars.p_half[i], used[i] & 1, &bars.bad);
+          if (jj < now.of[i]) {
+            wait(bars.p_half[i], used[i]);
+            if (ok) values(i, 0, jj == 0);
+            wait(bars.p_ready[i], used[i]++);
             if (ok) {
-              fence_after();
-              values(i, st, 1, jj == 0);
-              ok = wait_or_bad(&bars.p_ready[i], used[i] & 1, &bars.bad);
-            }
-            if (ok) {
-              ++used[i];
-              fence_after();
-              values(i, st, 0, false);
-              if (jj + 1 == p.count[i]) signal(&bars.o_done[i]);
+              values(i, 1, false);
+              if (jj + 1 == now.of[i]) commit(&bars.o_done[i]);
             }
           }
-          if (ok && jj + 1 < p.count[i]) {
-            ok = wait_or_bad(&bars.k_full[next % kStages], (next / kStages) & 1, &bars.bad);
-            if (ok) {
-              fence_after();
-              scores(i, next % kStages);
-            }
-          }
+          if (jn < then.of[i]) ask(i, tile + 1, ends, jn + 1 == then.of[i]);
         }
-        if (!ok) break;
-        signal(&bars.v_empty[st]);
-        if (jj + 1 < n) {
-          signal(&bars.k_empty[next % kStages]);
-          if (jj + 2 == n) signal(&bars.q_empty);
-        }
+        commit(&bars.v_empty[tile % kStages]);
+        if (more) commit(&bars.k_empty[(tile + 1) % kStages]);
+        ++tile;
+        now = then;
+        jj = jn;
       }
-      ++item;
+      // every MMA has ended, and with it the arrivals that it owes
+      commit(&bars.end);
+      (void)mbarrier_wait(&bars.end, 0);
     }
-    // every MMA has ended, and with it the arrivals that it owes
-    signal(&bars.end);
-    (void)mbarrier_wait(&bars.end, 0);
-  } else if (warp < kProducerWarp) {
+    __syncwarp();
+  } else {
     // ---- softmax: a thread per row ----
+    pdl_wait();                                        // it writes rows
     const int i = warp >> 2;                           // block
     const int r = tid & (kRows - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + i * kTile + lanes, to = tmem + 2 * kTile + i * HD + lanes;
     const float scale = a.scale * kLog2e;
+    const int rows_tok = kRows / G, tok = i * rows_tok + r / G, g = r % G;
     uint32_t tile = 0, used = 0, finished = 0;
-    bool ok = true;
-    for (int index = blockIdx.x; ok && index < pieces; index += gridDim.x) {
-      const Piece p = piece_of(a, w, index, shift, G);
-      if (p.lead && p.s.bad && tid == 0 && a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
-      if (p.s.len == 0) {                 // nothing cached, or bad lengths: zero rows
-        if (index % w.splits != 0 || r >= G * p.rows_tok) continue;
-        for (int64_t t = static_cast<int64_t>(p.k) * 2 * p.rows_tok + i * p.rows_tok + r / G;
-             t < p.s.rows; t += static_cast<int64_t>(w.tiles) * 2 * p.rows_tok) {
-          T* out = static_cast<T*>(a.out) + (p.s.start + t) * a.out_row_stride +
-                   static_cast<int64_t>(p.h * G + r % G) * HD;
-          for (int c = 0; c < HD; c += 8) st_vec(out + c, make_uint4(0, 0, 0, 0));
-        }
-        continue;
-      }
-      if (p.k >= p.tiles) continue;
-      const int tok = p.tok0 + i * p.rows_tok + r / G, g = r % G;
-      const bool mine = r < G * p.rows_tok && tok < p.s.rows;
-      const int see = mine ? p.s.len - p.s.rows + tok + 1 : 0;
+    Plan p;
+    while (ok && take(p)) {
+      const int count = p.count[i];
+      const bool mine = r < G * rows_tok && tok < p.tokens;
+      // (rows of nobody are not hidden: their results go nowhere)
+      const int see = !mine ? 0x7fffffff : (p.len > 0 ? p.seen0 + tok + 1 : 0);
       float m = -INFINITY, l = 0.0f;
-      for (int jj = 0; jj < p.count[i]; ++jj) {
+      for (int jj = 0; jj < count; ++jj) {
         if (!(ok = wait_or_bad(&bars.s_full[i], used & 1, &bars.bad))) break;
         ++used;
         fence_after();
         const int pos0 = (p.j0 + jj) * kTile;
-        // The row in two halves.  P takes the columns of the upper one, so
-        // that the lower can wait in tensor memory while the upper's
-        // exponentials are taken: a thread then holds 64 to 96 scores, not
-        // 128 and what it makes of them.
-        uint32_t lo[kTile / 2], hi[kTile / 2];
-        tmem_load32(ts, lo);
-        tmem_load32(ts + 32, lo + 32);
-        tmem_load32(ts + 64, hi);
-        tmem_load32(ts + 96, hi + 32);
-        tmem_load_wait<kTile / 2>(lo);
-        tmem_tie<kTile / 2>(hi);
-        const bool cut = pos0 + kTile > see;
-        if (cut) {
-          hide<kTile / 2>(lo, see - pos0);
-          hide<kTile / 2>(hi, see - pos0 - kTile / 2);
-        }
-        float mx = max3(lo[0], hi[0], lo[1]), my = max3(lo[2], hi[2], hi[1]);
+        // Half a row at a time, read from tensor memory once for the maximum
+        // and again for the weights: a load takes some 40 cycles, and held
+        // rows (128 registers) and unrolled code (instruction fetches, which
+        // short chunks do not amortise) cost more.
+        const bool cut = __any_sync(0xffffffffu, pos0 + kTile > see);
+        float mx = -INFINITY, my = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += kTile / 2) {
+          uint32_t x[kTile / 2];
+          tmem_load32(ts + c, x);
+          tmem_load32(ts + c + 32, x + 32);
+          tmem_load_wait<kTile / 2>(x);
+          if (cut) hide<kTile / 2>(x, see - pos0 - c);
+          float mz = max3(x[0], x[1], x[2]), mw = max3(x[3], x[4], x[5]);
 #pragma unroll
-        for (int c = 3; c + 1 < kTile / 2; c += 2) {
-          mx = max3(__float_as_uint(mx), lo[c], lo[c + 1]);
-          my = max3(__float_as_uint(my), hi[c], hi[c + 1]);
+          for (int e = 6; e + 8 <= kTile / 2; e += 8) {
+            mx = max3(__float_as_uint(mx), x[e], x[e + 1]);
+            my = max3(__float_as_uint(my), x[e + 2], x[e + 3]);
+            mz = max3(__float_as_uint(mz), x[e + 4], x[e + 5]);
+            mw = max3(__float_as_uint(mw), x[e + 6], x[e + 7]);
+          }
+          mx = max3(__float_as_uint(mx), x[kTile / 2 - 2], x[kTile / 2 - 1]);
+          my = fmaxf(my, fmaxf(mz, mw));
         }
-        mx = max3(__float_as_uint(mx), lo[kTile / 2 - 1], hi[kTile / 2 - 1]);
         mx = fmaxf(mx, my);
         mx *= scale;
-        if (__any_sync(0xffffffffu, mx > m + kRescaleLog2)) {
+        if (__any_sync(0xffffffffu, mine && mx > m + kRescaleLog2)) {
           const float m_new = fmaxf(m, mx);
           const float f = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
           l *= f;
@@ -561,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (jj > 0) {
             // the products that wrote O are done: this tile's scores were
             // issued behind them
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
               uint32_t o[32];
               tmem_load32(to + c, o);
@@ -572,13 +792,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (pos0 + kTile > p.s.len) {
+        if (pos0 + kTile > p.len) {
           // rows of V past the end hold anything: their weights are 0, and so
           // must they be
           const uint32_t t = tile + jj;
           if (!(ok = wait_or_bad(&bars.v_full[t % kStages], (t / kStages) & 1, &bars.bad))) break;
           const uint32_t v = base + L::kV + (t % kStages) * L::kMatrix;
-          const int past = p.s.len - pos0;
+          const int past = p.len - pos0;
           for (int z = r; z < (kTile - past) * (HD / 8); z += kRows) {
             const int row = past + z / (HD / 8), ch = z % (HD / 8);
             asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(
@@ -593,84 +813,115 @@ __global__ void __launch_bounds__(kThreads, 1)
         // P rounds to the storage type, as its tensor-core operand: half a
         // step per weight, against a sum that stays in fp32
         uint64_t sum[2] = {0, 0};
-        auto weights = [&](const uint32_t* x, int part) {   // 32 positions of the tile
-          uint32_t pk[16];
+#pragma unroll 1
+        for (int c = 0; c < kTile; c += kTile / 2) {
+          uint32_t x[kTile / 2], pk[kTile / 4];
+          tmem_load32(ts + c, x);
+          tmem_load32(ts + c + 32, x + 32);
+          tmem_load_wait<kTile / 2>(x);
+          if (cut) {
+            hide<kTile / 2>(x, see - pos0 - c);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 z = halves_of(fma2(pair_of(x[e], x[e + 1]), scale2, off2));
-            const float e0 = ex2(z.x), e1 = ex2(z.y);
-            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair_of(e0, e1));
-            pk[e / 2] = pack16(e0, e1, T());
+            for (int e = 0; e < kTile / 2; e += 2) {
+              const float2 z = halves_of(fma2(pair_of(x[e], x[e + 1]), scale2, off2));
+              const float e0 = ex2(z.x), e1 = ex2(z.y);
+              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair_of(e0, e1));
+              pk[e / 2] = pack16(e0, e1, T());
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kTile / 2; e += 2) {
+              const uint64_t z2 = fma2(pair_of(x[e], x[e + 1]), scale2, off2);
+              const float2 z = halves_of(z2);
+              float e0, e1;
+              if (by_polynomial(e / 2)) {
+                const float2 y = ex2_pair(z);
+                e0 = y.x;
+                e1 = y.y;
+              } else {
+                e0 = ex2(z.x);
+                e1 = ex2(z.y);
+              }
+              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair_of(e0, e1));
+              pk[e / 2] = pack16(e0, e1, T());
+            }
           }
-          tmem_store16(ts + kTile / 2 + part * 16, pk);
-        };
-        auto publish = [&](uint64_t* bar) {                 // products over them may start
+          tmem_store32(ts + c / 2, pk);   // over columns that have been read
+          // the products over these positions may start
           tmem_store_wait();
           fence_before();
           __syncwarp();
-          if (lane == 0) mbarrier_arrive(bar);
-        };
-        tmem_load32(ts, lo);
-        weights(hi, 2);
-        weights(hi + 32, 3);
-        tmem_load_wait<32>(lo);
-        publish(&bars.p_half[i]);
-        tmem_load32(ts + 32, lo + 32);
-        if (cut) hide<32>(lo, see - pos0);
-        weights(lo, 0);
-        tmem_load_wait<32>(lo + 32);
-        if (cut) hide<32>(lo + 32, see - pos0 - 32);
-        weights(lo + 32, 1);
-        publish(&bars.p_ready[i]);
+          if (lane == 0) mbarrier_arrive(c == 0 ? &bars.p_half[i] : &bars.p_ready[i]);
+        }
         const float2 s0 = halves_of(add2(sum[0], sum[1]));
         l += s0.x + s0.y;
       }
-      tile += max(p.count[0], p.count[1]);
+      tile += p.j1 - p.j0;
       if (!ok) break;
       // ---- the piece's rows ----
       float inv = 0.0f;
-      if (p.count[i] > 0) {
+      if (count > 0) {
         if (!(ok = wait_or_bad(&bars.o_done[i], finished & 1, &bars.bad))) break;
         ++finished;
         fence_after();
         inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       }
-      const int64_t row256 = static_cast<int64_t>(index) * 2 * kRows + i * kRows + r;
-      if (w.splits > 1 && p.count[i] > 0) {
-        if (mine) w.ml[row256] = make_float2(m, l);
-        inv = 1.0f;
-      }
-      T* out = static_cast<T*>(a.out) + static_cast<int64_t>(p.s.start + tok) * a.out_row_stride +
-               static_cast<int64_t>(p.h * G + g) * HD;
-#pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        if (p.count[i] > 0) {
+      // a CTA's first piece may begin inside its cell (slot 0), its last end there
+      const int64_t row256 = (2 * static_cast<int64_t>(blockIdx.x) + (p.j0 > 0 ? 0 : 1)) * 2 * kRows +
+                             i * kRows + r;
+      if (!p.whole && mine) w.ml[row256] = make_float2(m, l);
+      const int64_t at_row = static_cast<int64_t>(p.row0 + tok) * a.out_row_stride +
+                             static_cast<int64_t>(p.h * G + g) * HD;
+      const uint32_t stage = base + L::kOut + warp * 4096;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 64) {
+        uint32_t o[64];
+        if (count > 0) {
           tmem_load32(to + c, o);
-          tmem_load_wait<32>(o);
+          tmem_load32(to + c + 32, o + 32);
+          tmem_load_wait<64>(o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
+          for (int e = 0; e < 64; ++e) o[e] = 0;
         }
-        if (!mine) continue;
-        if (w.splits > 1) {
-          if (p.count[i] > 0) {
+        if (!p.whole) {
+          if (mine) {
             float4* dst = reinterpret_cast<float4*>(w.part + row256 * HD + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 16; ++e)
               dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
                                    __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
           }
-        } else {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              f[e] = inv == 0.0f ? 0.0f : __uint_as_float(o[8 * v + e]) * inv;
-            st_vec(out + c + v * 8, S::pack(f));
-          }
+          continue;
         }
+        // A lane has a row; a store of 32 rows at once would touch 32
+        // half-filled sectors.  Through shared memory eight lanes take a
+        // row's 128 bytes instead (7300 -> 2400 cycles for a cell's rows).
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            f[e] = inv == 0.0f ? 0.0f : __uint_as_float(o[8 * v + e]) * inv;
+          const uint4 y = S::pack(f);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                           stage + lane * 128 + ((v ^ (lane & 7)) << 4)),
+                       "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w)
+                       : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          const int row = v * 4 + (lane >> 3), ch = lane & 7;
+          uint4 y;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                       : "r"(stage + row * 128 + ((ch ^ (row & 7)) << 4))
+                       : "memory");
+          const int64_t to_row = __shfl_sync(0xffffffffu, mine ? at_row : -1, row);
+          if (to_row >= 0) st_vec(static_cast<T*>(a.out) + to_row + c + ch * 8, y);
+        }
+        __syncwarp();
       }
       fence_before();
     }
@@ -685,72 +936,65 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the sums of a cell's pieces, in order: one warp per row.
+// Joins the pieces of the cells that were cut, in order: blocks (c, *) look
+// after the cell whose first cut is the end of CTA c's run, a warp per row.
+constexpr int kJoinBlocks = 8;
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-    paged_chunk_join_kernel(const __grid_constant__ PagedAttnArgs a, TcWork w) {
+    paged_chunk_join_kernel(const __grid_constant__ PagedAttnArgs a, TcWork w, int grid) {
   using S = Storage<T>;
-  const int cell = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int shift = ilog2(a.page_size), G = a.n_q_heads / a.n_kv_heads;
-  pdl_wait();
   constexpr int E = HD / 32;
-  for (int rr = blockIdx.y * 8 + warp; rr < 2 * kRows; rr += gridDim.y * 8) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int shift = ilog2(a.page_size), G = a.n_q_heads / a.n_kv_heads;
+  const int pair = 2 * (kRows / G);
+  pdl_wait();
+  int64_t before;
+  bool bad_lengths;
+  const int64_t total = line_length(a, shift, pair, lane, &before, &bad_lengths);
+  const int64_t share = (total + grid - 1) / grid;
+  const int64_t x = (static_cast<int64_t>(blockIdx.x) + 1) * share;
+  if (x >= total) return;
+  const Walk c = find_cell(a, shift, pair, before, x);
+  const int first = cut_at(x, c);
+  if (first == 0 || first == c.n || cut_at(x - share, c) > 0) return;
+  for (int rr = blockIdx.y * 8 + warp; rr < 2 * kRows; rr += kJoinBlocks * 8) {
     const int i = rr / kRows, r = rr % kRows;
-    float M = -INFINITY, lsum = 0.0f, o[E];
+    const int tok = (2 * c.t + i) * c.rows_tok + r / G, g = r % G;
+    if (r >= G * c.rows_tok || tok >= c.s.rows) continue;
+    float M = -INFINITY, sum = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    Piece p;
-    for (int s = 0; s < w.splits; ++s) {
-      p = piece_of(a, w, cell * w.splits + s, shift, G);
-      if (p.k >= p.tiles || p.s.len == 0) return;
-      if (p.count[i] == 0) continue;
-      const int64_t row = (static_cast<int64_t>(cell) * w.splits + s) * 2 * kRows + rr;
-      const float2 ml = w.ml[row];
+    int j = 0;
+    for (int64_t cta = blockIdx.x; j < c.n; ++cta) {
+      const int to = cut_at((cta + 1) * share, c);
+      if (to == j) continue;              // no piece of it there
+      const int64_t row = (2 * cta + (j > 0 ? 0 : 1)) * 2 * kRows + rr;
+      j = to;
+      const float2 ml = __ldcg(w.ml + row);
+      if (ml.x == -INFINITY) continue;    // the row sees nothing of it
       const float m_new = fmaxf(M, ml.x);
-      const float f0 = M == -INFINITY ? 0.0f : exp2f(M - m_new);
-      const float f1 = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m_new);
+      const float f0 = exp2f(M - m_new), f1 = exp2f(ml.x - m_new);
       M = m_new;
-      lsum = lsum * f0 + ml.y * f1;
+      sum = sum * f0 + ml.y * f1;
       const float* src = w.part + row * HD + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + (f1 == 0.0f ? 0.0f : src[e] * f1);
+      for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + __ldcg(src + e) * f1;
     }
-    const int tok = p.tok0 + i * p.rows_tok + r / G, g = r % G;
-    if (r >= G * p.rows_tok || tok >= p.s.rows) continue;
-    const float inv = lsum > 0.0f || lsum != lsum ? 1.0f / lsum : 0.0f;
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(p.s.start + tok) * a.out_row_stride +
-             static_cast<int64_t>(p.h * G + g) * HD + lane * E;
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(c.s.start + tok) * a.out_row_stride +
+             static_cast<int64_t>(c.h * G + g) * HD + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) out[e] = S::from_float(o[e] * inv);
   }
 }
 
-TcWork plan(int64_t tokens, int64_t batch, int64_t max_q_len, int n_q_heads, int n_kv_heads,
-            int64_t max_positions) {
-  TcWork w{};
-  const int64_t pair = 2 * (kRows / (n_q_heads / n_kv_heads));
-  const int64_t tiles = (max_q_len + pair - 1) / pair;
-  w.tiles = static_cast<int>(tiles);
-  const int64_t cells = tiles * batch * n_kv_heads;
-  w.cells = cells > 0x3fffffff ? 0 : static_cast<int>(cells);   // the loops count in ints
-  // cells that can hold rows
-  int64_t live = tokens / pair + batch;
-  if (live > tiles * batch) live = tiles * batch;
-  live *= n_kv_heads;
-  int64_t splits = sm_count() / (live > 0 ? live : 1);
-  const int64_t most = max_positions / (4 * kTile);    // four tiles a piece, at least
-  if (splits > most) splits = most;
-  w.splits = splits < 1 ? 1 : static_cast<int>(splits);
-  return w;
-}
+int chunk_grid() { return sm_count(); }
 
 template <typename T, int HD>
 cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cudaStream_t stream) {
   const int G = a.n_q_heads / a.n_kv_heads;
-  const int64_t max_q_len = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
-  TcWork w = plan(a.tokens, a.batch, max_q_len, a.n_q_heads, a.n_kv_heads,
-                  static_cast<int64_t>(a.max_pages) * a.page_size);
-  const int64_t rows = static_cast<int64_t>(w.cells) * w.splits * 2 * kRows;
+  TcWork w;
+  const int64_t rows = static_cast<int64_t>(chunk_grid()) * 2 * 2 * kRows;
   w.ml = static_cast<float2*>(workspace);
   w.part = reinterpret_cast<float*>(w.ml + rows);
   const int box = a.page_size < kTile ? a.page_size : kTile;
@@ -776,26 +1020,22 @@ cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cuda
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
-  const int pieces = w.cells * w.splits;
-  const int grid = pieces < sm_count() ? pieces : sm_count();
+  const int grid = chunk_grid();
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, pdl, a,
                     qmap, kmap, vmap, w, box_shift);
-  if (e != cudaSuccess || w.splits == 1) return e;
+  // a table too short for a cell that could be cut needs no join
+  if (e != cudaSuccess || static_cast<int64_t>(a.max_pages) * a.page_size <= (2 * kMinPiece - 1) * kTile)
+    return e;
   return launch_kernel(paged_chunk_join_kernel<T, HD>,
-                       dim3(static_cast<unsigned>(w.cells), 8), dim3(256), 0, stream, true, a, w);
+                       dim3(static_cast<unsigned>(grid), kJoinBlocks), dim3(256), 0, stream, true,
+                       a, w, grid);
 }
 
 }  // namespace
 
-size_t paged_attention_tc_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
-                                          int n_q_heads, int n_kv_heads, int head_dim) {
-  if (max_q_len > tokens) max_q_len = tokens;
-  // pieces are at most SMs where there are any, whatever the lengths
-  const TcWork w = plan(tokens, batch, max_q_len, n_q_heads, n_kv_heads, int64_t(1) << 40);
-  if (w.cells == 0) return 0;
-  if (w.splits == 1) return 16;
-  return static_cast<size_t>(w.cells) * w.splits * 2 * kRows *
-         (static_cast<size_t>(head_dim) * 4 + 8);
+size_t paged_attention_tc_workspace_bytes(int head_dim) {
+  return static_cast<size_t>(chunk_grid()) * 2 * 2 * kRows *
+         (static_cast<size_t>(head_dim) * 4 + sizeof(float2));
 }
 
 cudaError_t launch_paged_attention_tc(const PagedAttnArgs& a, int dtype, void* workspace, bool pdl,

@@ -22,21 +22,27 @@ __device__ __forceinline__ void mbarrier_expect(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbarrier_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ bool mbarrier_test(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbarrier_test(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
+      : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
 }
-// One lane of a converged warp.  MMAs and TMA copies take their operands from
-// uniform registers: issued one lane at a time behind a lane test they cost
-// about 200 cycles each, behind an elected lane of a converged warp what the
-// hardware needs (64 for a 128 x 128 x 16 MMA).
+__device__ __forceinline__ bool mbarrier_test(uint64_t* bar, uint32_t parity) {
+  return mbarrier_test(smem_addr(bar), parity);
+}
+constexpr uint32_t kWaitPolls = 1u << 22;   // try_wait suspends: some seconds
+
+// One lane of a converged warp, to issue MMAs or TMA copies: these take their
+// operands from uniform registers, and issued lane by lane, or in a loop that
+// makes its descriptors as it goes, they cost about 200 cycles each; unrolled
+// behind an elected lane, what the hardware needs (64 for a 128 x 128 x 16
+// MMA).
 __device__ __forceinline__ bool elect_lane() {
   uint32_t on;
   asm volatile(
@@ -48,7 +54,7 @@ __device__ __forceinline__ bool elect_lane() {
 }
 // Waits for the phase of the given parity, a few seconds at most: false then.
 __device__ __forceinline__ bool mbarrier_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 22); ++i)
+  for (uint32_t i = 0; i < kWaitPolls; ++i)
     if (mbarrier_test(bar, parity)) return true;
   return false;
 }
