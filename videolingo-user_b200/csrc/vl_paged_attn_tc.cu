@@ -94,6 +94,13 @@ static_assert(sizeof(Bars) <= 1024, "barrier block");
 struct TcWork {
   float* part;        // [2 * grid][256 rows][HD]: a CTA's cut pieces
   float2* ml;         // [2 * grid][256] their (max, sum)
+  int* next;          // [2 * grid] the slot that holds the cell's next piece, or -1
+  struct CutCell* first;   // [grid] the cut cell that begins in a CTA
+};
+
+struct CutCell {
+  int row0, tokens, h;   // as in Plan
+  int cut;               // 0: none
 };
 
 // A cell is a pair of blocks of one sequence and kv head against the n tiles
@@ -141,6 +148,12 @@ __device__ __forceinline__ int64_t head_size(const SeqView& s, int pair) {
   if (s.rows == 0) return 0;
   const int past = max(0, s.len - s.rows), pairs = (s.rows + pair - 1) / pair;
   return cells_before(past, pairs - 1, pair) + past + s.rows + kCellCost;
+}
+
+// 64-bit division, at the price of a 32-bit one where that will do.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
 }
 
 // The line's length; before: where the sequences that this lane adds up
@@ -208,7 +221,7 @@ __device__ __forceinline__ Walk find_cell(const PagedAttnArgs& a, int shift, int
   while (w.b < a.batch) {
     const int64_t head = head_size(w.s, pair), into = x - w.at;
     if (into < head * a.n_kv_heads) {
-      w.h = static_cast<int>(into / head);
+      w.h = static_cast<int>(divide(into, head));
       w.at += w.h * head;
       int hi = w.pairs;                   // the last cell of the head that begins at or before x
       while (hi - w.t > 1) {
@@ -420,10 +433,11 @@ __device__ __forceinline__ float2 ex2_pair(float2 z) {
   return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(rf.x) << 23)),
                      __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(rf.y) << 23)));
 }
-// Which of the 32 pairs of half a row go that way: three of eight, spread.
-__device__ constexpr bool by_polynomial(int pair) {
-  return pair % 8 == 1 || pair % 8 == 4 || pair % 8 == 6;
-}
+// Which of the 32 pairs of half a row go that way: one in four.  A row's 128
+// exponentials then take 1190 cycles with one warp on a scheduler and 1940
+// with two, against 1360 and 2240 with none, 1350 and 2040 with three of
+// eight.
+__device__ constexpr bool by_polynomial(int pair) { return pair % 4 == 1; }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
   return pack_bf16x2(lo, hi);
 }
@@ -478,6 +492,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // The planning warp looks the lengths up while the others set up; they and
+  // the tables are not written by the kernel before this one.
+  Run run;
+  Walk at;
+  int64_t share = 0;
+  if (warp == kPlanWarp) {
+    run.shift = shift;
+    run.pair = 2 * (kRows / G);
+    int64_t before;
+    bool bad_lengths;
+    const int64_t total = line_length(a, shift, run.pair, lane, &before, &bad_lengths);
+    if (bad_lengths && blockIdx.x == 0 && a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
+    share = divide(total + gridDim.x - 1, gridDim.x);
+    run.x0 = min(total, blockIdx.x * share);
+    run.x1 = min(total, run.x0 + share);
+    at.b = a.batch;
+    if (run.x0 < run.x1) at = find_cell(a, shift, run.pair, before, run.x0);
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -497,21 +529,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp == kPlanWarp) {
-    // ---- the walk; lengths and tables are not written by the kernel before
-    // this one ----
-    Run run;
-    run.shift = shift;
-    run.pair = 2 * (kRows / G);
-    int64_t before;
-    bool bad_lengths;
-    const int64_t total = line_length(a, shift, run.pair, lane, &before, &bad_lengths);
-    if (bad_lengths && blockIdx.x == 0 && a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    run.x0 = min(total, blockIdx.x * share);
-    run.x1 = min(total, run.x0 + share);
-    Walk at;
-    at.b = a.batch;
-    if (run.x0 < run.x1) at = find_cell(a, shift, run.pair, before, run.x0);
+    // ---- the walk ----
+    CutCell begins{};
+    pdl_wait();                                        // the join before may be reading
     for (bool more = true; more; ++piece) {
       more = settle(a, run, at);
       const int slot = piece % kPlans;
@@ -534,6 +554,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           p.count[0] = block_tiles(at, 0);
           p.count[1] = block_tiles(at, 1);
           p.whole = at.j0 == 0 && at.j1 == at.n;
+          if (!p.whole) {
+            // a CTA's first piece may begin inside its cell (slot 0), its last end there
+            int then = -1;
+            if (at.j1 < at.n) {
+              int cta = blockIdx.x + 1;
+              while (cut_at((cta + 1) * share, at) == at.j1) ++cta;
+              then = 2 * cta;
+            }
+            w.next[2 * blockIdx.x + (at.j0 > 0 ? 0 : 1)] = then;
+            if (at.j0 == 0) begins = CutCell{p.row0, p.tokens, p.h, 1};
+          }
         }
         bars.plan[slot] = p;
         mbarrier_arrive(&bars.plan_full[slot]);
@@ -541,6 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (more) next_cell(a, shift, run.pair, at);
     }
+    if (lane == 0) w.first[blockIdx.x] = begins;
     // the last ones have been read before this block goes
     for (uint32_t k = piece < kPlans ? 0 : piece - kPlans; k < piece; ++k)
       if (!wait_or_bad(&bars.plan_empty[k % kPlans], (k / kPlans) & 1, &bars.bad)) break;
@@ -685,9 +717,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       Count now, then;
       bool more = next_piece(now);
       if (more) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (now.of[i] > 0) ask(i, 0, true, now.of[i] == 1);
+        if (now.of[0] > 0) {
+          ask(0, 0, true, now.of[0] == 1);
+          // the second block starts half a tile later, and stays there: one's
+          // products run under the other's exponentials
+          wait(bars.p_half[0], 0);
+        }
+        if (now.of[1] > 0) ask(1, 0, true, now.of[1] == 1);
         commit(&bars.k_empty[0]);
       }
       int jj = 0;
@@ -759,7 +795,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_load32(ts + c, x);
           tmem_load32(ts + c + 32, x + 32);
           tmem_load_wait<kTile / 2>(x);
-          if (cut) hide<kTile / 2>(x, see - pos0 - c);
+          if (cut) {
+            hide<kTile / 2>(x, see - pos0 - c);
+            tmem_store32(ts + c, x);      // for the second reading
+            tmem_store32(ts + c + 32, x + 32);
+            tmem_store_wait();
+          }
           float mz = max3(x[0], x[1], x[2]), mw = max3(x[3], x[4], x[5]);
 #pragma unroll
           for (int e = 6; e + 8 <= kTile / 2; e += 8) {
@@ -819,8 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_load32(ts + c, x);
           tmem_load32(ts + c + 32, x + 32);
           tmem_load_wait<kTile / 2>(x);
-          if (cut) {
-            hide<kTile / 2>(x, see - pos0 - c);
+          if (cut) {                      // weights that are exactly 0
 #pragma unroll
             for (int e = 0; e < kTile / 2; e += 2) {
               const float2 z = halves_of(fma2(pair_of(x[e], x[e + 1]), scale2, off2));
@@ -866,7 +906,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after();
         inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       }
-      // a CTA's first piece may begin inside its cell (slot 0), its last end there
       const int64_t row256 = (2 * static_cast<int64_t>(blockIdx.x) + (p.j0 > 0 ? 0 : 1)) * 2 * kRows +
                              i * kRows + r;
       if (!p.whole && mine) w.ml[row256] = make_float2(m, l);
@@ -901,8 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int v = 0; v < 8; ++v) {
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            f[e] = inv == 0.0f ? 0.0f : __uint_as_float(o[8 * v + e]) * inv;
+          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * v + e]) * inv;
           const uint4 y = S::pack(f);
           asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
                            stage + lane * 128 + ((v ^ (lane & 7)) << 4)),
@@ -936,59 +974,63 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the cells that were cut, in order: blocks (c, *) look
-// after the cell whose first cut is the end of CTA c's run, a warp per row.
+// Joins the pieces of the cut cell that begins in CTA blockIdx.x, in order: a
+// warp per row.
 constexpr int kJoinBlocks = 8;
+constexpr int kMaxPieces = 1024;          // of a cell: at most one per CTA
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-    paged_chunk_join_kernel(const __grid_constant__ PagedAttnArgs a, TcWork w, int grid) {
+    paged_chunk_join_kernel(const __grid_constant__ PagedAttnArgs a, TcWork w) {
   using S = Storage<T>;
-  constexpr int E = HD / 32;
+  constexpr int E = HD / 32;              // dims of a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int shift = ilog2(a.page_size), G = a.n_q_heads / a.n_kv_heads;
-  const int pair = 2 * (kRows / G);
+  const int G = a.n_q_heads / a.n_kv_heads, rows_tok = kRows / G;
+  __shared__ int slots[kMaxPieces];
+  __shared__ int pieces;
   pdl_wait();
-  int64_t before;
-  bool bad_lengths;
-  const int64_t total = line_length(a, shift, pair, lane, &before, &bad_lengths);
-  const int64_t share = (total + grid - 1) / grid;
-  const int64_t x = (static_cast<int64_t>(blockIdx.x) + 1) * share;
-  if (x >= total) return;
-  const Walk c = find_cell(a, shift, pair, before, x);
-  const int first = cut_at(x, c);
-  if (first == 0 || first == c.n || cut_at(x - share, c) > 0) return;
+  const CutCell c = w.first[blockIdx.x];
+  if (c.cut == 0) return;
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int slot = 2 * blockIdx.x + 1; slot >= 0 && n < kMaxPieces; slot = __ldcg(w.next + slot))
+      slots[n++] = slot;
+    pieces = n;
+  }
+  __syncthreads();
   for (int rr = blockIdx.y * 8 + warp; rr < 2 * kRows; rr += kJoinBlocks * 8) {
-    const int i = rr / kRows, r = rr % kRows;
-    const int tok = (2 * c.t + i) * c.rows_tok + r / G, g = r % G;
-    if (r >= G * c.rows_tok || tok >= c.s.rows) continue;
+    const int r = rr % kRows, tok = rr / kRows * rows_tok + r / G, g = r % G;
+    if (r >= G * rows_tok || tok >= c.tokens) continue;
     float M = -INFINITY, sum = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    int j = 0;
-    for (int64_t cta = blockIdx.x; j < c.n; ++cta) {
-      const int to = cut_at((cta + 1) * share, c);
-      if (to == j) continue;              // no piece of it there
-      const int64_t row = (2 * cta + (j > 0 ? 0 : 1)) * 2 * kRows + rr;
-      j = to;
+    for (int k = 0; k < pieces; ++k) {
+      const int64_t row = static_cast<int64_t>(slots[k]) * 2 * kRows + rr;
       const float2 ml = __ldcg(w.ml + row);
+      float y[E];
+      if (E == 4) {
+        const float4 q = __ldcg(reinterpret_cast<const float4*>(w.part + row * HD) + lane);
+        y[0] = q.x, y[1] = q.y, y[E - 2] = q.z, y[E - 1] = q.w;
+      } else {
+        const float2 q = __ldcg(reinterpret_cast<const float2*>(w.part + row * HD) + lane);
+        y[0] = q.x, y[1] = q.y;
+      }
       if (ml.x == -INFINITY) continue;    // the row sees nothing of it
       const float m_new = fmaxf(M, ml.x);
       const float f0 = exp2f(M - m_new), f1 = exp2f(ml.x - m_new);
       M = m_new;
       sum = sum * f0 + ml.y * f1;
-      const float* src = w.part + row * HD + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + __ldcg(src + e) * f1;
+      for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + y[e] * f1;
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(c.s.start + tok) * a.out_row_stride +
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(c.row0 + tok) * a.out_row_stride +
              static_cast<int64_t>(c.h * G + g) * HD + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) out[e] = S::from_float(o[e] * inv);
   }
 }
 
-int chunk_grid() { return sm_count(); }
+int chunk_grid() { return sm_count() < kMaxPieces ? sm_count() : kMaxPieces; }
 
 template <typename T, int HD>
 cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cudaStream_t stream) {
@@ -997,6 +1039,8 @@ cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cuda
   const int64_t rows = static_cast<int64_t>(chunk_grid()) * 2 * 2 * kRows;
   w.ml = static_cast<float2*>(workspace);
   w.part = reinterpret_cast<float*>(w.ml + rows);
+  w.first = reinterpret_cast<CutCell*>(w.part + rows * HD);
+  w.next = reinterpret_cast<int*>(w.first + chunk_grid());
   const int box = a.page_size < kTile ? a.page_size : kTile;
   int box_shift = 0;
   while ((1 << box_shift) < box) ++box_shift;
@@ -1028,14 +1072,15 @@ cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cuda
     return e;
   return launch_kernel(paged_chunk_join_kernel<T, HD>,
                        dim3(static_cast<unsigned>(grid), kJoinBlocks), dim3(256), 0, stream, true,
-                       a, w, grid);
+                       a, w);
 }
 
 }  // namespace
 
 size_t paged_attention_tc_workspace_bytes(int head_dim) {
   return static_cast<size_t>(chunk_grid()) * 2 * 2 * kRows *
-         (static_cast<size_t>(head_dim) * 4 + sizeof(float2));
+             (static_cast<size_t>(head_dim) * 4 + sizeof(float2)) +
+         static_cast<size_t>(chunk_grid()) * (sizeof(CutCell) + 2 * sizeof(int));
 }
 
 cudaError_t launch_paged_attention_tc(const PagedAttnArgs& a, int dtype, void* workspace, bool pdl,
