@@ -10,13 +10,11 @@
 // next to nothing, so it is bound by HBM, or for a decode step by the
 // latency of one round trip (q_start -> page id -> store).
 //
-// Layout: a warp takes heads of one token, a lane one 16-byte vector of a
-// head; every access of a warp is one contiguous 512 bytes.  A rotate-half
-// lane gets the other half of its pairs from the lane half a rotation away
-// by shuffle, so a vector is loaded once and the same code serves every
-// rotary_dim; interleaved pairs lie within a lane.  A lane's vector index is
-// the same in every head, so its cosines and sines are evaluated once per
-// token.  Vector loads are requested before the angles are evaluated.
+// Layout: a block takes a few tokens.  Its first threads look the tokens'
+// places up, then all of them evaluate the tokens' cosines and sines (once
+// per token, in shared memory) while the first vectors are on their way, and
+// then move 16-byte vectors: a task is the two vectors of a head that turn
+// together (one, when interleaved), or one that is only copied.
 #include <cmath>
 
 #include "vl_common.cuh"
@@ -27,125 +25,175 @@
 namespace vl {
 namespace {
 
-constexpr int kAppendWarps = 4;
-constexpr int kAppendAhead = 6;   // head rows a lane holds in flight
+constexpr int kAppendThreads = 256;
+constexpr int kAppendAhead = 4;   // tasks of a thread in flight
+constexpr int kAppendTokens = 4;  // of a block, at most
 
-// wpt warps share a token's heads (1, 2 or 4, so that few tokens still
-// spread over the SMs).
+// n / d for n, d < 2^16 by the factor ceil(2^32 / d).
+struct Divisor {
+  uint32_t d, factor;
+};
+__device__ __forceinline__ int quotient(int n, const Divisor& v) {
+  return v.d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), v.factor));
+}
+
+struct AppendTasks {
+  int turns;        // of a token: (q and k heads) * vectors (pairs of vectors) that turn
+  int tails;        // (q and k heads) * vectors behind rotary_dim
+  Divisor token;    // turns + tails + v heads * vectors
+  Divisor turn;     // turning tasks of a head
+  Divisor tail;
+  Divisor whole;    // vectors of a head
+};
+
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kAppendWarps * 32)
+__global__ void __launch_bounds__(kAppendThreads)
     paged_append_kernel(const __grid_constant__ PagedAppendArgs a,
-                        const __grid_constant__ InvFreq freq, int wpt) {
+                        const __grid_constant__ InvFreq freq,
+                        const __grid_constant__ AppendTasks tasks, int block_tokens) {
   using S = Storage<T>;
   constexpr int E = S::kVec;
-  __shared__ float2 cs_all[kAppendWarps][kMaxHalfRot];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t wid = static_cast<int64_t>(blockIdx.x) * kAppendWarps + warp;
-  const int64_t t = wid / wpt;
-  const int part = static_cast<int>(wid % wpt);
-  if (t >= a.tokens) return;
+  constexpr int G = kAppendAhead;
+  __shared__ __align__(16) float2 cs[kAppendTokens * kMaxHalfRot];
+  __shared__ int64_t s_at[kAppendTokens];   // the cache row's offset, -1: not cached, -2: no token
+  __shared__ int s_pos[kAppendTokens];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * block_tokens;
+  const int nt = static_cast<int>(min(static_cast<int64_t>(block_tokens), a.tokens - t0));
+  const int half = a.rotary_dim / 2, half_vecs = half / E;
+  const int kv0 = a.n_q_heads;
+  const int count = nt * static_cast<int>(tasks.token.d);
 
-  const int nv = a.head_dim / E;            // vectors of a head, <= 32
-  const int hpw = 32 / nv;                  // heads of a warp row
-  const int v = lane % nv, hl = lane / nv;
-  const bool lane_on = hl < hpw;
-  const int heads = a.n_q_heads + 2 * a.n_kv_heads;
-  const int kv0 = a.n_q_heads, v0 = a.n_q_heads + a.n_kv_heads;
-  const int half_vecs = a.rotary_dim / 2 / E;   // rotate-half: vectors of a half
-  const bool rotates = v * E < a.rotary_dim;
-
-  auto source = [&](int h) -> const T* {
-    if (h < kv0)
-      return static_cast<const T*>(a.q) + t * a.q_row_stride + static_cast<int64_t>(h) * a.head_dim;
-    if (h < v0)
-      return static_cast<const T*>(a.k) + t * a.k_row_stride +
-             static_cast<int64_t>(h - kv0) * a.head_dim;
-    return static_cast<const T*>(a.v) + t * a.v_row_stride +
-           static_cast<int64_t>(h - v0) * a.head_dim;
+  struct Task {
+    int token, head, vec;   // head: q, then k, then v heads
+    bool turns;
   };
-  const int step = hpw * wpt;
-  uint4 x[kAppendAhead];
-  auto load = [&](int h0) {
+  auto task_of = [&](int n) {
+    Task k;
+    k.token = quotient(n, tasks.token);
+    int m = n - k.token * static_cast<int>(tasks.token.d);
+    k.turns = m < tasks.turns;
+    if (k.turns) {
+      k.head = quotient(m, tasks.turn);
+      k.vec = m - k.head * static_cast<int>(tasks.turn.d);
+    } else if ((m -= tasks.turns) < tasks.tails) {
+      k.head = quotient(m, tasks.tail);
+      k.vec = a.rotary_dim / E + m - k.head * static_cast<int>(tasks.tail.d);
+    } else {
+      m -= tasks.tails;
+      const int h = quotient(m, tasks.whole);
+      k.head = kv0 + a.n_kv_heads + h;
+      k.vec = m - h * static_cast<int>(tasks.whole.d);
+    }
+    return k;
+  };
+  auto source = [&](const Task& k) {
+    const int64_t t = t0 + k.token;
+    const T* row;
+    int h = k.head;
+    if (h < kv0) {
+      row = static_cast<const T*>(a.q) + t * a.q_row_stride;
+    } else if ((h -= kv0) < a.n_kv_heads) {
+      row = static_cast<const T*>(a.k) + t * a.k_row_stride;
+    } else {
+      h -= a.n_kv_heads;
+      row = static_cast<const T*>(a.v) + t * a.v_row_stride;
+    }
+    return row + static_cast<int64_t>(h) * a.head_dim + k.vec * E;
+  };
+  uint4 x1[G], x2[G];
+  auto load = [&](int n0) {                 // readable whether or not a sequence holds the token
 #pragma unroll
-    for (int i = 0; i < kAppendAhead; ++i) {
-      const int h = h0 + i * step + hl;
-      if (lane_on && h < heads) x[i] = ld_vec(source(h) + v * E);
+    for (int g = 0; g < G; ++g) {
+      const int n = n0 + g * kAppendThreads;
+      if (n < count) {
+        const Task k = task_of(n);
+        const T* src = source(k);
+        x1[g] = ld_vec(src);
+        if (!kInterleaved && k.turns) x2[g] = ld_vec(src + half);
+      }
     }
   };
-  // the rows are readable whether or not a sequence holds them
-  load(part * hpw);
+  load(tid);
 
-  const int b = find_sequence(a.q_start, a.batch, t, lane);
-  const int64_t q0 = a.q_start[b], q1 = a.q_start[b + 1];
-  if (t < q0 || t >= q1) return;            // behind the last sequence
-  const int64_t pos = static_cast<int64_t>(a.kv_len[b]) - (q1 - t);
-  const int shift = ilog2(a.page_size);
-  const int64_t page_at = pos >> shift;
-  int64_t page = -1;
-  if (pos >= 0 && page_at < a.max_pages) page = a.page_table[b * a.table_stride + page_at];
-  const bool cached = page >= 0 && page < a.num_pages;
-  if (!cached && part == 0 && lane == 0 && a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
-  const int64_t at = page * a.page_stride +
-                     (pos & (a.page_size - 1)) * static_cast<int64_t>(a.n_kv_heads) * a.head_dim;
-
-  float2* cs = cs_all[warp];
-  const double angle = static_cast<double>(pos) * a.position_scale;
-  for (int d = lane; d < a.rotary_dim / 2; d += 32) cs[d] = rope_cos_sin(angle * freq.v[d]);
-  __syncwarp();
-  float c[E], s[E];
-  if (kInterleaved) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float2 p = rotates ? cs[v * (E / 2) + e / 2] : make_float2(1.0f, 0.0f);
-      c[e] = p.x;
-      s[e] = (e & 1) ? p.y : -p.y;          // x1' = x1 c - x2 s, x2' = x2 c + x1 s
+  if (warp < nt) {                          // a token's place
+    const int64_t t = t0 + warp;
+    const int b = find_sequence(a.q_start, a.batch, t, lane);
+    const int64_t q0 = a.q_start[b], q1 = a.q_start[b + 1];
+    const int64_t pos = static_cast<int64_t>(a.kv_len[b]) - (q1 - t);
+    int64_t at = -2;
+    if (t >= q0 && t < q1) {
+      const int64_t page_at = pos >> ilog2(a.page_size);
+      int64_t page = -1;
+      if (pos >= 0 && page_at < a.max_pages) page = a.page_table[b * a.table_stride + page_at];
+      at = -1;
+      if (page >= 0 && page < a.num_pages)
+        at = page * a.page_stride +
+             (pos & (a.page_size - 1)) * static_cast<int64_t>(a.n_kv_heads) * a.head_dim;
+      else if (lane == 0 && a.status)
+        atomicOr(a.status, VL_STATUS_BAD_PAGE);
     }
-  } else {
-    const bool second = v >= half_vecs;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float2 p = rotates ? cs[(second ? v - half_vecs : v) * E + e] : make_float2(1.0f, 0.0f);
-      c[e] = p.x;
-      s[e] = second ? p.y : -p.y;
+    if (lane == 0) {
+      s_at[warp] = at;
+      s_pos[warp] = static_cast<int>(pos);
     }
   }
-  const int partner = kInterleaved || !rotates ? lane
-                      : (v >= half_vecs ? lane - half_vecs : lane + half_vecs);
+  __syncthreads();
+  for (int i = tid; i < nt * half; i += kAppendThreads) {
+    const int t = i / half, d = i - t * half;
+    cs[t * kMaxHalfRot + d] =
+        rope_cos_sin(static_cast<double>(s_pos[t]) * a.position_scale * freq.v[d]);
+  }
+  __syncthreads();
 
-  for (int h0 = part * hpw; h0 < heads; h0 += kAppendAhead * step) {
-    if (h0 != part * hpw) load(h0);
+  for (int n0 = tid; n0 < count; n0 += G * kAppendThreads) {
+    if (n0 != tid) load(n0);
 #pragma unroll
-    for (int i = 0; i < kAppendAhead; ++i) {
-      const int hw = h0 + i * step;         // warp-uniform
-      if (hw >= heads) break;
-      const int h = hw + hl;
-      uint4 o = x[i];
-      if (!kInterleaved) {
-        o.x = __shfl_sync(0xffffffffu, x[i].x, partner);
-        o.y = __shfl_sync(0xffffffffu, x[i].y, partner);
-        o.z = __shfl_sync(0xffffffffu, x[i].z, partner);
-        o.w = __shfl_sync(0xffffffffu, x[i].w, partner);
-      }
-      if (!lane_on || h >= heads) continue;
-      uint4 y = x[i];
-      if (h < v0 && rotates) {
-        float f[E], g[E], r[E];
-        S::unpack(x[i], f);
-        S::unpack(o, g);
-#pragma unroll
-        for (int e = 0; e < E; ++e) r[e] = f[e] * c[e] + (kInterleaved ? g[e ^ 1] : g[e]) * s[e];
-        y = S::pack(r);
-      }
+    for (int g = 0; g < G; ++g) {
+      const int n = n0 + g * kAppendThreads;
+      if (n >= count) break;
+      const Task k = task_of(n);
+      const int64_t at = s_at[k.token];
+      if (at == -2 || (at == -1 && k.head >= kv0)) continue;
       T* dst;
-      if (h < kv0) {
-        dst = static_cast<T*>(a.q_out) + t * a.q_out_row_stride +
-              static_cast<int64_t>(h) * a.head_dim;
-      } else {
-        if (!cached) continue;
-        dst = h < v0 ? static_cast<T*>(a.k_cache) + at + static_cast<int64_t>(h - kv0) * a.head_dim
-                     : static_cast<T*>(a.v_cache) + at + static_cast<int64_t>(h - v0) * a.head_dim;
+      int h = k.head;
+      if (h < kv0)
+        dst = static_cast<T*>(a.q_out) + (t0 + k.token) * a.q_out_row_stride;
+      else if ((h -= kv0) < a.n_kv_heads)
+        dst = static_cast<T*>(a.k_cache) + at;
+      else {
+        h -= a.n_kv_heads;
+        dst = static_cast<T*>(a.v_cache) + at;
       }
-      st_vec(dst + v * E, y);
+      dst += static_cast<int64_t>(h) * a.head_dim + k.vec * E;
+      if (!k.turns) {
+        st_vec(dst, x1[g]);
+        continue;
+      }
+      float p[E], y[E];
+      S::unpack(x1[g], p);
+      if (kInterleaved) {
+        const float2* cv = cs + k.token * kMaxHalfRot + k.vec * (E / 2);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 w = cv[e / 2];
+          y[e] = p[e] * w.x - p[e + 1] * w.y;
+          y[e + 1] = p[e + 1] * w.x + p[e] * w.y;
+        }
+        st_vec(dst, S::pack(y));
+      } else {
+        float r[E], z[E];
+        S::unpack(x2[g], r);
+        const float2* cv = cs + k.token * kMaxHalfRot + k.vec * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 w = cv[e];
+          y[e] = p[e] * w.x - r[e] * w.y;
+          z[e] = r[e] * w.x + p[e] * w.y;
+        }
+        st_vec(dst, S::pack(y));
+        st_vec(dst + half, S::pack(z));
+      }
     }
   }
 }
@@ -214,7 +262,9 @@ cudaError_t append_typed(const PagedAppendArgs& a, cudaStream_t stream) {
   constexpr int E = Storage<T>::kVec;
   const InvFreq freq = make_inv_freq(a.base, a.rotary_dim);
   const bool rot_vec = a.interleaved ? a.rotary_dim % E == 0 : (a.rotary_dim / 2) % E == 0;
-  const bool vec = a.head_dim % E == 0 && a.head_dim / E <= 32 && rot_vec &&
+  // (the task numbers of a block stay below 2^16)
+  const bool vec = a.head_dim % E == 0 && rot_vec &&
+                   (a.n_q_heads + 2 * a.n_kv_heads) * (a.head_dim / E) <= 16384 &&
                    a.page_stride % E == 0 && a.k_row_stride % E == 0 && a.v_row_stride % E == 0 &&
                    aligned16(a.k) && aligned16(a.v) && aligned16(a.k_cache) &&
                    aligned16(a.v_cache) &&
@@ -224,15 +274,29 @@ cudaError_t append_typed(const PagedAppendArgs& a, cudaStream_t stream) {
     paged_append_scalar_kernel<T><<<static_cast<unsigned>(a.tokens), 128, 0, stream>>>(a, freq);
     return cudaGetLastError();
   }
-  const int64_t sms = sm_count();
-  const int wpt = a.tokens <= 4 * sms ? 4 : (a.tokens <= 8 * sms ? 2 : 1);
-  const int64_t blocks = (a.tokens * wpt + kAppendWarps - 1) / kAppendWarps;
-  if (a.interleaved)
-    paged_append_kernel<T, true>
-        <<<static_cast<unsigned>(blocks), kAppendWarps * 32, 0, stream>>>(a, freq, wpt);
-  else
-    paged_append_kernel<T, false>
-        <<<static_cast<unsigned>(blocks), kAppendWarps * 32, 0, stream>>>(a, freq, wpt);
+  const int nv = a.head_dim / E, qk = a.n_q_heads + a.n_kv_heads;
+  const int turn = a.interleaved ? a.rotary_dim / E : a.rotary_dim / 2 / E;
+  const int tail = nv - a.rotary_dim / E;
+  auto divisor = [](int d) {
+    const uint32_t u = d > 0 ? d : 1;
+    return Divisor{u, static_cast<uint32_t>(((uint64_t(1) << 32) + u - 1) / u)};
+  };
+  AppendTasks tasks;
+  tasks.turns = qk * turn;
+  tasks.tails = qk * tail;
+  tasks.token = divisor(tasks.turns + tasks.tails + a.n_kv_heads * nv);
+  tasks.turn = divisor(turn);
+  tasks.tail = divisor(tail);
+  tasks.whole = divisor(nv);
+  // tokens of a block: enough for every thread to have its tasks in flight,
+  // but one while there are few blocks
+  int block_tokens = kAppendAhead * kAppendThreads / static_cast<int>(tasks.token.d);
+  if (block_tokens > kAppendTokens) block_tokens = kAppendTokens;
+  if (block_tokens < 1 || a.tokens <= 2 * sm_count()) block_tokens = 1;
+  const int64_t blocks = (a.tokens + block_tokens - 1) / block_tokens;
+  auto kernel = a.interleaved ? paged_append_kernel<T, true> : paged_append_kernel<T, false>;
+  kernel<<<static_cast<unsigned>(blocks), kAppendThreads, 0, stream>>>(a, freq, tasks,
+                                                                       block_tokens);
   return cudaGetLastError();
 }
 
