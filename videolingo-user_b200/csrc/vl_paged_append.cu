@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kAppendThreads)
   using S = Storage<T>;
   constexpr int E = S::kVec;
   constexpr int G = kAppendAhead;
+  constexpr int kPairs = kInterleaved ? E / 2 : E;   // of a task
   __shared__ __align__(16) float2 cs[kAppendTokens * kMaxHalfRot];
   __shared__ int64_t s_at[kAppendTokens];   // the cache row's offset, -1: not cached, -2: no token
   __shared__ int s_pos[kAppendTokens];
@@ -138,11 +139,18 @@ __global__ void __launch_bounds__(kAppendThreads)
       s_pos[warp] = static_cast<int>(pos);
     }
   }
+  // The frequencies are a kernel parameter: read through a generic address,
+  // as constants they would be fetched one lane at a time.
+  const double* freqs = freq.v;
+  asm volatile("" : "+l"(freqs));
+  const int my_d = tid % (half > 0 ? half : 1);
+  const double my_f = tid < half * nt ? freqs[my_d] : 0.0;
   __syncthreads();
   for (int i = tid; i < nt * half; i += kAppendThreads) {
     const int t = i / half, d = i - t * half;
-    cs[t * kMaxHalfRot + d] =
-        rope_cos_sin(static_cast<double>(s_pos[t]) * a.position_scale * freq.v[d]);
+    // pair e of vector j at [e][j]: the lanes of a warp read neighbours
+    cs[t * kMaxHalfRot + d % kPairs * (half / kPairs) + d / kPairs] =
+        rope_cos_sin(static_cast<double>(s_pos[t]) * a.position_scale * (i == tid ? my_f : freqs[d]));
   }
   __syncthreads();
 
@@ -173,10 +181,10 @@ __global__ void __launch_bounds__(kAppendThreads)
       float p[E], y[E];
       S::unpack(x1[g], p);
       if (kInterleaved) {
-        const float2* cv = cs + k.token * kMaxHalfRot + k.vec * (E / 2);
+        const float2* cv = cs + k.token * kMaxHalfRot + k.vec;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
-          const float2 w = cv[e / 2];
+          const float2 w = cv[e / 2 * (half / kPairs)];
           y[e] = p[e] * w.x - p[e + 1] * w.y;
           y[e + 1] = p[e + 1] * w.x + p[e] * w.y;
         }
@@ -184,10 +192,10 @@ __global__ void __launch_bounds__(kAppendThreads)
       } else {
         float r[E], z[E];
         S::unpack(x2[g], r);
-        const float2* cv = cs + k.token * kMaxHalfRot + k.vec * E;
+        const float2* cv = cs + k.token * kMaxHalfRot + k.vec;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float2 w = cv[e];
+          const float2 w = cv[e * (half / kPairs)];
           y[e] = p[e] * w.x - r[e] * w.y;
           z[e] = r[e] * w.x + p[e] * w.y;
         }
