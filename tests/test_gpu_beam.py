@@ -140,6 +140,21 @@ def test_select_ties_go_to_the_lower_index(dev):
     assert tok.tolist() == [[77] * 4] and par.tolist() == [[0, 1, 2, 3]]
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("beams", [1, 4, 32])
+def test_select_more_candidates_than_the_heap_holds(dev, name, beams):
+    """Rows in ascending order (every value beats the ones before it) and rows
+    of few values (nearly all candidates are ties)."""
+    vocab = 20000
+    up = torch.linspace(-8.0, 8.0, vocab).to(torch_dtype(name)).repeat(2 * beams, 1)
+    up[1:] -= 0.25 * torch.arange(1, 2 * beams).view(-1, 1).to(torch_dtype(name))
+    scores = -torch.linspace(0, 3, 2 * beams).view(2, beams) * 1.7
+    run_select(dev, up.to(dev), scores)
+    g = torch.Generator(device="cpu").manual_seed(16)
+    few = torch.randint(0, 3, (2 * beams, vocab), generator=g).to(torch_dtype(name))
+    run_select(dev, few.to(dev), scores)
+
+
 def test_select_in_place_repeated_and_captured(dev):
     """scores_out = scores and finished_out = finished, captured and replayed."""
     batch, beams, vocab = 2, 4, 5000

@@ -4,31 +4,35 @@
 // Selection.  A live beam b offers token v at s_b + l_bv - lse_b with
 // lse_b = log sum_v exp(l_bv); the entry keeps the `beams` largest values,
 // ties to the lower b * vocab + v.  Within a row the order is that of the
-// logits, so the logits are read once: a row is cut into pieces that fit the
-// registers of one CTA, which finds the piece's maximum, its sum of
-// exponentials about that maximum and its `beams` largest logits; a second
-// launch merges the pieces of the rows and the rows of an entry.  It is
-// bound by the read of the logits, or for one entry by two launches'
-// latency.
-//   * Largest logits of a warp: the K-th largest of the 32 lane maxima is a
-//     lower bound of the warp's K-th largest value, and few values reach it;
-//     only the vectors that do are looked at element by element and
-//     inserted into a list held one entry per lane.  Values are visited in
-//     index order, so equal ones keep it.
+// logits, so the logits are read once: CTAs stream pieces of rows and keep
+// the maximum, the sum of exponentials about it and the `beams` largest
+// logits; a second launch merges the pieces of the rows and the rows of an
+// entry.  It is bound by the read of the logits (about eight instructions an
+// element keep up with it), or for one entry by two launches' latency.
+//   * The K-th largest of the lanes' maxima of the first round bounds the K-th
+//     largest value from below and lets few values through (a few dozen of
+//     50,000, as what gets through raises the bound again): these go to a
+//     heap in shared memory, which is sorted at the end.  What does not fit
+//     (rows in ascending order, rows of equal values) goes to a list per warp,
+//     one entry a lane, best first, whose last entry then is the bound;
+//     values come in index order, so equal ones keep it.  Inserting into a
+//     list takes a warp some 700 cycles, a place on the heap a lane 100.
 //   * Lists are merged pairwise as bitonic sequences, five exchanges each.
-//   * exp is evaluated on l - max of the lane's own values, summed in fp32
-//     per lane (at most 64 terms) and in fp64 above that, and values are
-//     compared in fp64: beams are told apart to about 1e-7.
+//   * exp is taken of l - max (of the lane's values so far), summed in fp32
+//     per lane and in fp64 above that; values are compared in fp64: beams are
+//     told apart to about 1e-7.
 //
 // Reordering.  See vl_paged_beam_reorder in vl_api.h for the rule.  Every
 // CTA of an entry works the small plan out for itself (a bitmap of the
 // entry's range in shared memory), so one launch does tables and copies and
 // nothing waits for another CTA.
+#include <atomic>
 #include <cmath>
 
 #include "vl_common.cuh"
 #include "vl_kernels.h"
 #include "vl_paged.cuh"
+#include "vl_tma.cuh"
 
 namespace vl {
 namespace {
@@ -65,14 +69,37 @@ __device__ __forceinline__ void merge_lists(V& v, int& i, V w, int j, int lane) 
   }
 }
 
+// 32 entries in any order into a list.
+template <typename V>
+__device__ __forceinline__ void sort_list(V& v, int& i, int lane) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1) {      // runs of n, every other one turned round
+#pragma unroll
+    for (int s = n >> 1; s > 0; s >>= 1) {
+      const V ov = __shfl_xor_sync(0xffffffffu, v, s);
+      const int oi = __shfl_xor_sync(0xffffffffu, i, s);
+      const bool first = ((lane & s) == 0) == ((lane & n) == 0);
+      if (better(ov, oi, v, i) == first) {
+        v = ov;
+        i = oi;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // selection, launch 1: a piece of a row per CTA
 // ---------------------------------------------------------------------------
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 256;         // that read logits; one more warp brings them in
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelVecs = 8;              // 16-byte vectors a thread holds
+constexpr int kSelBlock = kSelThreads + 32;
+constexpr int kSelVecs = 8;              // 16-byte vectors of a thread at a time
+constexpr int kSelStage = kSelThreads * kSelVecs * 16;   // bytes of all threads'
+constexpr int kHeap = 512;               // candidates of a piece outside the lists
+constexpr int kSelStages = 3;            // on their way, or being read
+constexpr float kLog2e = 1.4426950408889634f;
 
-// A piece's result: its largest logits and sum of exp(l - max).
+// A piece's sum of exp(l - max).
 struct PieceSum {
   double sum;
   float max;
@@ -87,10 +114,13 @@ __device__ __forceinline__ int float_key(float x) {
 __device__ __forceinline__ float key_float(int k) {
   return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
+__device__ __forceinline__ void readers_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kSelThreads) : "memory");
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kSelThreads)
-    beam_piece_kernel(const __grid_constant__ BeamSelectArgs a, int pieces, int64_t piece_vecs,
+__global__ void __launch_bounds__(kSelBlock)
+    beam_piece_kernel(const __grid_constant__ BeamSelectArgs a, int pieces,
                       PieceSum* __restrict__ sums, float* __restrict__ vals,
                       int* __restrict__ ids) {
   using S = Storage<T>;
@@ -99,124 +129,301 @@ __global__ void __launch_bounds__(kSelThreads)
   __shared__ int s_id[kSelWarps][32];
   __shared__ double s_sum[kSelWarps];
   __shared__ float s_max[kSelWarps];
+  extern __shared__ __align__(16) unsigned char ring[];   // [kSelStages][kSelStage]
+  __shared__ uint64_t full[kSelStages], empty[kSelStages];
+  __shared__ uint4 s_edge[kSelWarps];
+  __shared__ float heap_val[kHeap];        // candidates, in no order
+  __shared__ int heap_id[kHeap];
+  __shared__ int s_heaped;                 // places given out, of any number
+  __shared__ int s_bad;                    // a wait ran out
+  __shared__ int s_bound;                  // key of a value that K values of the piece reach
   const int64_t row = blockIdx.y;
   const int piece = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_release();
   if (a.finished != nullptr && a.finished[row]) return;   // the merge does not read its pieces
 
-  // The row as 16-byte vectors from the boundary at or below its start;
-  // vectors that reach outside the row are read element by element.
+  // The row's whole 16-byte vectors, cut evenly; its first piece also has the
+  // elements before them, its last those behind.
   const T* base = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  const T* first = base - mis;
-  const int64_t end = a.vocab + mis;       // vector elements [mis, end) are the row's
-  const int64_t v0 = static_cast<int64_t>(piece) * piece_vecs;
-  const int64_t v1 = min(v0 + piece_vecs, (end + E - 1) / E);
-  uint4 raw[kSelVecs];
-  float vmax[kSelVecs];
-#pragma unroll
-  for (int i = 0; i < kSelVecs; ++i) {
-    const int64_t j = v0 + i * kSelThreads + tid;
-    const int64_t e0 = j * E;
-    if (j < v1 && e0 >= mis && e0 + E <= end) {
-      raw[i] = ld_stream(first + e0);
-    } else {
-      float f[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        f[e] = j < v1 && e0 + e >= mis && e0 + e < end ? S::to_float(first[e0 + e]) : kNegInf;
-      raw[i] = S::pack(f);
-    }
-  }
-  float m = kNegInf;
-#pragma unroll
-  for (int i = 0; i < kSelVecs; ++i) {
-    float f[E];
-    S::unpack(raw[i], f);
-    float x = f[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) x = fmaxf(x, f[e]);
-    vmax[i] = x;
-    m = fmaxf(m, x);
-  }
-  // a NaN makes the sum NaN, +inf makes it NaN too (inf - inf)
-  float l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kSelVecs; ++i) {
-    float f[E];
-    S::unpack(raw[i], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      l += f[e] == kNegInf ? 0.0f : exp2f((f[e] - m) * 1.44269504f);
-  }
+  const int vocab = static_cast<int>(a.vocab);
+  const int head = min(vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) /
+                                  static_cast<int>(sizeof(T)));
+  const int vecs = (vocab - head) / E;
+  const int v0 = static_cast<int>(static_cast<int64_t>(vecs) * piece / pieces);
+  const int v1 = static_cast<int>(static_cast<int64_t>(vecs) * (piece + 1) / pieces);
+  const uint4* whole = reinterpret_cast<const uint4*>(base + head);
 
-  // the warp's maximum, sum and K-th largest lane maximum
-  const int key = float_key(m);
-  const float wm = key_float(__reduce_max_sync(0xffffffffu, key));
-  double sum = l == 0.0f ? 0.0 : static_cast<double>(l) * exp2(static_cast<double>(m - wm) * 1.4426950408889634);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  int rest = key, bound = key;
-  for (int k = 0; k < a.beams; ++k) {
-    bound = __reduce_max_sync(0xffffffffu, rest);
-    if (k + 1 == a.beams) break;
-    const unsigned at = __ballot_sync(0xffffffffu, rest == bound);
-    if (lane == __ffs(at) - 1) rest = static_cast<int>(0x80000000);
-  }
-  // (with K = 32 the last of them; lanes already taken out count lowest)
-  const float floor_val = bound == static_cast<int>(0x80000000) ? kNegInf : key_float(bound);
-
-  float lv = kNegInf;
+  float m = kNegInf, l = 0.0f;             // this lane's maximum and sum about it
+  float lv = kNegInf, worst = kNegInf;     // the warp's list: value, index of entry `lane`
   int li = kNoIndex;
-  float worst = kNegInf;
+  uint4 nothing;
+  {
+    float f[E];
 #pragma unroll
-  for (int i = 0; i < kSelVecs; ++i) {
-    unsigned todo = __ballot_sync(0xffffffffu, vmax[i] >= floor_val && vmax[i] > worst);
-    while (todo) {
-      const int src = __ffs(todo) - 1;
-      todo &= todo - 1;
-      uint4 w;
-      w.x = __shfl_sync(0xffffffffu, raw[i].x, src);
-      w.y = __shfl_sync(0xffffffffu, raw[i].y, src);
-      w.z = __shfl_sync(0xffffffffu, raw[i].z, src);
-      w.w = __shfl_sync(0xffffffffu, raw[i].w, src);
+    for (int e = 0; e < E; ++e) f[e] = kNegInf;
+    nothing = S::pack(f);
+  }
+
+  // kSelVecs vectors of every lane; the i-th has place i * kSelThreads + tid,
+  // place p0 lies at from[0] in shared memory and begins at element id0 of the
+  // row.  first: nothing is listed yet.
+  auto take = [&](const uint4* raw, const uint4* from, int p0, int id0, bool first) {
+    float vmax[kSelVecs], top = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kSelVecs; ++i) {
       float f[E];
-      S::unpack(w, f);
-      const int64_t e0 = (v0 + i * kSelThreads + warp * 32 + src) * E - mis;
+      S::unpack(raw[i], f);
+      vmax[i] = fmaxf(f[0], f[1]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (f[e] > worst && f[e] >= floor_val) {       // warp-uniform
-          const int place = __popc(__ballot_sync(0xffffffffu, lv >= f[e]));
+      for (int e = 2; e < E; e += 2) vmax[i] = fmaxf(vmax[i], fmaxf(f[e], f[e + 1]));
+      top = fmaxf(top, vmax[i]);
+    }
+    // a NaN makes the sum NaN, and so does +inf (inf - inf)
+    if (top > m) {
+      l = m == kNegInf ? l : l * ex2((m - top) * kLog2e);
+      m = top;
+    }
+    const float about = m == kNegInf ? 0.0f : m;
+    const uint64_t minus = pair_of(-about, -about), log2e = pair_of(kLog2e, kLog2e);
+    uint64_t part[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kSelVecs; ++i) {
+      float f[E];
+      S::unpack(raw[i], f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 z = halves_of(mul2(add2(pair_of(f[e], f[e + 1]), minus), log2e));
+        part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], pair_of(ex2(z.x), ex2(z.y)));
+      }
+    }
+    const float2 sum2 = halves_of(add2(part[0], part[1]));
+    l += sum2.x + sum2.y;
+    if (first) {
+      // The K-th largest of all lanes' maxima: every warp's K largest, then
+      // every warp the K-th of those.
+      const int lowest = static_cast<int>(0x80000000);
+      int rest = float_key(top), kth = lowest;
+      for (int k = 0; k < a.beams; ++k) {
+        const int best = __reduce_max_sync(0xffffffffu, rest);
+        const unsigned at = __ballot_sync(0xffffffffu, rest == best);
+        if (lane == __ffs(at) - 1) rest = lowest;
+        if (lane == k) kth = best;
+      }
+      s_id[warp][lane] = kth;
+      readers_sync();
+      int of[kSelWarps];
+#pragma unroll
+      for (int w = 0; w < kSelWarps; ++w) of[w] = s_id[w][lane];
+      for (int k = 0; k < a.beams; ++k) {
+        int mine = of[0];
+#pragma unroll
+        for (int w = 1; w < kSelWarps; ++w) mine = max(mine, of[w]);
+        kth = __reduce_max_sync(0xffffffffu, mine);
+        const unsigned at = __ballot_sync(0xffffffffu, mine == kth);
+        if (lane == __ffs(at) - 1) {
+          bool taken = false;
+#pragma unroll
+          for (int w = 0; w < kSelWarps; ++w)
+            if (!taken && of[w] == kth) {
+              of[w] = lowest;
+              taken = true;
+            }
+        }
+      }
+      if (kth != lowest) {
+        if (tid == 0) atomicMax(&s_bound, kth);
+        worst = fmaxf(worst, key_float(max(kth - (kth == 0 ? 2 : 1), float_key(kNegInf))));
+      }
+    }
+    // Values at or below what K listed values of any warp beat need no
+    // listing; equal ones do, in case their index is lower, so worst stands
+    // just below (the key below +0 is -0, which no comparison tells from it).
+    const int shared = *reinterpret_cast<volatile int*>(&s_bound);
+    worst = fmaxf(worst, key_float(max(shared - (shared == 0 ? 2 : 1), float_key(kNegInf))));
+    unsigned mine = 0;                     // this lane's vectors that are worth a look
+#pragma unroll
+    for (int i = 0; i < kSelVecs; ++i) mine |= vmax[i] > worst ? 1u << i : 0u;
+    // Such values are few: they go to the piece's heap, to be sorted at the
+    // end, and a vector whose values have no room there to the warp's list.
+    unsigned full_up = 0;
+    for (unsigned look = mine; look; look &= look - 1) {
+      const int i = __ffs(look) - 1, slot = i * kSelThreads + tid - p0;
+      const T* x = reinterpret_cast<const T*>(from + slot);
+      unsigned over = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) over |= S::to_float(x[e]) > worst ? 1u << e : 0u;
+      int at = atomicAdd(&s_heaped, __popc(over));
+      if (at + __popc(over) > kHeap) {
+        full_up |= 1u << i;
+        continue;
+      }
+      for (; over; over &= over - 1, ++at) {
+        const int e = __ffs(over) - 1;
+        heap_val[at] = S::to_float(x[e]);
+        heap_id[at] = id0 + slot * E + e;
+      }
+    }
+    mine = full_up;
+    if (__ballot_sync(0xffffffffu, mine != 0) == 0) return;
+    unsigned vectors = __reduce_or_sync(0xffffffffu, mine);
+#pragma unroll 1
+    while (vectors) {                      // in index order
+      const int i = __ffs(vectors) - 1;
+      vectors &= vectors - 1;
+      unsigned todo = __ballot_sync(0xffffffffu, (mine >> i) & 1u);
+#pragma unroll 1
+      while (todo) {
+        const int slot = i * kSelThreads + warp * 32 + __ffs(todo) - 1 - p0;
+        todo &= todo - 1;
+        const float v = lane < E ? S::to_float(reinterpret_cast<const T*>(from + slot)[lane])
+                                 : kNegInf;
+        unsigned hits = __ballot_sync(0xffffffffu, v > worst);
+#pragma unroll 1
+        while (hits) {
+          const int e = __ffs(hits) - 1;
+          const float x = __shfl_sync(0xffffffffu, v, e);
+          const int place = __popc(__ballot_sync(0xffffffffu, lv >= x));
           const float uv = __shfl_up_sync(0xffffffffu, lv, 1);
           const int ui = __shfl_up_sync(0xffffffffu, li, 1);
           if (lane > place) {
             lv = uv;
             li = ui;
           } else if (lane == place) {
-            lv = f[e];
-            li = static_cast<int>(e0 + e);
+            lv = x;
+            li = id0 + slot * E + e;
           }
-          worst = __shfl_sync(0xffffffffu, lv, a.beams - 1);
+          worst = fmaxf(worst, __shfl_sync(0xffffffffu, lv, a.beams - 1));
+          hits &= hits - 1;
+          hits &= __ballot_sync(0xffffffffu, v > worst);
         }
       }
     }
+    const float last = __shfl_sync(0xffffffffu, lv, a.beams - 1);
+    if (lane == 0 && last > kNegInf) atomicMax(&s_bound, float_key(last));
+  };
+  // elements [from, to) of the row, fewer than a vector's, as this warp's
+  // lane 0's
+  auto edge = [&](int from, int to) {
+    uint4 raw[kSelVecs];
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      f[e] = lane == 0 && from + e < to ? S::to_float(base[from + e]) : kNegInf;
+    raw[0] = S::pack(f);
+#pragma unroll
+    for (int i = 1; i < kSelVecs; ++i) raw[i] = nothing;
+    if (lane == 0) s_edge[warp] = raw[0];
+    __syncwarp();
+    take(raw, s_edge + warp, warp * 32, from, false);
+  };
+
+  constexpr int kStep = kSelVecs * kSelThreads;
+  const int rounds = max(1, (v1 - v0 + kStep - 1) / kStep);
+  for (int k = tid; k < kHeap; k += kSelBlock) {
+    heap_val[k] = kNegInf;
+    heap_id[k] = kNoIndex;
   }
-  s_val[warp][lane] = lv;
-  s_id[warp][lane] = li;
+  if (tid == 0) {
+    s_bound = float_key(kNegInf);
+    s_heaped = 0;
+    s_bad = 0;
+    for (int k = 0; k < kSelStages; ++k) {
+      mbarrier_init(&full[k], 1);
+      mbarrier_init(&empty[k], kSelWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+
+  if (warp == kSelWarps) {
+    // ---- the piece's rounds, through a ring in shared memory ----
+    for (int k = 0; k < rounds; ++k) {
+      const int slot = k % kSelStages, n = min(kStep, v1 - v0 - k * kStep);
+      if (k >= kSelStages && !mbarrier_wait(&empty[slot], ((k / kSelStages) & 1) ^ 1)) {
+        if (lane == 0) s_bad = 1;
+        break;
+      }
+      const uint32_t dst = smem_addr(ring) + slot * kSelStage;
+      const uint4* src = whole + v0 + static_cast<int64_t>(k) * kStep;
+      if (n > 0 && elect_lane()) {
+        mbarrier_expect(&full[slot], n * 16);
+        bulk_load(dst, src, n * 16, &full[slot]);
+      }
+      __syncwarp();
+      if (k + 1 < rounds && k >= kSelStages) {
+        // Raise the bound: the K-th best of what is on the heap by now (what
+        // is still being written there counts as -inf).
+        const int on_heap = min(*reinterpret_cast<volatile int*>(&s_heaped), 64);
+        float best = kNegInf;
+        int none = kNoIndex;
+        for (int j = 0; j < on_heap; j += 32) {
+          float x = *reinterpret_cast<volatile float*>(&heap_val[j + lane]);
+          int id = kNoIndex;
+          sort_list(x, id, lane);
+          merge_lists(best, none, x, id, lane);
+        }
+        const float last = __shfl_sync(0xffffffffu, best, a.beams - 1);
+        if (lane == 0 && last > kNegInf) atomicMax(&s_bound, float_key(last));
+        __syncwarp();
+      }
+    }
+    return;
+  }
+
+  if (piece == 0 && warp == 0 && head > 0) edge(0, head);
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    const int at = v0 + k * kStep, slot = k % kSelStages;
+    if (at < v1 && !mbarrier_wait(&full[slot], (k / kSelStages) & 1)) s_bad = 1;
+    const uint4* stage = reinterpret_cast<const uint4*>(ring + slot * kSelStage);
+    uint4 raw[kSelVecs];
+#pragma unroll
+    for (int i = 0; i < kSelVecs; ++i) {
+      const int j = i * kSelThreads + tid;
+      raw[i] = at + j < v1 ? stage[j] : nothing;
+    }
+    take(raw, stage, 0, head + at * E, k == 0);
+    __syncwarp();
+    if (lane == 0) mbarrier_arrive(&empty[slot]);
+  }
+  if (piece == pieces - 1 && warp == kSelWarps - 1 && head + vecs * E < vocab)
+    edge(head + vecs * E, vocab);
+
+  // the warp's maximum and sum
+  const float wm = key_float(__reduce_max_sync(0xffffffffu, float_key(m)));
+  double sum = l == 0.0f ? 0.0 : static_cast<double>(l * ex2((m - wm) * kLog2e));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {
     s_sum[warp] = sum;
     s_max[warp] = wm;
   }
-  __syncthreads();
-#pragma unroll
-  for (int n = kSelWarps / 2; n > 0; n >>= 1) {
+  readers_sync();
+  // the heap into the lists, 32 candidates at a time; unless it ran over, no
+  // other list has entries
+  const int heaped = s_heaped;
+  for (int at = warp * 32; at < min(heaped, kHeap); at += kSelThreads) {
+    float x = heap_val[at + lane];
+    int id = heap_id[at + lane];
+    sort_list(x, id, lane);
+    merge_lists(lv, li, x, id, lane);
+  }
+  int n = kSelWarps / 2;
+  while (n > 0 && 32 * n >= heaped) n >>= 1;
+  if (n > 0) {
+    s_val[warp][lane] = lv;
+    s_id[warp][lane] = li;
+    readers_sync();
+  }
+#pragma unroll 1
+  for (; n > 0; n >>= 1) {
     if (warp < n) {
       merge_lists(lv, li, s_val[warp + n][lane], s_id[warp + n][lane], lane);
       s_val[warp][lane] = lv;
       s_id[warp][lane] = li;
     }
-    if (n > 1) __syncthreads();
+    if (n > 1) readers_sync();
   }
   if (warp != 0) return;
   const int64_t at = row * pieces + piece;
@@ -224,14 +431,14 @@ __global__ void __launch_bounds__(kSelThreads)
     vals[at * a.beams + lane] = lv;
     ids[at * a.beams + lane] = li;
   }
-  if (lane == 0) {
-    float cm = s_max[0];
-    for (int w = 1; w < kSelWarps; ++w) cm = fmaxf(cm, s_max[w]);
-    double cs = 0.0;
-    for (int w = 0; w < kSelWarps; ++w)
-      cs += s_sum[w] == 0.0 ? 0.0 : s_sum[w] * exp2(static_cast<double>(s_max[w] - cm) * 1.4426950408889634);
-    sums[at] = PieceSum{cs, cm, 0.0f};
-  }
+  float cm = lane < kSelWarps ? s_max[lane] : kNegInf;
+  double cs = lane < kSelWarps ? s_sum[lane] : 0.0;
+  const float top = warp_max(cm);
+  cs = cs == 0.0 ? 0.0 : cs * static_cast<double>(ex2((cm - top) * kLog2e));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) cs += __shfl_xor_sync(0xffffffffu, cs, o);
+  // (a failed piece offers nothing)
+  if (lane == 0) sums[at] = PieceSum{s_bad ? static_cast<double>(NAN) : cs, top, 0.0f};
 }
 
 // ---------------------------------------------------------------------------
@@ -283,7 +490,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
       double sum = 0.0;
       for (int p = lane; p < pieces; p += 32) {
         const PieceSum ps = sums[row * pieces + p];
-        if (ps.sum != 0.0) sum += ps.sum * exp2(static_cast<double>(ps.max - m) * 1.4426950408889634);
+        if (ps.sum != 0.0) sum += ps.sum * static_cast<double>(ex2((ps.max - m) * kLog2e));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -316,8 +523,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   int64_t token = a.pad_id;
   bool done = true;
   if (lane < a.beams && di != kNoIndex) {
-    parent = static_cast<int>(di / a.vocab);
-    token = di % a.vocab;
+    const int vocab = static_cast<int>(a.vocab);
+    parent = di / vocab;
+    token = di - parent * vocab;
     done = a.finished != nullptr && a.finished[entry * a.beams + parent];
     for (int e = 0; e < a.n_eos; ++e) done = done || token == a.eos[e];
   }
@@ -331,28 +539,39 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   }
 }
 
-// Pieces of a row: as many as its vectors need at kSelVecs per thread, cut
-// evenly.
-void select_pieces(int64_t vocab, int elems_per_vec, int* pieces, int64_t* piece_vecs) {
-  const int64_t vecs = (vocab + elems_per_vec - 1) / elems_per_vec + 1;   // a misaligned row has one more
-  const int64_t hold = static_cast<int64_t>(kSelThreads) * kSelVecs;
-  const int64_t n = (vecs + hold - 1) / hold;
-  *pieces = static_cast<int>(n);
-  *piece_vecs = (vecs + n - 1) / n;
+// Pieces of a row: two CTAs per SM keep the memory busy, and what a piece
+// costs by itself (first bound, lists, merges: as much as 100 elements a lane)
+// speaks for few, long ones; but at least one round of vectors each.  64 x 5
+// rows of 51865: 29 us in three pieces, 14 us in one.
+int select_pieces(int64_t rows, int64_t vocab, int elems_per_vec) {
+  const int64_t round = static_cast<int64_t>(kSelThreads) * kSelVecs * elems_per_vec;
+  const int64_t most = (vocab + round - 1) / round;
+  const int64_t want = (static_cast<int64_t>(sm_count()) * 2 + rows - 1) / rows;
+  const int64_t n = want < most ? want : most;
+  return static_cast<int>(n < 1 ? 1 : n);
 }
 
 template <typename T>
 cudaError_t select_typed(const BeamSelectArgs& a, void* workspace, cudaStream_t stream) {
-  int pieces;
-  int64_t piece_vecs;
-  select_pieces(a.vocab, Storage<T>::kVec, &pieces, &piece_vecs);
   const int64_t rows = a.batch * a.beams;
+  const int pieces = select_pieces(rows, a.vocab, Storage<T>::kVec);
   PieceSum* sums = static_cast<PieceSum*>(workspace);
   float* vals = reinterpret_cast<float*>(sums + rows * pieces);
   int* ids = reinterpret_cast<int*>(vals + rows * pieces * a.beams);
-  beam_piece_kernel<T><<<dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(rows)),
-                         kSelThreads, 0, stream>>>(a, pieces, piece_vecs, sums, vals, ids);
-  cudaError_t e = cudaGetLastError();
+  constexpr int smem = kSelStages * kSelStage;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(beam_piece_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  e = launch_kernel(beam_piece_kernel<T>,
+                    dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(rows)),
+                    dim3(kSelBlock), smem, stream, false, a, pieces, sums, vals, ids);
   if (e != cudaSuccess) return e;
   return launch_kernel(beam_merge_kernel, dim3(static_cast<unsigned>(a.batch)),
                        dim3(kMergeWarps * 32), 0, stream, true, a, pieces,
@@ -528,10 +747,9 @@ __global__ void __launch_bounds__(kReorderThreads)
 }  // namespace
 
 size_t beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab) {
-  int pieces;
-  int64_t piece_vecs;
-  select_pieces(vocab, Storage<float>::kVec, &pieces, &piece_vecs);   // the most pieces of any type
-  const size_t n = static_cast<size_t>(batch) * beams * pieces;
+  // (f32 rows have the most pieces)
+  const size_t n = static_cast<size_t>(batch) * beams *
+                   select_pieces(batch * beams, vocab, Storage<float>::kVec);
   return n * sizeof(PieceSum) + n * beams * (sizeof(float) + sizeof(int));
 }
 

@@ -1,5 +1,6 @@
-// Lookups shared by the paged-cache kernels: which sequence a packed row
-// belongs to, and whether a sequence's device-side lengths are usable.
+// Shared by the paged-cache and beam-search kernels: which sequence a packed
+// row belongs to, whether a sequence's device-side lengths are usable, and
+// arithmetic that fp32 code has no operators for.
 #pragma once
 
 #include "vl_common.cuh"
@@ -8,6 +9,44 @@
 namespace vl {
 
 __device__ __forceinline__ int ilog2(int pow2) { return 31 - __clz(pow2); }
+
+// The exponential unit's 2^x (relative error below 2^-22).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two floats in one 64-bit register, for the packed adds and multiply-adds
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ float2 halves_of(uint64_t x) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
 
 // The largest b in [0, batch) with q_start[b] <= row, or 0: the sequence of
 // a packed row if any holds it.  Called by a whole warp; 32 probes a round.

@@ -377,42 +377,11 @@ __device__ __forceinline__ void hide(uint32_t* r, int seen) {
 __device__ __forceinline__ void tmem_store_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;"
       : "=f"(y)
       : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
-  return y;
-}
-// two floats in one 64-bit register, for the packed adds and multiply-adds
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
-  return y;
-}
-__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
-  uint64_t y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(a), "r"(b));
-  return y;
-}
-__device__ __forceinline__ float2 halves_of(uint64_t x) {
-  float2 y;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
-  return y;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t y;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-  return y;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t y;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
   return y;
 }
 // 2^x of two values on the multiply-add pipe, beside the exponential unit:

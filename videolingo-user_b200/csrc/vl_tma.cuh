@@ -59,6 +59,16 @@ __device__ __forceinline__ bool mbarrier_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// A run of 16-byte units into shared memory (both ends on 16-byte boundaries).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // A box of a 4-D tensor map ([pages][page rows][kv heads][head dims]).
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int dim,
                                             int head, int row, int page, uint64_t* bar) {
