@@ -214,3 +214,44 @@ def test_plain_reorder_keeps_copies_and_frees():
                                           np.array([16, 16, 16], np.int32),
                                           np.array([3], np.int32), 4, kc, kc)
     assert out[:, 1].tolist() == [3, 4, 5] and np.array_equal(kc3, kc)   # fresh pages, no copies
+
+
+def test_trace_beams_follows_parents_and_stops_at_eos():
+    from vlasr.decoder import trace_beams
+    tokens = [[[10, 11]], [[12, 13]], [[9, 14]], [[9, 15]]]
+    parents = [[[0, 0]], [[1, 0]], [[0, 1]], [[0, 1]]]
+    hyps = trace_beams(tokens, parents, [[-3.0, -4.0]], eos_ids=(9,), length_penalty=1.0)
+    assert hyps == [[([11, 12, 9], -3.0, -1.0), ([10, 13, 14, 15], -4.0, -1.0)]]
+    ranked = trace_beams(tokens, parents, [[-3.0, -3.2]], eos_ids=(9,), length_penalty=1.0)
+    assert ranked[0][0][0] == [10, 13, 14, 15]              # the longer one wins per id
+    raw = trace_beams(tokens, parents, [[-3.0, -3.2]], eos_ids=(9,), length_penalty=0.0)
+    assert raw[0][0][0] == [11, 12, 9]
+    lost = trace_beams(tokens, parents, [[-3.0, float("-inf")]], eos_ids=(9,))
+    assert [len(h) for h in lost] == [1]
+
+
+def test_backend_passes_beams_on():
+    from vlasr.backend import VlasrAsrBackend
+
+    class Engine:
+        def __init__(self):
+            self.calls = []
+
+        def transcribe_ids(self, pcm, prompt_ids, max_new_tokens=256, **more):
+            self.calls.append(more)
+            return [[1]] * len(pcm)
+
+    class Processor:
+        class tokenizer:
+            @staticmethod
+            def decode(ids, skip_special_tokens=True):
+                return "word"
+
+        def apply_transcription_request(self, arrays):
+            return type("R", (), {"input_ids": [[1, 2]]})
+
+    for beams, want in ((1, {}), (4, {"beams": 4})):
+        engine = Engine()
+        VlasrAsrBackend(engine=engine, processor=Processor(), beams=beams,
+                        audio_loader=lambda path: np.ones(16000, np.float32)).transcribe("x", "en")
+        assert engine.calls == [want]

@@ -131,11 +131,13 @@ class VlasrAsrBackend:
     group        a torch.distributed process group: every rank runs the same
                  call; the chunks are sharded over the ranks (one GPU each)
                  and every rank returns the whole transcription
+    beams        beams of the decoder's search (1: greedy)
     """
 
     def __init__(self, model_dir=None, *, engine=None, processor=None, aligner=None,
                  language_resolver=None, audio_loader=None, chunk_seconds: float = 30.0,
-                 max_new_tokens: int = 256, aligner_batch: int = 4, group=None):
+                 max_new_tokens: int = 256, aligner_batch: int = 4, group=None,
+                 beams: int = 1):
         self.model_dir = Path(model_dir) if model_dir is not None else None
         self.engine = engine
         self.processor = processor
@@ -146,6 +148,7 @@ class VlasrAsrBackend:
         self.max_new_tokens = int(max_new_tokens)
         self.aligner_batch = int(aligner_batch)
         self.group = group      # a torch.distributed group: shard the chunks over its ranks
+        self.beams = int(beams)
 
     def _engine(self):
         if self.engine is None:
@@ -179,14 +182,17 @@ class VlasrAsrBackend:
 
         processor = self._processor()
         prompt_ids = list(processor.apply_transcription_request([arrays[0]]).input_ids[0])
+        search = {"beams": self.beams} if self.beams > 1 else {}
         try:
             if self.group is not None:
                 from .engine import transcribe_ids_sharded
                 per_chunk = transcribe_ids_sharded(self._engine(), arrays, prompt_ids,
-                                                   self.max_new_tokens, group=self.group)
+                                                   self.max_new_tokens, group=self.group,
+                                                   **search)
             else:
                 per_chunk = self._engine().transcribe_ids(arrays, prompt_ids,
-                                                          max_new_tokens=self.max_new_tokens)
+                                                          max_new_tokens=self.max_new_tokens,
+                                                          **search)
         except StageError:
             raise
         except Exception as exc:  # noqa: BLE001 - engine failures become stage errors

@@ -41,8 +41,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import ops
-from ._lib import VlasrInputError
+from . import ops, paged
+from ._lib import VlasrExecutionError, VlasrInputError
 
 EOS_IDS = (59246, 59253, 59255)
 AUDIO_TOKEN_ID = 59260
@@ -72,6 +72,13 @@ class DecodeResult:
     per_chunk_ids: list            # generated ids per chunk, through the first EOS
     steps: int                     # decode steps executed (lockstep rounds incl. the first id)
     forced_agreement: list | None = None   # teacher forcing: (argmax, margin) per step and chunk
+
+
+@dataclass
+class BeamResult:
+    per_chunk_ids: list            # ids of each chunk's best hypothesis, through its EOS
+    steps: int                     # decode steps executed (incl. the prefill's)
+    hypotheses: list               # per chunk, best first: (ids, log-probability, ranked score)
 
 
 class TextDecoder:
@@ -418,6 +425,184 @@ class TextDecoder:
         return DecodeResult(per_chunk_ids=self._collect(out, chunks), steps=steps,
                             forced_agreement=agreement)
 
+    # ------------------------------------------------------------------
+    # Beam search over a paged cache
+    # ------------------------------------------------------------------
+    def _paged_layers(self, h: torch.Tensor, st: dict, q_start: torch.Tensor,
+                      kv_len: torch.Tensor, table: torch.Tensor,
+                      max_q_len: int) -> torch.Tensor | None:
+        """Run the layers over packed rows `h` (updated in place) against the
+        pages of `table`; returns what the final norm still has to add."""
+        s = self.shape
+        qw, kw = s.heads * s.head_dim, s.kv_heads * s.head_dim
+        rows = h.shape[0]
+        # decode steps of a few rows through vl_decode_linear, as in step_logits
+        fused = self.fused and max_q_len == 1 and rows <= FUSED_MAX_ROWS
+        if fused:
+            ssq_a = torch.empty(s.hidden // 16, rows, dtype=torch.float32, device=self.device)
+            ssq_b = torch.empty_like(ssq_a)
+        delta = None
+        for l, lw in enumerate(self.layer_w):
+            if not fused or l == 0:
+                y = ops.add_rmsnorm(h, delta, lw["ln1"], eps=s.eps)
+                qkv = ops.decode_linear(y, lw["qkv_t"].t()) if fused else y @ lw["qkv_t"]
+            else:
+                qkv = ops.decode_linear(h, lw["qkv_t"].t(), norm_weight=lw["ln1"], ssq_in=ssq_a,
+                                        eps=s.eps, pdl=True)
+            q = paged.paged_rope_append(
+                qkv[:, :qw], qkv[:, qw:qw + kw], qkv[:, qw + kw:], st["k_cache"][l],
+                st["v_cache"][l], q_start, kv_len, table, base=s.rope_base)
+            a = paged.paged_attention(q, st["k_cache"][l], st["v_cache"][l], q_start, kv_len,
+                                      table, max_q_len=max_q_len, out=q, pdl=True)
+            if not fused:
+                delta = self._mlp(lw, h, a @ lw["o_t"])
+                continue
+            ops.decode_linear(a, lw["o_t"].t(), epilogue="residual", out=h, ssq_out=ssq_b)
+            m = ops.decode_linear(h, lw["gu_t"].t(), norm_weight=lw["ln2"], ssq_in=ssq_b,
+                                  eps=s.eps, epilogue="swiglu", pdl=True)
+            ops.decode_linear(m, lw["down_t"].t(), epilogue="residual", out=h,
+                              ssq_out=ssq_a if l + 1 < s.layers else None, pdl=True)
+        return delta
+
+    def _beam_state(self, chunks: int, beams: int, prompt: int, capacity: int,
+                    page_size: int) -> dict:
+        """Pages and step buffers of one beam-search size, kept for the next
+        call of the same one: a captured step points at them."""
+        key = ("beam", chunks, beams, prompt, capacity, page_size)
+        st = self._states.get(key)
+        if st is not None:
+            return st
+        self._states.clear()
+        s, dev, rows = self.shape, self.device, chunks * beams
+        whole = prompt // page_size                 # prompt pages that beams only read
+        pages = -(-capacity // page_size)
+        pool = beams * (pages - whole)              # a chunk's range of pages to write
+        total = chunks * (whole + pool)
+        shape = (s.layers, total, page_size, s.kv_heads, s.head_dim)
+        table = torch.full((chunks, pages), -1, dtype=torch.int32)
+        for c in range(chunks):
+            table[c, :whole] = torch.arange(c * whole, (c + 1) * whole)
+            if prompt % page_size:                  # the part-filled one is in the range
+                table[c, whole] = chunks * whole + c * pool
+        i32 = {"dtype": torch.int32, "device": dev}
+        st = {
+            "k_cache": torch.empty(shape, dtype=self.dtype, device=dev),
+            "v_cache": torch.empty(shape, dtype=self.dtype, device=dev),
+            "prompt_table": table.to(dev),
+            "prompt_start": torch.arange(0, chunks * prompt + 1, prompt, **i32),
+            "prompt_len": torch.full((chunks,), prompt, **i32),
+            "pool_start": torch.arange(chunks, **i32) * pool + chunks * whole,
+            "pool_pages": pool,
+            "table": torch.empty(rows, pages, **i32), "next_table": torch.empty(rows, pages, **i32),
+            "held": torch.empty(rows, **i32), "next_held": torch.empty(rows, **i32),
+            "kv_len": torch.empty(rows, **i32),
+            "q_start": torch.arange(rows + 1, **i32),
+            "tokens": torch.empty(chunks, beams, dtype=torch.int64, device=dev),
+            "parents": torch.empty(chunks, beams, **i32),
+            "scores": torch.empty(chunks, beams, dtype=torch.float32, device=dev),
+            "finished": torch.empty(chunks, beams, dtype=torch.bool, device=dev),
+            "all_tokens": torch.empty(capacity, chunks, beams, dtype=torch.int64, device=dev),
+            "all_parents": torch.empty(capacity, chunks, beams, **i32),
+            "step": torch.zeros(1, dtype=torch.int64, device=dev),
+            "status": torch.zeros(1, **i32),
+            "graph": None,
+        }
+        self._states[key] = st
+        return st
+
+    def _beam_select(self, st: dict, logits: torch.Tensor) -> None:
+        """The best continuations of every chunk's beams, noted for the end;
+        their page tables, each with a page of its own to write next."""
+        paged.beam_select(logits, st["scores"], finished=st["finished"], eos_ids=self.eos_ids,
+                          pad_id=self.eos_ids[0], tokens=st["tokens"], parents=st["parents"],
+                          scores_out=st["scores"], finished_out=st["finished"])
+        st["all_tokens"].index_copy_(0, st["step"], st["tokens"][None])
+        st["all_parents"].index_copy_(0, st["step"], st["parents"][None])
+        st["step"].add_(1)
+        paged.paged_beam_reorder(st["table"], st["parents"], st["held"], st["pool_start"],
+                                 st["pool_pages"], st["k_cache"], st["v_cache"],
+                                 out=st["next_table"], kv_len_out=st["next_held"],
+                                 status=st["status"])
+        st["table"].copy_(st["next_table"])
+        st["held"].copy_(st["next_held"])
+
+    def _beam_step(self, st: dict) -> None:
+        """One step of every beam (device state only, so that it can be captured)."""
+        torch.add(st["held"], 1, out=st["kv_len"])
+        h = ops.embed_gather(st["tokens"].view(-1, 1), self.embed).view(-1, self.shape.hidden)
+        delta = self._paged_layers(h, st, st["q_start"], st["kv_len"], st["table"], 1)
+        st["held"].copy_(st["kv_len"])
+        self._beam_select(st, self._logits(h, delta))
+
+    def generate_beam(self, audio: torch.Tensor, prompt_ids, *, beams: int = 4,
+                      max_new_tokens: int = 256, length_penalty: float = 1.0,
+                      page_size: int = 32, graphs: bool = True) -> BeamResult:
+        """Beam search of up to max_new_tokens ids per chunk; arguments as in
+        generate().  Hypotheses are ranked by log-probability /
+        length ** length_penalty, length counting the EOS; a finished
+        hypothesis stays in its beam and competes with its log-probability."""
+        s = self.shape
+        prompt = torch.as_tensor(prompt_ids, dtype=torch.int64).to(self.device).contiguous()
+        L = prompt.numel()
+        if audio.dim() == 2:
+            audio = audio.view(-1, AUDIO_TOKENS_PER_CHUNK, s.hidden)
+        audio = audio.to(self.dtype).contiguous()
+        chunks = audio.shape[0]
+        if not 1 <= beams <= paged.BEAM_MAX:
+            raise VlasrInputError(f"beams must be in [1, {paged.BEAM_MAX}]")
+        if chunks < 1 or L < 1 or max_new_tokens < 1:
+            raise VlasrInputError("at least one chunk, prompt id and new token are required")
+        if L + max_new_tokens > self.max_seq_len:
+            raise VlasrInputError("prompt plus budget exceeds the decoder's max_seq_len")
+        st = self._beam_state(chunks, beams, L, L + max_new_tokens, page_size)
+        # prefill, all chunks together
+        h = ops.embed_gather(prompt, self.embed, audio=audio, audio_token_id=self.audio_token_id,
+                             shared_ids=True, batch=chunks).view(chunks * L, s.hidden)
+        delta = self._paged_layers(h, st, st["prompt_start"], st["prompt_len"],
+                                   st["prompt_table"], L)
+        last = torch.arange(chunks, device=self.device) * L + (L - 1)
+        logits = self._logits(h[last].contiguous(),
+                              None if delta is None else delta[last].contiguous())
+        # every chunk's beams start from its prompt, one of them alive
+        st["table"].copy_(st["prompt_table"].repeat_interleave(beams, 0))
+        st["held"].fill_(L)
+        st["scores"].fill_(float("-inf"))
+        st["scores"][:, 0] = 0.0
+        st["finished"].zero_()
+        st["step"].zero_()
+        st["status"].zero_()
+        self._beam_select(st, logits.repeat_interleave(beams, 0))
+        steps = 1
+        if graphs and st["graph"] is None and max_new_tokens > 1:
+            side = torch.cuda.Stream(self.device)
+            side.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(side):
+                self._beam_step(st)                 # eagerly: it also warms the libraries up
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    self._beam_step(st)
+            torch.cuda.current_stream(self.device).wait_stream(side)
+            st["graph"] = graph
+            steps = 2
+        for steps in range(steps, max_new_tokens):
+            if steps % 8 == 0 and bool(st["finished"].all()):
+                break
+            if graphs:
+                st["graph"].replay()
+            else:
+                self._beam_step(st)
+        steps = int(st["step"].item())
+        if int(st["status"].item()):
+            raise VlasrExecutionError(f"beam search: page status {int(st['status'].item())}")
+        return BeamResult(*self._beam_collect(st, steps, length_penalty))
+
+    def _beam_collect(self, st: dict, steps: int, length_penalty: float):
+        tokens = st["all_tokens"][:steps].tolist()
+        parents = st["all_parents"][:steps].tolist()
+        hypotheses = trace_beams(tokens, parents, st["scores"].tolist(), self.eos_ids,
+                                 length_penalty)
+        return [h[0][0] for h in hypotheses], steps, hypotheses
+
     def _collect(self, out: torch.Tensor, chunks: int) -> list[list[int]]:
         return collect_ids(out.t().tolist()[:chunks], self.eos_ids)
 
@@ -437,3 +622,24 @@ def collect_ids(rows_per_chunk, eos_ids=EOS_IDS) -> list[list[int]]:
                 break
         per_chunk.append(seq)
     return per_chunk
+
+
+def trace_beams(tokens, parents, scores, eos_ids=EOS_IDS, length_penalty: float = 1.0) -> list:
+    """Hypotheses of each chunk from the tokens and parents chosen at every step
+    ([steps][chunks][beams]) and the beams' final log-probabilities: per chunk
+    a list of (ids through the first EOS, log-probability, ranked score), best
+    first.  Empty places (-inf) are left out while others remain."""
+    result = []
+    for c, finals in enumerate(scores):
+        found = []
+        for b, score in enumerate(finals):
+            at, row = b, []
+            for step in range(len(tokens) - 1, -1, -1):
+                row.append(tokens[step][c][at])
+                at = parents[step][c][at]
+            ids = collect_ids([row[::-1]], eos_ids)[0]
+            found.append((ids, score, score / max(len(ids), 1) ** length_penalty))
+        found.sort(key=lambda h: -h[2])
+        alive = [h for h in found if h[1] != float("-inf")]
+        result.append(alive or found[:1])
+    return result

@@ -69,9 +69,11 @@ class AsrEngine:
                                    max_seq_len=max_seq_len)
         self.timings = EngineTimings()
 
-    def transcribe_ids(self, pcm, prompt_ids, max_new_tokens: int = 256) -> list[list[int]]:
+    def transcribe_ids(self, pcm, prompt_ids, max_new_tokens: int = 256,
+                       beams: int = 1) -> list[list[int]]:
         """pcm: [samples] or [chunks, 480000] f32 (numpy or torch, host or
-        device) -> generated ids per chunk."""
+        device) -> generated ids per chunk: greedy decoding, or with beams > 1
+        the best hypothesis of a beam search."""
         if isinstance(pcm, torch.Tensor) and pcm.dim() == 2:
             chunks_t = pcm.to(self.device, torch.float32).contiguous()
         else:
@@ -89,16 +91,21 @@ class AsrEngine:
         ev[1].record()
         audio = self.encoder.encode(mel)
         ev[2].record()
-        result = self.decoder.generate(audio, prompt_ids, max_new_tokens=max_new_tokens)
+        if beams > 1:
+            result = self.decoder.generate_beam(audio, prompt_ids, beams=beams,
+                                                max_new_tokens=max_new_tokens)
+        else:
+            result = self.decoder.generate(audio, prompt_ids, max_new_tokens=max_new_tokens)
         ev[3].record()
         torch.cuda.synchronize(self.device)
+        stages = self.decoder.last_timings if beams <= 1 else (0.0, 0.0)
         self.timings = EngineTimings(ev[0].elapsed_time(ev[1]), ev[1].elapsed_time(ev[2]),
-                                     ev[2].elapsed_time(ev[3]), *self.decoder.last_timings)
+                                     ev[2].elapsed_time(ev[3]), *stages)
         return result.per_chunk_ids
 
 
 def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int = 256,
-                           group=None) -> list[list[int]]:
+                           group=None, beams: int = 1) -> list[list[int]]:
     """Multi-GPU engine call: one process per GPU, chunks sharded by
     contiguous range over the ranks of `group` (the partition of the
     benchmark chain, vlasr.pipeline.shard_range); every rank runs its shard
@@ -113,8 +120,9 @@ def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int =
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)
     c0, c1 = shard_range(chunks, rank, world)
-    mine = engine.transcribe_ids(chunks_np[c0:c1], prompt_ids,
-                                 max_new_tokens=max_new_tokens) if c1 > c0 else []
+    more = {"beams": beams} if beams > 1 else {}
+    mine = engine.transcribe_ids(chunks_np[c0:c1], prompt_ids, max_new_tokens=max_new_tokens,
+                                 **more) if c1 > c0 else []
     gathered: list = [None] * world
     dist.all_gather_object(gathered, mine, group=group)
     out: list[list[int]] = []
