@@ -10,6 +10,12 @@ namespace vl {
 
 __device__ __forceinline__ int ilog2(int pow2) { return 31 - __clz(pow2); }
 
+// 64-bit division, at the price of a 32-bit one where that will do.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
+
 // The exponential unit's 2^x (relative error below 2^-22).
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -218,6 +218,10 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = ilog2(a.page_size);
   const int G = a.n_q_heads / a.n_kv_heads;
+  if (tid == kFewWarps * 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+  }
   if (tid == 0) {
     for (int s = 0; s < kFewStages; ++s) {
       mbarrier_init(&sm.full[s], 1);
@@ -226,13 +230,37 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     sm.bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // lengths and tables are not written by the kernel before this one
+  // lengths and tables are not written by the kernel before this one; the
+  // tables are on their way to L2 while the lengths are added up
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kFewThreads + tid;
+       i * 32 < a.batch * a.table_stride - (a.table_stride - a.max_pages);
+       i += static_cast<int64_t>(gridDim.x) * kFewThreads)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.page_table + i * 32));
   int64_t before;
   const bool note = blockIdx.x == 0 && warp == 0;
   const int64_t total = few_total(a, shift, lane, &before, nullptr);
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  if (share < 1) share = 1;
+  const int64_t share = max(int64_t(1), divide(total + gridDim.x - 1, gridDim.x));
   const int64_t u0 = blockIdx.x * share, u1 = min(total, u0 + share);
+  Cursor c;
+  c.b = a.batch;
+  if (u0 < u1) c = few_locate(a, shift, lane, before, u0);
+  // the first tile's pages, for the producer
+  const int box_rows = 1 << box_shift;
+  auto pages_of = [&](int64_t u) {        // lane l: the l-th box's page
+    const int local = static_cast<int>(u - c.base);
+    const int pos0 = (local % c.tiles) * kFewTile;
+    int page = 0;
+    if (lane * box_rows < min(kFewTile, c.s.len - pos0)) {
+      page = a.page_table[c.b * a.table_stride + ((pos0 + (lane << box_shift)) >> shift)];
+      if (page < 0 || page >= a.num_pages) {            // read as rows of zeros
+        page = static_cast<int>(a.num_pages);
+        if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
+      }
+    }
+    return page;
+  };
+  int page = 0;
+  if (warp == kFewWarps && u0 < u1) page = pages_of(u0);
   __syncthreads();
   pdl_wait();
   pdl_release();
@@ -244,11 +272,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
   }
   if (u0 >= u1) return;
-  Cursor c = few_locate(a, shift, lane, before, u0);
 
   if (warp == kFewWarps) {
     // ---- producer ----
-    const int box_rows = 1 << box_shift;
     int stage = 0;
     uint32_t phase = 0;
     int64_t issued = 0;
@@ -258,15 +284,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       const int h = local / c.tiles, tile = local - h * c.tiles;
       const int pos0 = tile * kFewTile;
       const int need = (min(kFewTile, c.s.len - pos0) + box_rows - 1) >> box_shift;
-      // lane l looks up the l-th box's page, before the wait for the stage
-      int page = 0;
-      if (lane < need) {
-        page = a.page_table[c.b * a.table_stride + ((pos0 + (lane << box_shift)) >> shift)];
-        if (page < 0 || page >= a.num_pages) {          // read as rows of zeros
-          page = static_cast<int>(a.num_pages);
-          if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
-        }
-      }
+      if (u != u0) page = pages_of(u);    // before the wait for the stage
       if (issued >= kFewStages && !mbarrier_wait(&sm.empty[stage], phase ^ 1)) {
         if (lane == 0) atomicExch(&sm.bad, 1);
         break;
@@ -545,10 +563,15 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
 
 // Joins the partial sums of the pairs that were cut, in CTA order, and
 // writes the zero rows of sequences without positions.
+constexpr int kFewGridMax = 512;          // CTAs, and so pieces of a pair
+constexpr int kJoinThreads = 128;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinThreads)
     paged_few_join_kernel(const __grid_constant__ PagedAttnArgs a, FewWork work) {
   using S = Storage<T>;
+  __shared__ float weight[kFewGridMax][kFewRows];
+  __shared__ float inv[kFewRows];
   const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
   const int shift = ilog2(a.page_size);
   const int G = a.n_q_heads / a.n_kv_heads;
@@ -561,49 +584,89 @@ __global__ void __launch_bounds__(128)
   if (tiles == 0) {
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int64_t vecs = static_cast<int64_t>(s.rows) * G * (HD / 8);
-    for (int64_t i = tid; i < vecs; i += 128)
+    for (int64_t i = tid; i < vecs; i += kJoinThreads)
       st_vec(out + i / (G * (HD / 8)) * a.out_row_stride + i % (G * (HD / 8)) * 8, zero);
     return;
   }
   const int64_t share = work.base[a.batch + 1];
   const int64_t u0 = work.base[b] + static_cast<int64_t>(h) * tiles, u1 = u0 + tiles;
-  const int64_t c0 = u0 / share, c1 = (u1 - 1) / share;
+  const int64_t c0 = divide(u0, share), c1 = divide(u1 - 1, share);
   if (c0 == c1) return;                   // finished where it was computed
-  auto slot = [&](int64_t c) {            // a CTA's first piece is its slot 0
-    return work.part + (2 * c + (c == c0 && u0 != c * share ? 1 : 0)) * few_partial_floats(HD);
+  const int pieces = static_cast<int>(c1 - c0) + 1, R = s.rows * G;
+  // a CTA's first piece is its slot 0: only the pair's first may be the second
+  const float* part = work.part + 2 * c0 * few_partial_floats(HD);
+  const int late = u0 != c0 * share ? 1 : 0;
+  auto slot = [&](int k) {
+    return part + static_cast<int64_t>(2 * k + (k == 0 ? late : 0)) * few_partial_floats(HD);
   };
-  for (int i = tid; i < s.rows * G * (HD / 8); i += 128) {
-    const int n = i / (HD / 8), d = (i % (HD / 8)) * 8;
-    float M = -INFINITY;
-    for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(slot(c) + kFewRows * HD + 2 * n));
-    float L = 0.0f, f[8];
+  // A thread's share of the first pieces is asked for before their weights are
+  // known: the sums (four dims of a row) and, eight threads a row, (max, sum).
+  constexpr int kTeam = kJoinThreads / kFewRows, kAhead = 8;
+  const int n = tid / kTeam, k0 = tid % kTeam;
+  float2 ml[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-    for (int64_t c = c0; c <= c1; ++c) {
-      const float* p = slot(c);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + kFewRows * HD + 2 * n));
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + n * HD + d));
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(p + n * HD + d + 4));
-      const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-      L = fmaf(ml.y, w, L);
-      f[0] = fmaf(x.x, w, f[0]);
-      f[1] = fmaf(x.y, w, f[1]);
-      f[2] = fmaf(x.z, w, f[2]);
-      f[3] = fmaf(x.w, w, f[3]);
-      f[4] = fmaf(y.x, w, f[4]);
-      f[5] = fmaf(y.y, w, f[5]);
-      f[6] = fmaf(y.z, w, f[6]);
-      f[7] = fmaf(y.w, w, f[7]);
+  for (int u = 0; u < 4; ++u) {
+    ml[u] = make_float2(-INFINITY, 0.0f);
+    if (n < R && k0 + u * kTeam < pieces)
+      ml[u] = __ldcg(reinterpret_cast<const float2*>(slot(k0 + u * kTeam) + kFewRows * HD + 2 * n));
+  }
+  float4 x[kAhead];
+  auto ask = [&](int i, int k) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (k + u < pieces && i < R * (HD / 4))
+        x[u] = __ldcg(reinterpret_cast<const float4*>(slot(k + u)) + i);   // rows lie densely
+  };
+  ask(tid, 0);
+  auto more = [&](int k) {                // (max, sum) of a piece behind the first 32
+    return __ldcg(reinterpret_cast<const float2*>(slot(k) + kFewRows * HD + 2 * n));
+  };
+  float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), L = 0.0f;
+  if (n < R)
+    for (int k = k0 + 4 * kTeam; k < pieces; k += kTeam) M = fmaxf(M, more(k).x);
+#pragma unroll
+  for (int o = kTeam / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (n < R) {
+    auto note = [&](int k, const float2& v) {
+      const float w = v.x == -INFINITY ? 0.0f : exp2f(v.x - M);
+      weight[k][n] = w;
+      L = fmaf(v.y, w, L);
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (k0 + u * kTeam < pieces) note(k0 + u * kTeam, ml[u]);
+    for (int k = k0 + 4 * kTeam; k < pieces; k += kTeam) note(k, more(k));
+  }
+#pragma unroll
+  for (int o = kTeam / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  if (k0 == 0) inv[n] = L == 0.0f ? 0.0f : 1.0f / L;
+  __syncthreads();
+  for (int i = tid; i < R * (HD / 4); i += kJoinThreads) {
+    const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < pieces; k += kAhead) {
+      if (i != tid || k > 0) ask(i, k);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (k + u < pieces) {
+          const float w = weight[k + u][row];
+          f.x = fmaf(x[u].x, w, f.x);
+          f.y = fmaf(x[u].y, w, f.y);
+          f.z = fmaf(x[u].z, w, f.z);
+          f.w = fmaf(x[u].w, w, f.w);
+        }
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= inv;
-    st_vec(out + static_cast<int64_t>(n / G) * a.out_row_stride + static_cast<int64_t>(n % G) * HD + d,
-           S::pack(f));
+    const float r = inv[row];
+    const uint2 y = make_uint2(pack16(f.x * r, f.y * r, T()), pack16(f.z * r, f.w * r, T()));
+    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row / G) * a.out_row_stride +
+                              static_cast<int64_t>(row % G) * HD + d) = y;
   }
 }
 
-int few_grid() { return sm_count() * kFewCtasPerSm; }
+int few_grid() {
+  const int n = sm_count() * kFewCtasPerSm;
+  return n < kFewGridMax ? n : kFewGridMax;
+}
 
 size_t few_workspace(int64_t batch, int hd) {
   return ((static_cast<size_t>(batch) + 2) * 8 + 255) / 256 * 256 +
@@ -644,7 +707,7 @@ cudaError_t few_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cudaSt
   if (e != cudaSuccess) return e;
   return launch_kernel(paged_few_join_kernel<T, HD>,
                        dim3(static_cast<unsigned>(a.batch), static_cast<unsigned>(a.n_kv_heads)),
-                       dim3(128), 0, stream, true, a, work);
+                       dim3(kJoinThreads), 0, stream, true, a, work);
 }
 
 template <typename T>

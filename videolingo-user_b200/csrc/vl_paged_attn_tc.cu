@@ -150,12 +150,6 @@ __device__ __forceinline__ int64_t head_size(const SeqView& s, int pair) {
   return cells_before(past, pairs - 1, pair) + past + s.rows + kCellCost;
 }
 
-// 64-bit division, at the price of a 32-bit one where that will do.
-__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
-  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
-  return x / y;
-}
-
 // The line's length; before: where the sequences that this lane adds up
 // begin (a whole warp, the l-th 32nd of them each).
 __device__ __forceinline__ int64_t line_length(const PagedAttnArgs& a, int shift, int pair,
