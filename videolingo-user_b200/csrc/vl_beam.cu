@@ -119,7 +119,7 @@ __device__ __forceinline__ void readers_sync() {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSelBlock)
+__global__ void __launch_bounds__(kSelBlock, 2)
     beam_piece_kernel(const __grid_constant__ BeamSelectArgs a, int pieces,
                       PieceSum* __restrict__ sums, float* __restrict__ vals,
                       int* __restrict__ ids) {
@@ -583,6 +583,7 @@ cudaError_t select_typed(const BeamSelectArgs& a, void* workspace, cudaStream_t 
 // reordering
 // ---------------------------------------------------------------------------
 constexpr int kReorderThreads = 256;
+constexpr int kReorderAhead = 4;         // vectors of a thread in flight
 
 template <typename Vec>
 __global__ void __launch_bounds__(kReorderThreads)
@@ -621,24 +622,21 @@ __global__ void __launch_bounds__(kReorderThreads)
 
   // whole pages: shared with the parent, marked in the bitmap, copied into
   // the new table by the entry's first CTA
-  for (int i = 0; i < a.beams; ++i) {
+  for (int k = tid; k < a.beams * a.max_pages; k += kReorderThreads) {
+    const int i = k / a.max_pages, j = k - i * a.max_pages;
     const int whole = s_len[i] < 0 ? 0 : s_len[i] >> shift;
-    const int32_t* src = a.page_table + (entry * a.beams + s_row[i]) * a.table_stride;
-    int32_t* dst = a.table_out + (entry * a.beams + i) * a.table_out_stride;
-    for (int j = tid; j < a.max_pages; j += kReorderThreads) {
-      int page = -1;
-      if (j < whole) {
-        page = src[j];
-        if (page < 0 || page >= a.num_pages) {
-          page = -1;
-          s_bad = 1;
-        } else if (range_ok && page >= first && page < first + a.pool_pages) {
-          const int at = static_cast<int>(page - first);
-          atomicOr(&used[at >> 5], 1u << (at & 31));
-        }
+    int page = -1;
+    if (j < whole) {
+      page = a.page_table[(entry * a.beams + s_row[i]) * a.table_stride + j];
+      if (page < 0 || page >= a.num_pages) {
+        page = -1;
+        s_bad = 1;
+      } else if (range_ok && page >= first && page < first + a.pool_pages) {
+        const int at = static_cast<int>(page - first);
+        atomicOr(&used[at >> 5], 1u << (at & 31));
       }
-      if (blockIdx.x == 0) dst[j] = page;
     }
+    if (blockIdx.x == 0) a.table_out[(entry * a.beams + i) * a.table_out_stride + j] = page;
   }
   __syncthreads();
 
@@ -730,13 +728,13 @@ __global__ void __launch_bounds__(kReorderThreads)
                     (s < a.layers ? s : s - a.layers) * a.layer_stride_bytes;
       const Vec* src = reinterpret_cast<const Vec*>(cache + from);
       Vec* dst = reinterpret_cast<Vec*>(cache + to);
-      for (int64_t v = tid; v < vecs; v += 4 * kReorderThreads) {
-        Vec x[4];
+      for (int64_t v = tid; v < vecs; v += kReorderAhead * kReorderThreads) {
+        Vec x[kReorderAhead];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kReorderAhead; ++u)
           if (v + u * kReorderThreads < vecs) x[u] = src[v + u * kReorderThreads];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kReorderAhead; ++u)
           if (v + u * kReorderThreads < vecs) dst[v + u * kReorderThreads] = x[u];
       }
     }
@@ -765,10 +763,11 @@ cudaError_t launch_beam_select(const BeamSelectArgs& a, int dtype, void* workspa
 
 cudaError_t launch_beam_reorder(const BeamReorderArgs& a, cudaStream_t stream) {
   if (a.batch == 0) return cudaSuccess;
-  // about four CTAs per SM over the entries, and no more than there are
-  // segments when every row but one copies
-  int64_t per = (static_cast<int64_t>(sm_count()) * 4 + a.batch - 1) / a.batch;
-  const int64_t most = 2 * a.layers * (a.beams > 1 ? a.beams - 1 : 1);
+  // about eight CTAs per SM over the entries (32 x 5 rows, 28 layers: 25.0 us,
+  // with four 27.0), and no more than there are segments when half the rows
+  // copy
+  int64_t per = (static_cast<int64_t>(sm_count()) * 8 + a.batch - 1) / a.batch;
+  const int64_t most = 2 * a.layers * (a.beams > 1 ? a.beams / 2 : 1);
   if (per > most) per = most;
   if (per < 1) per = 1;
   const dim3 grid(static_cast<unsigned>(per), static_cast<unsigned>(a.batch));
