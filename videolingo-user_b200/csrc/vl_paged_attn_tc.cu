@@ -46,10 +46,12 @@ constexpr int kRows = 128;                // rows of a block (MMA M)
 constexpr int kTile = 128;                // positions of a tile
 constexpr int kStages = 2;                // of K and of V
 constexpr int kSoftThreads = 256;         // two blocks' warps
-constexpr int kProducerWarp = 8;
-constexpr int kMmaWarp = 9;
-constexpr int kPlanWarp = 10;
-constexpr int kThreads = 352;
+constexpr int kEndWarp = 8;               // four warps that finish rows
+constexpr int kQKWarp = 12;
+constexpr int kMmaWarp = 13;
+constexpr int kPlanWarp = 14;
+constexpr int kVWarp = 15;
+constexpr int kThreads = 512;
 constexpr int kPlans = 4;                 // pieces that the walk is ahead
 constexpr float kRescaleLog2 = 8.0f;
 
@@ -61,8 +63,9 @@ struct Shape {
   static constexpr int kQ = 0;                         // two blocks
   static constexpr int kK = 2 * kMatrix;
   static constexpr int kV = kK + kStages * kMatrix;
-  static constexpr int kOut = kV + kStages * kMatrix;  // 32 rows x 64 dims a softmax warp
-  static constexpr int kBars = kOut + 8 * 4096;
+  static constexpr int kOut = kV + kStages * kMatrix;  // 32 rows x 64 dims a finishing warp
+  static constexpr int kSums = kOut + 4 * 4096;        // (max, sum) of two blocks' rows
+  static constexpr int kBars = kSums + 2 * kRows * 8;
   static constexpr int kBytes = kBars + 1024 + 1024;    // barriers, and the ring's alignment
 };
 
@@ -82,7 +85,8 @@ struct Plan {
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_half[2], p_ready[2], o_done[2];
+  uint64_t s_full[2], p_half[2], p_ready[2], o_done[2], o_free[2], sums_full[2],
+      sums_free[2];
   uint64_t plan_full[kPlans], plan_empty[kPlans];
   uint64_t end;
   Plan plan[kPlans];
@@ -110,15 +114,16 @@ struct CutCell {
 // runs of the line.  Where a run ends inside a cell the cell is cut, at a
 // whole tile, if both ends are worth a piece; else it goes to the side that
 // has more of it.
-constexpr int kCellCost = 2 * kTile;      // of a cell by itself, in positions
-constexpr int kMinPiece = 4;              // tiles
+constexpr int kCellCost = 256;     // of a cell by itself, in positions
+constexpr int kMinPiece = 3;              // tiles
 
 // Where a walk along the line stands.
 struct Walk {
   int b;              // sequence (batch: past the end)
   SeqView s;
   int past;           // positions before the new tokens
-  int h, t;           // kv head, pair of blocks
+  int h, u;           // kv head, place in its order of pairs of blocks
+  int t;              // that pair
   int pairs;          // of the sequence
   int64_t at, size;   // the cell's place on the line
   int n;              // its tiles
@@ -139,15 +144,19 @@ __device__ __forceinline__ int tiles_seen(const SeqView& s, int last_token) {
   const int see = s.len - s.rows + last_token;         // positions of that token
   return s.len > 0 && see > 0 ? (see + kTile - 1) / kTile : 0;
 }
-// A head's first t cells on the line, none of them the sequence's last.
-__device__ __forceinline__ int64_t cells_before(int past, int t, int pair) {
-  return t * (static_cast<int64_t>(past) + kCellCost) +
-         static_cast<int64_t>(t) * (t + 1) / 2 * pair;
+// A head's first u cells on the line.  Its pairs come as last, first, last but
+// one, second, ...: two neighbours add up to the same, so that runs of few
+// whole cells differ less (16 x 383 tokens: 35.7 -> 34.5 us).
+__device__ __forceinline__ int64_t cells_before(int past, int rows, int pairs, int u, int pair) {
+  const int64_t each = static_cast<int64_t>(past) + kCellCost, c = u >> 1;
+  int64_t size = u * each + (c * (pairs + 1) + ((u & 1) ? pairs - c : 0)) * pair;
+  if (u > 0) size -= pairs * static_cast<int64_t>(pair) - rows;   // the last is shorter
+  return size;
 }
 __device__ __forceinline__ int64_t head_size(const SeqView& s, int pair) {
   if (s.rows == 0) return 0;
   const int past = max(0, s.len - s.rows), pairs = (s.rows + pair - 1) / pair;
-  return cells_before(past, pairs - 1, pair) + past + s.rows + kCellCost;
+  return cells_before(past, s.rows, pairs, pairs, pair);
 }
 
 // The line's length; before: where the sequences that this lane adds up
@@ -174,6 +183,7 @@ __device__ __forceinline__ int64_t line_length(const PagedAttnArgs& a, int shift
 }
 
 __device__ __forceinline__ void enter_cell(int pair, Walk& w) {
+  w.t = (w.u & 1) ? w.u >> 1 : w.pairs - 1 - (w.u >> 1);
   const int last = min(w.s.rows, (w.t + 1) * pair);
   w.n = tiles_seen(w.s, last);
   w.size = static_cast<int64_t>(w.past) + last + kCellCost;
@@ -185,7 +195,7 @@ __device__ __forceinline__ void enter_sequence(const PagedAttnArgs& a, int shift
     w.s = sequence_view(a, w.b, shift);
     if (w.s.rows > 0) break;
   }
-  w.h = w.t = 0;
+  w.h = w.u = 0;
   if (w.b == a.batch) return;
   w.past = max(0, w.s.len - w.s.rows);
   w.pairs = (w.s.rows + pair - 1) / pair;
@@ -193,8 +203,8 @@ __device__ __forceinline__ void enter_sequence(const PagedAttnArgs& a, int shift
 }
 __device__ __forceinline__ void next_cell(const PagedAttnArgs& a, int shift, int pair, Walk& w) {
   w.at += w.size;
-  if (++w.t == w.pairs) {
-    w.t = 0;
+  if (++w.u == w.pairs) {
+    w.u = 0;
     if (++w.h == a.n_kv_heads) {
       ++w.b;
       enter_sequence(a, shift, pair, w);
@@ -218,12 +228,12 @@ __device__ __forceinline__ Walk find_cell(const PagedAttnArgs& a, int shift, int
       w.h = static_cast<int>(divide(into, head));
       w.at += w.h * head;
       int hi = w.pairs;                   // the last cell of the head that begins at or before x
-      while (hi - w.t > 1) {
-        const int mid = (w.t + hi) / 2;
-        if (w.at + cells_before(w.past, mid, pair) <= x) w.t = mid;
+      while (hi - w.u > 1) {
+        const int mid = (w.u + hi) / 2;
+        if (w.at + cells_before(w.past, w.s.rows, w.pairs, mid, pair) <= x) w.u = mid;
         else hi = mid;
       }
-      w.at += cells_before(w.past, w.t, pair);
+      w.at += cells_before(w.past, w.s.rows, w.pairs, w.u, pair);
       enter_cell(pair, w);
       break;
     }
@@ -269,6 +279,9 @@ __device__ __forceinline__ bool wait_or_bad(uint64_t* bar, uint32_t parity, int*
   return mbarrier_test(at, parity) || wait_longer(at, parity, bad);
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -420,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t raw0 = smem_addr(smem_raw);
   const uint32_t base = (raw0 + 1023) & ~1023u;
   Bars& bars = *reinterpret_cast<Bars*>(smem_raw + (base - raw0) + L::kBars);
+  float2* sums = reinterpret_cast<float2*>(smem_raw + (base - raw0) + L::kSums);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = ilog2(a.page_size);
   const int G = a.n_q_heads / a.n_kv_heads;
@@ -438,10 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbarrier_init(&bars.p_half[i], kSoftThreads / 64);    // a block's warps
       mbarrier_init(&bars.p_ready[i], kSoftThreads / 64);
       mbarrier_init(&bars.o_done[i], 1);
+      mbarrier_init(&bars.o_free[i], 4);                    // the finishing warps
+      mbarrier_init(&bars.sums_full[i], kSoftThreads / 64);
+      mbarrier_init(&bars.sums_free[i], 4);
     }
     for (int k = 0; k < kPlans; ++k) {
       mbarrier_init(&bars.plan_full[k], 1);
-      mbarrier_init(&bars.plan_empty[k], 2 + kSoftThreads / 32);   // every reader's warp
+      mbarrier_init(&bars.plan_empty[k], 3 + kSoftThreads / 32 + 4);   // every reader's warp
     }
     mbarrier_init(&bars.end, 1);
     bars.bad = 0;
@@ -455,6 +472,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == kQKWarp && elect_lane()) {
+    prefetch_map(&qmap);
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+  }
+  __syncwarp();
   // The planning warp looks the lengths up while the others set up; they and
   // the tables are not written by the kernel before this one.
   Run run;
@@ -539,17 +562,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the last ones have been read before this block goes
     for (uint32_t k = piece < kPlans ? 0 : piece - kPlans; k < piece; ++k)
       if (!wait_or_bad(&bars.plan_empty[k % kPlans], (k / kPlans) & 1, &bars.bad)) break;
-  } else if (warp == kProducerWarp) {
-    // ---- copies: Q of a piece, then its K and V tiles in turn ----
+  } else if (warp == kQKWarp || warp == kVWarp) {
+    // ---- copies: one warp Q of a piece and its K tiles, another the V tiles ----
+    const bool qk = warp == kQKWarp;
     pdl_wait();
-    pdl_release();
+    if (qk) pdl_release();
     const int box_rows = 1 << box_shift, rows_tok = kRows / G;
+    const int boxes = kTile >> box_shift;              // of a tile: 1 .. 8
+    uint64_t* const full = qk ? bars.k_full : bars.v_full;
+    uint64_t* const empty = qk ? bars.k_empty : bars.v_empty;
+    const CUtensorMap* const map = qk ? &kmap : &vmap;
+    const uint32_t ring = base + (qk ? L::kK : L::kV);
     uint32_t tile = 0, asked[2] = {0, 0};              // tiles and Q blocks so far
     Plan p;
     while (ok && take(p)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (!ok || p.count[i] == 0) continue;
+        if (!qk || !ok || p.count[i] == 0) continue;
         if (asked[i] > 0) ok = wait_or_bad(&bars.q_empty[i], (asked[i] - 1) & 1, &bars.bad);
         if (!ok) continue;
         ++asked[i];
@@ -562,42 +591,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
-      for (int j = p.j0; ok && j < p.j1; ++j, ++tile) {
+      int page = 0, at_box = 32;                       // pages of 32 boxes, and the tile's first
+      for (int j = p.j0; ok && j < p.j1; ++j, ++tile, at_box += boxes) {
         const int pos0 = j * kTile;
-        const int need = (min(kTile, p.len - pos0) + box_rows - 1) >> box_shift;
-        // lane l looks up the l-th box's page, all before the waits
-        int page = 0;
-        if (lane < need) {
-          page = a.page_table[p.b * a.table_stride + ((pos0 + (lane << box_shift)) >> shift)];
-          if (page < 0 || page >= a.num_pages) {       // read as rows of zeros
-            page = static_cast<int>(a.num_pages);
-            if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
+        if (at_box == 32) {
+          at_box = 0;
+          const int pos = pos0 + (lane << box_shift);
+          if (pos < min(p.len, p.j1 * kTile)) {
+            page = a.page_table[p.b * a.table_stride + (pos >> shift)];
+            if (page < 0 || page >= a.num_pages) {     // read as rows of zeros
+              page = static_cast<int>(a.num_pages);
+              if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
+            }
           }
         }
+        const int need = (min(kTile, p.len - pos0) + box_rows - 1) >> box_shift;
         const int st = tile % kStages;
-        const uint32_t parity = ((tile / kStages) & 1) ^ 1;
-        const uint32_t bytes = static_cast<uint32_t>(need) * box_rows * 128 * L::kHalves;
-        auto fetch = [&](uint32_t matrix, const CUtensorMap* map, uint64_t* full) {
-          if (elect_lane()) mbarrier_expect(full, bytes);
-          __syncwarp();
-          for (int k = 0; k < need; ++k) {
-            const int pk = __shfl_sync(0xffffffffu, page, k);
-            const uint32_t dst = matrix + st * L::kMatrix + k * box_rows * 128;
-            const int row = (pos0 + (k << box_shift)) & (a.page_size - 1);
-            if (elect_lane()) {
+        if (tile >= kStages) ok = wait_or_bad(&empty[st], ((tile / kStages) & 1) ^ 1, &bars.bad);
+        if (!ok) break;
+        int pk[8];
 #pragma unroll
-              for (int c = 0; c < L::kHalves; ++c)
-                tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pk, full);
-            }
-            __syncwarp();
+        for (int k = 0; k < 8; ++k) pk[k] = __shfl_sync(0xffffffffu, page, (at_box + k) & 31);
+        if (elect_lane()) {
+          mbarrier_expect(&full[st], static_cast<uint32_t>(need) * box_rows * 128 * L::kHalves);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (k >= need) break;
+            const uint32_t dst = ring + st * L::kMatrix + k * box_rows * 128;
+            const int row = (pos0 + (k << box_shift)) & (a.page_size - 1);
+#pragma unroll
+            for (int c = 0; c < L::kHalves; ++c)
+              tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pk[k], &full[st]);
           }
-        };
-        if (tile >= kStages) ok = wait_or_bad(&bars.k_empty[st], parity, &bars.bad);
-        if (!ok) break;
-        fetch(base + L::kK, &kmap, &bars.k_full[st]);
-        if (tile >= kStages) ok = wait_or_bad(&bars.v_empty[st], parity, &bars.bad);
-        if (!ok) break;
-        fetch(base + L::kV, &vmap, &bars.v_full[st]);
+        }
+        __syncwarp();
       }
     }
     if (*reinterpret_cast<volatile int*>(&bars.bad)) {
@@ -608,10 +635,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (int i = 0; i < 2; ++i)
         if (asked[i] > 0) drain(&bars.q_full[i], (asked[i] - 1) & 1);
-      for (uint32_t t = tile < kStages ? 0 : tile - kStages; t <= tile; ++t) {
-        drain(&bars.k_full[t % kStages], (t / kStages) & 1);
-        drain(&bars.v_full[t % kStages], (t / kStages) & 1);
-      }
+      for (uint32_t t = tile < kStages ? 0 : tile - kStages; t <= tile; ++t)
+        drain(&full[t % kStages], (t / kStages) & 1);
     }
   } else if (warp == kMmaWarp) {
     // ---- products: one thread ----
@@ -630,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         kd[i] = desc(base + L::kK + i * L::kMatrix, 16, 1024);
         vd[i] = desc(base + L::kV + i * L::kMatrix, L::kColumn, 1024);
       }
-      uint32_t tile = 0, heads[2] = {0, 0}, used[2] = {0, 0};
+      uint32_t tile = 0, heads[2] = {0, 0}, used[2] = {0, 0}, begun[2] = {0, 0};
       auto wait = [&](uint64_t& bar, uint32_t parity) {
         ok = ok && wait_or_bad(&bar, parity & 1, &bars.bad);
       };
@@ -703,6 +728,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (jj < now.of[i]) {
+            // O of the block's last cell has been read
+            if (jj == 0 && begun[i]++ > 0) wait(bars.o_free[i], begun[i]);
             wait(bars.p_half[i], used[i]);
             if (ok) values(i, 0, jj == 0);
             wait(bars.p_ready[i], used[i]++);
@@ -724,19 +751,107 @@ __global__ void __launch_bounds__(kThreads, 1)
       (void)mbarrier_wait(&bars.end, 0);
     }
     __syncwarp();
+  } else if (warp >= kEndWarp && warp < kEndWarp + 4) {
+    // ---- rows of a piece, while the softmax warps are at the next one ----
+    pdl_wait();                                        // it writes rows
+    const int r = tid - kEndWarp * 32;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int rows_tok = kRows / G, g = r % G;
+    const uint32_t stage = base + L::kOut + (warp - kEndWarp) * 4096;
+    uint32_t finished[2] = {0, 0};
+    Plan p;
+    while (ok && take(p)) {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const int count = i ? p.count[1] : p.count[0], tok = i * rows_tok + r / G;
+        const bool mine = r < G * rows_tok && tok < p.tokens;
+        if (!(ok = wait_or_bad(&bars.sums_full[i], (piece - 1) & 1, &bars.bad))) break;
+        const float2 ml = sums[i * kRows + r];
+        __syncwarp();
+        if (lane == 0) mbarrier_arrive(&bars.sums_free[i]);
+        float inv = 0.0f;
+        if (count > 0) {
+          uint32_t& n = i ? finished[1] : finished[0];
+          if (!(ok = wait_or_bad(&bars.o_done[i], n & 1, &bars.bad))) break;
+          ++n;
+          fence_after();
+          inv = ml.y > 0.0f || ml.y != ml.y ? 1.0f / ml.y : 0.0f;
+        }
+        const int64_t row256 =
+            (2 * static_cast<int64_t>(blockIdx.x) + (p.j0 > 0 ? 0 : 1)) * 2 * kRows + i * kRows + r;
+        if (!p.whole && mine) w.ml[row256] = ml;
+        const int64_t at_row = static_cast<int64_t>(p.row0 + tok) * a.out_row_stride +
+                               static_cast<int64_t>(p.h * G + g) * HD;
+        const uint32_t to = tmem + 2 * kTile + i * HD + lanes;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 64) {
+          uint32_t o[64];
+          if (count > 0) {
+            tmem_load32(to + c, o);
+            tmem_load32(to + c + 32, o + 32);
+            tmem_load_wait<64>(o);
+            if (c + 64 == HD) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbarrier_arrive(&bars.o_free[i]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) o[e] = 0;
+          }
+          if (!p.whole) {
+            if (mine) {
+              float4* dst = reinterpret_cast<float4*>(w.part + row256 * HD + c);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                     __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+            }
+            continue;
+          }
+          // A lane has a row; a store of 32 rows at once would touch 32
+          // half-filled sectors.  Through shared memory eight lanes take a
+          // row's 128 bytes instead (7300 -> 2400 cycles for a cell's rows).
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * v + e]) * inv;
+            const uint4 y = S::pack(f);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                             stage + lane * 128 + ((v ^ (lane & 7)) << 4)),
+                         "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w)
+                         : "memory");
+          }
+          __syncwarp();
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const int row = v * 4 + (lane >> 3), ch = lane & 7;
+            uint4 y;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(stage + row * 128 + ((ch ^ (row & 7)) << 4))
+                         : "memory");
+            const int64_t to_row = __shfl_sync(0xffffffffu, mine ? at_row : -1, row);
+            if (to_row >= 0) st_vec(static_cast<T*>(a.out) + to_row + c + ch * 8, y);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok && r == 0 && a.status) atomicOr(a.status, VL_STATUS_TIMEOUT);
   } else {
     // ---- softmax: a thread per row ----
-    pdl_wait();                                        // it writes rows
     const int i = warp >> 2;                           // block
     const int r = tid & (kRows - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + i * kTile + lanes, to = tmem + 2 * kTile + i * HD + lanes;
     const float scale = a.scale * kLog2e;
-    const int rows_tok = kRows / G, tok = i * rows_tok + r / G, g = r % G;
-    uint32_t tile = 0, used = 0, finished = 0;
+    const int rows_tok = kRows / G, tok = i * rows_tok + r / G;
+    uint32_t tile = 0, used = 0;
     Plan p;
     while (ok && take(p)) {
-      const int count = p.count[i];
+      const int count = i ? p.count[1] : p.count[0];
       const bool mine = r < G * rows_tok && tok < p.tokens;
       // (rows of nobody are not hidden: their results go nowhere)
       const int see = !mine ? 0x7fffffff : (p.len > 0 ? p.seen0 + tok + 1 : 0);
@@ -861,70 +976,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tile += p.j1 - p.j0;
       if (!ok) break;
-      // ---- the piece's rows ----
-      float inv = 0.0f;
-      if (count > 0) {
-        if (!(ok = wait_or_bad(&bars.o_done[i], finished & 1, &bars.bad))) break;
-        ++finished;
-        fence_after();
-        inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      }
-      const int64_t row256 = (2 * static_cast<int64_t>(blockIdx.x) + (p.j0 > 0 ? 0 : 1)) * 2 * kRows +
-                             i * kRows + r;
-      if (!p.whole && mine) w.ml[row256] = make_float2(m, l);
-      const int64_t at_row = static_cast<int64_t>(p.row0 + tok) * a.out_row_stride +
-                             static_cast<int64_t>(p.h * G + g) * HD;
-      const uint32_t stage = base + L::kOut + warp * 4096;
-#pragma unroll 1
-      for (int c = 0; c < HD; c += 64) {
-        uint32_t o[64];
-        if (count > 0) {
-          tmem_load32(to + c, o);
-          tmem_load32(to + c + 32, o + 32);
-          tmem_load_wait<64>(o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) o[e] = 0;
-        }
-        if (!p.whole) {
-          if (mine) {
-            float4* dst = reinterpret_cast<float4*>(w.part + row256 * HD + c);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                   __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-          }
-          continue;
-        }
-        // A lane has a row; a store of 32 rows at once would touch 32
-        // half-filled sectors.  Through shared memory eight lanes take a
-        // row's 128 bytes instead (7300 -> 2400 cycles for a cell's rows).
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          float f[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * v + e]) * inv;
-          const uint4 y = S::pack(f);
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
-                           stage + lane * 128 + ((v ^ (lane & 7)) << 4)),
-                       "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w)
-                       : "memory");
-        }
-        __syncwarp();
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const int row = v * 4 + (lane >> 3), ch = lane & 7;
-          uint4 y;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                       : "r"(stage + row * 128 + ((ch ^ (row & 7)) << 4))
-                       : "memory");
-          const int64_t to_row = __shfl_sync(0xffffffffu, mine ? at_row : -1, row);
-          if (to_row >= 0) st_vec(static_cast<T*>(a.out) + to_row + c + ch * 8, y);
-        }
-        __syncwarp();
-      }
-      fence_before();
+      // maximum and sum of the rows, for the warps that finish them
+      if (piece > 1 && !(ok = wait_or_bad(&bars.sums_free[i], piece & 1, &bars.bad))) break;
+      sums[i * kRows + r] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&bars.sums_full[i]);
     }
     if (!ok && r == 0 && a.status) atomicOr(a.status, VL_STATUS_TIMEOUT);
   }
