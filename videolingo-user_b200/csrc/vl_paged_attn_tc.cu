@@ -22,12 +22,19 @@
 //     has grown by more than 2^8 since the last time: until then weights are
 //     taken about the old maximum, which fp32 sums and both 16-bit types
 //     hold (P <= 2^8).
-//   * one warp turns page ids into TMA boxes, one thread issues the MMAs.
-//     CTAs are persistent; the next item's Q and K arrive while the last one
-//     is being finished.
-// Items (256 rows x kv head) are dealt heaviest first.  When there are fewer
-// than SMs, the positions of each are cut into pieces whose partial sums a
-// second launch joins.
+//   * a warp each turns page ids into TMA boxes of K and of V, one thread
+//     issues the MMAs, four warps scale and store finished rows while the
+//     others are at the next cell, one warp walks along the cells.
+// Cells (256 rows x kv head) lie on one line that the CTAs share equally.  A
+// long cell is cut where a share ends, and a second launch joins the partial
+// sums of its pieces.
+//
+// 2048 tokens after 14336, 16 / 4 heads of 128, bf16: 225 us, 1140 TFLOP/s, 0.69
+// of cuBLAS's rate.  What bounds it is the chain of a block's tile (maximum,
+// exponentials, two products: some 4000 cycles for two blocks side by side,
+// 2050 of them tensor cores' and 1940 the exponentials').  Short cells add what
+// they cost by themselves (16 x 383 tokens, 33 us: 9000 cycles until the first
+// scores, 3000 for a cell's last product and its rows, runs of 2 or 3 cells).
 #include <cuda.h>
 
 #include <atomic>
@@ -80,11 +87,13 @@ struct Plan {
   int count[2];       // tiles of each block
   int whole;          // all tiles of its cell
   int last;           // no piece: the run is over
+  int apart;          // the run is worth setting its two blocks apart
 };
 
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t v_tail[kStages];
   uint64_t s_full[2], p_half[2], p_ready[2], o_done[2], o_free[2], sums_full[2],
       sums_free[2];
   uint64_t plan_full[kPlans], plan_empty[kPlans];
@@ -115,6 +124,10 @@ struct CutCell {
 // whole tile, if both ends are worth a piece; else it goes to the side that
 // has more of it.
 constexpr int kCellCost = 256;     // of a cell by itself, in positions
+// A run of this many positions sets its blocks half a tile apart, which costs
+// it 1.5 us at the start: 16 x 383 tokens (1245 a run) 34.1 us set apart, 33.3
+// in step; 23 ragged sequences (4000) 88 and 95 us.
+constexpr int64_t kApart = 16 * kTile;
 constexpr int kMinPiece = 3;              // tiles
 
 // Where a walk along the line stands.
@@ -444,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbarrier_init(&bars.k_empty[s], 1);
       mbarrier_init(&bars.v_full[s], 1);
       mbarrier_init(&bars.v_empty[s], 1);
+      mbarrier_init(&bars.v_tail[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbarrier_init(&bars.q_full[i], 1);
@@ -539,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           p.j1 = at.j1;
           p.count[0] = block_tiles(at, 0);
           p.count[1] = block_tiles(at, 1);
+          p.apart = share >= kApart;
           p.whole = at.j0 == 0 && at.j1 == at.n;
           if (!p.whole) {
             // a CTA's first piece may begin inside its cell (slot 0), its last end there
@@ -574,6 +589,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     const CUtensorMap* const map = qk ? &kmap : &vmap;
     const uint32_t ring = base + (qk ? L::kK : L::kV);
     uint32_t tile = 0, asked[2] = {0, 0};              // tiles and Q blocks so far
+    // Rows of V past a sequence's end hold anything: their weights are 0, and
+    // so must they be.  The tile is cleared there once it has arrived, while
+    // the next one is on its way, and only then handed on.
+    uint32_t tails = 0;                                // a bit a stage: its next parity
+    int clear = kTile, clear_stage = 0;                // the first row to clear
+    auto clear_tail = [&] {
+      if (clear == kTile) return;
+      ok = wait_or_bad(&bars.v_tail[clear_stage], (tails >> clear_stage) & 1, &bars.bad);
+      tails ^= 1u << clear_stage;
+      const uint32_t v = ring + clear_stage * L::kMatrix;
+      for (int z = lane; z < (kTile - clear) * (HD / 8); z += 32) {
+        const int row = clear + z / (HD / 8), ch = z % (HD / 8);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(
+                         v + (ch >> 3) * L::kColumn + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
+                     "r"(0)
+                     : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbarrier_arrive(&full[clear_stage]);
+      clear = kTile;
+    };
     Plan p;
     while (ok && take(p)) {
 #pragma unroll
@@ -612,8 +649,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         int pk[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) pk[k] = __shfl_sync(0xffffffffu, page, (at_box + k) & 31);
+        const bool tail = !qk && p.len - pos0 < kTile;
+        uint64_t* const landed = tail ? &bars.v_tail[st] : &full[st];
         if (elect_lane()) {
-          mbarrier_expect(&full[st], static_cast<uint32_t>(need) * box_rows * 128 * L::kHalves);
+          mbarrier_expect(landed, static_cast<uint32_t>(need) * box_rows * 128 * L::kHalves);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             if (k >= need) break;
@@ -621,12 +660,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = (pos0 + (k << box_shift)) & (a.page_size - 1);
 #pragma unroll
             for (int c = 0; c < L::kHalves; ++c)
-              tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pk[k], &full[st]);
+              tma_load_4d(dst + c * L::kColumn, map, c * 64, p.h, row, pk[k], landed);
           }
         }
         __syncwarp();
+        clear_tail();
+        if (tail) {
+          clear = p.len - pos0;
+          clear_stage = st;
+        }
       }
     }
+    if (ok) clear_tail();
     if (*reinterpret_cast<volatile int*>(&bars.bad)) {
       // leave no copy in flight (each wait is bounded; what was never asked
       // for lets it run out)
@@ -637,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (asked[i] > 0) drain(&bars.q_full[i], (asked[i] - 1) & 1);
       for (uint32_t t = tile < kStages ? 0 : tile - kStages; t <= tile; ++t)
         drain(&full[t % kStages], (t / kStages) & 1);
+      if (clear < kTile) drain(&bars.v_tail[clear_stage], (tails >> clear_stage) & 1);
     }
   } else if (warp == kMmaWarp) {
     // ---- products: one thread ----
@@ -685,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // tiles of a piece, and of its blocks (a piece without tiles is not ours)
       struct Count {
-        int all, of[2];
+        int all, of[2], apart;
       };
       auto next_piece = [&](Count& c) {
         for (;;) {
@@ -694,6 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Plan& p = bars.plan[piece % kPlans];
           const bool over = p.last != 0;
           c.all = p.j1 - p.j0;
+          c.apart = p.apart;
           c.of[0] = p.count[0];
           c.of[1] = p.count[1];
           mbarrier_arrive(&bars.plan_empty[piece % kPlans]);
@@ -707,9 +754,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (more) {
         if (now.of[0] > 0) {
           ask(0, 0, true, now.of[0] == 1);
-          // the second block starts half a tile later, and stays there: one's
-          // products run under the other's exponentials
-          wait(bars.p_half[0], 0);
+          // in a long run the second block starts half a tile later, and stays
+          // there: one's products run under the other's exponentials
+          if (now.apart) wait(bars.p_half[0], 0);
         }
         if (now.of[1] > 0) ask(1, 0, true, now.of[1] == 1);
         commit(&bars.k_empty[0]);
@@ -811,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // A lane has a row; a store of 32 rows at once would touch 32
           // half-filled sectors.  Through shared memory eight lanes take a
-          // row's 128 bytes instead (7300 -> 2400 cycles for a cell's rows).
+          // row's 128 bytes instead.
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
             float f[8];
@@ -848,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + i * kTile + lanes, to = tmem + 2 * kTile + i * HD + lanes;
     const float scale = a.scale * kLog2e;
     const int rows_tok = kRows / G, tok = i * rows_tok + r / G;
-    uint32_t tile = 0, used = 0;
+    uint32_t used = 0;
     Plan p;
     while (ok && take(p)) {
       const int count = i ? p.count[1] : p.count[0];
@@ -911,22 +958,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (pos0 + kTile > p.len) {
-          // rows of V past the end hold anything: their weights are 0, and so
-          // must they be
-          const uint32_t t = tile + jj;
-          if (!(ok = wait_or_bad(&bars.v_full[t % kStages], (t / kStages) & 1, &bars.bad))) break;
-          const uint32_t v = base + L::kV + (t % kStages) * L::kMatrix;
-          const int past = p.len - pos0;
-          for (int z = r; z < (kTile - past) * (HD / 8); z += kRows) {
-            const int row = past + z / (HD / 8), ch = z % (HD / 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(
-                             v + (ch >> 3) * L::kColumn + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
-                         "r"(0)
-                         : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
         const float off = m == -INFINITY ? 0.0f : -m;
         const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
         // P rounds to the storage type, as its tensor-core operand: half a
@@ -974,7 +1005,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 s0 = halves_of(add2(sum[0], sum[1]));
         l += s0.x + s0.y;
       }
-      tile += p.j1 - p.j0;
       if (!ok) break;
       // maximum and sum of the rows, for the warps that finish them
       if (piece > 1 && !(ok = wait_or_bad(&bars.sums_free[i], piece & 1, &bars.bad))) break;
