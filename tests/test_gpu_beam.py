@@ -155,6 +155,29 @@ def test_select_more_candidates_than_the_heap_holds(dev, name, beams):
     run_select(dev, few.to(dev), scores)
 
 
+@pytest.mark.parametrize("name,vocab", [("f32", 59264), ("f32", 40001), ("bf16", 120000)])
+def test_select_rows_in_one_piece(dev, name, vocab):
+    """So many rows that each is one piece and goes round its ring of copies
+    more than once."""
+    batch, beams = 75, 4
+    logits, scores = make(dev, name, batch, beams, vocab, seed=17)
+    # one f32-exact place a row with a value of its own per entry and beam, so
+    # that 16-bit logits tie nowhere among the best
+    best = torch.arange(batch * beams, device=dev)
+    logits[best, (best * 131) % vocab] = 24.0
+    tok, par, val, _ = vlasr.beam_select(logits, scores.to(dev))
+    torch.cuda.synchronize()
+    x = logits.double()
+    values = scores.to(dev).double().view(-1, 1) + x - torch.logsumexp(x, 1, keepdim=True)
+    top, at = values.view(batch, beams * vocab).topk(beams + 1)
+    clear = (top[:, :-1] - top[:, 1:]).amin(1) > 2 * VALUE_TOL
+    assert int(clear.sum()) >= batch // 2
+    assert torch.equal(tok[clear], (at % vocab)[clear, :beams])
+    assert torch.equal(par[clear].long(), (at // vocab)[clear, :beams])
+    assert ((val.double() - top[:, :beams]).abs() <=
+            VALUE_TOL + 2.0 ** -24 * top[:, :beams].abs()).all()
+
+
 def test_select_in_place_repeated_and_captured(dev):
     """scores_out = scores and finished_out = finished, captured and replayed."""
     batch, beams, vocab = 2, 4, 5000

@@ -539,3 +539,81 @@ def test_wrapper_refusals(dev):
         vlasr.paged_rope_append(p.q, p.k, p.v, *args[1:], rotary_dim=66)
     with pytest.raises(vlasr.VlasrInputError, match="q_out needs q"):
         vlasr.paged_rope_append(None, p.k, p.v, *args[1:], q_out=p.q)
+
+
+@pytest.mark.parametrize("name,nq,nkv,hd,ps", [("bf16", 4, 2, 128, 32), ("f16", 5, 1, 64, 16),
+                                               ("bf16", 8, 1, 64, 256)])
+def test_attention_chunks_over_long_caches(dev, name, nq, nkv, hd, ps):
+    """Few cells and many tiles: each is cut into pieces that are joined; one
+    ends right where the cache does, one is too short to be cut."""
+    new, past = [33, 1, 70, 0, 20], [2999, 767, 1466, 40, 100]
+    p = Paged(dev, name, new, past, nq, nkv, hd, ps, seed=60, pad=3)
+    run_attention(p, max(new))
+
+
+def test_attention_long_single_tokens(dev):
+    """One and two sequences whose units spread over many blocks."""
+    for new, past in (([1], [5000]), ([1, 2], [1, 3001])):
+        p = Paged(dev, "bf16", new, past, 8, 2, 128, 64, seed=61)
+        run_attention(p, max(new))
+
+
+@pytest.mark.parametrize("seqs,max_q", [(33, 1), (1100, 1), (40, 24), (1100, 24)])
+def test_attention_many_sequences(dev, seqs, max_q):
+    """The lookup of sequences beyond one and beyond 32 lanes' worth, empty
+    ones and runs of short ones among them."""
+    rng = np.random.default_rng(seqs + max_q)
+    new = rng.integers(0, 2, seqs) if max_q == 1 else \
+        np.where(rng.random(seqs) < 0.1, rng.integers(1, max_q + 1, seqs), rng.integers(0, 2, seqs))
+    past = rng.integers(0, 40, seqs)
+    new[seqs // 2] = max_q
+    p = Paged(dev, "f16", new.tolist(), past.tolist(), 2, 1, 64, 16, seed=62, pad=2)
+    run_attention(p, max_q)
+
+
+def test_attention_chunk_longer_than_promised(dev):
+    """As for single tokens: zero rows and the status bit, the others as they are."""
+    p = Paged(dev, "bf16", [20, 60, 33], [30, 200, 0], 4, 1, 64, 16, seed=63)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=40,
+                                status=status)
+    torch.cuda.synchronize()
+    assert int(status) == vlasr.VL_STATUS_BAD_PAGE
+    assert int(out[20:80].count_nonzero()) == 0
+    qs, kl, tab = p.ints()
+    want, tol = paged_ref.attention(f64(p.q).reshape(p.tokens, 4, 64), f64(p.kc), f64(p.vc), qs,
+                                    kl * np.array([1, 0, 1]), tab, 64 ** -0.5,
+                                    np.zeros((p.tokens, 4, 64)), paged_ref.HALF_STEP["bf16"])
+    check_rows(out, want.reshape(p.tokens, -1), tol.reshape(p.tokens, -1), "bf16")
+
+
+def test_attention_chunks_captured_at_once(dev):
+    """Two graphs of chunks that are cut and joined, replayed side by side with
+    a workspace each; lengths that change between replays are followed."""
+    ps = [Paged(dev, "bf16", [40, 25], [1500, 3], 4, 1, 128, 32, seed=64 + s) for s in range(2)]
+    want = [run_attention(p, 40).clone() for p in ps]
+    graphs, outs = [], []
+    streams = [torch.cuda.Stream(dev) for _ in ps]
+    for p, st in zip(ps, streams):
+        st.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(st):
+            out = torch.zeros_like(p.q)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=40,
+                                      out=out)
+        graphs.append(g)
+        outs.append(out)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert torch.equal(out, w)
+    ps[0].kv_len[0] -= 700
+    short = run_attention(ps[0], 40).clone()
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], short) and not torch.equal(short, want[0])
