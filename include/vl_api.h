@@ -4,7 +4,11 @@
  *
  *   log-mel frontend, residual-add + LayerNorm, residual-add + RMSNorm,
  *   exact-erf GELU (optionally with a fused bias add), SwiGLU, rotary
- *   embedding on Q/K in place, token-embedding gather and KV-cache append.
+ *   embedding on Q/K in place, token-embedding gather and KV-cache append;
+ *
+ * and of what a beam search over a paged KV cache needs (the section "Paged
+ * KV cache and beam search": rotary embedding + paged append, paged
+ * attention, beam selection, page-table reordering).
  *
  * Reference interfaces replaced (paths inside the VideoLingo-user project):
  *   native/asr/src/mel_frontend.h:26-32   compute_mel / compute_mel_batched

@@ -15,6 +15,10 @@
 // per token, in shared memory) while the first vectors are on their way, and
 // then move 16-byte vectors: a task is the two vectors of a head that turn
 // together (one, when interleaved), or one that is only copied.
+//
+// 16 x 383 tokens, 16 / 4 heads of 128, bf16 (75 MB): 19.2 us, 0.60 of the
+// measured copy rate; issue slots are 0.57 busy, the rest is what the short
+// blocks wait for (lookup, sincosf, first vectors).  16 x 1: 3.4 us.
 #include <cmath>
 
 #include "vl_common.cuh"

@@ -22,6 +22,10 @@
 //     warps, across pairs, through a ring of 64-position stages.
 //   * A consumer warp owns 16 positions of a stage and keeps its own running
 //     maximum and sums; warps are joined once per pair.
+// 64 sequences of up to 4096 positions (269 MB), 16 / 4 heads of 128: 53.5 us,
+// 5.0 TB/s, 0.77 of the measured copy rate (0.82 when all are equally long);
+// what is left is the ring's start and the join.  4 sequences of 500: 8.8 us,
+// two launches' latency.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -811,9 +815,10 @@ cudaError_t any_launch(const PagedAttnArgs& a, bool pdl, cudaStream_t stream) {
 
 enum class Kind { kFew, kChunk, kAny };
 
-// 16 rows fill two 8-wide MMA columns of the few-token kernel, which
-// streams the cache at HBM's rate; from there on the tcgen05 kernel's 128-row
-// blocks re-read it less often.
+// Up to 16 rows per kv head (two 8-wide MMA columns) the few-token kernel
+// streams the cache; from there on the tcgen05 kernel's 128-row blocks re-read
+// it less often.  64 x 4 tokens over 2048 positions, G = 4 (16 rows): 57 us
+// against 71; 16 x 4 over 1000: 16 against 28; 4 x 1 over 500: 8 against 16.
 Kind paged_kind(int64_t max_q_len, int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
   if (dtype == kDtypeF32 || (head_dim != 64 && head_dim != 128)) return Kind::kAny;
   return max_q_len * (n_q_heads / n_kv_heads) <= kFewRows ? Kind::kFew : Kind::kChunk;
