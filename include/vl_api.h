@@ -589,7 +589,9 @@ VL_EXPORT int vl_argmax_eos(const void* logits, int64_t rows, int64_t vocab, int
  * lengths.  They cannot be checked on the host; what is out of range is
  * skipped, and VL_STATUS_BAD_PAGE is OR-ed into *status (if given).  No call
  * here allocates, synchronises or keeps anything between calls; calls on
- * different streams are independent as long as their buffers are.
+ * different streams are independent as long as their buffers are.  A call
+ * without tokens or sequences does nothing, and the pointers of its empty
+ * buffers may be NULL.  max_pages * page_size is at most 2^31 - 256.
  */
 
 /*
@@ -718,7 +720,7 @@ VL_EXPORT int vl_beam_select(const void* logits, int64_t batch, int beams, int64
  * [layers][num_pages] pages of page_bytes bytes (row_bytes * page_size),
  * layer_stride_bytes and page_stride_bytes apart; layers 0 moves no cache.
  * Ranges of different entries must not overlap.  beams <= 32,
- * beams * pool_pages and pool_pages <= 16384, max_pages <= 4096.
+ * pool_pages <= 16384, max_pages <= 4096.
  */
 VL_EXPORT int vl_paged_beam_reorder(const int32_t* page_table, const int32_t* parents,
                                     const int32_t* kv_len, const int32_t* pool_start,

@@ -617,3 +617,30 @@ def test_attention_chunks_captured_at_once(dev):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], short) and not torch.equal(short, want[0])
+
+
+def test_empty_batches(dev):
+    """No tokens, and no sequences: empty results, nothing else touched."""
+    kc = torch.full((4, 16, 2, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    vc = kc.clone()
+    i32 = dict(dtype=torch.int32, device=dev)
+    status = torch.zeros(1, **i32)
+    for batch in (0, 3):
+        q = torch.empty(0, 4 * 64, dtype=torch.bfloat16, device=dev)
+        k = torch.empty(0, 2 * 64, dtype=torch.bfloat16, device=dev)
+        start, length = torch.zeros(batch + 1, **i32), torch.full((batch,), 5, **i32)
+        table = torch.zeros(batch, 2, **i32)
+        got = vlasr.paged_rope_append(q, k, k, kc, vc, start, length, table, status=status)
+        assert got.shape == (0, 256)
+        for max_q in (1, 50):
+            got = vlasr.paged_attention(q, kc, vc, start, length, table, max_q_len=max_q,
+                                        status=status)
+            assert got.shape == (0, 256)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and (kc == 7).all() and (vc == 7).all()
+    tok, par, val, end = vlasr.beam_select(torch.empty(0, 100, device=dev),
+                                           torch.empty(0, 4, device=dev))
+    assert tok.shape == par.shape == val.shape == end.shape == (0, 4)
+    out, held = vlasr.paged_beam_reorder(torch.empty(0, 2, **i32), torch.empty(0, 4, **i32),
+                                         torch.empty(0, **i32), torch.empty(0, **i32), 2, kc, vc)
+    assert out.shape == (0, 2) and held.shape == (0,)

@@ -255,3 +255,35 @@ def test_backend_passes_beams_on():
         VlasrAsrBackend(engine=engine, processor=Processor(), beams=beams,
                         audio_loader=lambda path: np.ones(16000, np.float32)).transcribe("x", "en")
         assert engine.calls == [want]
+
+
+def test_empty_calls_and_what_is_not_aligned(lib):
+    """No tokens or no sequences: nothing to do, whatever the empty buffers'
+    pointers; a buffer that is not aligned to its type is refused."""
+    def append(tokens, batch, q=FAR, k=2 * FAR, kvl=FAKE, max_pages=8):
+        return lib.vl_paged_rope_append(
+            q, k, k and 3 * FAR, q and 4 * FAR, 5 * FAR, 6 * FAR, FAKE, kvl, kvl, tokens, batch,
+            max_pages, max_pages, 16, 4, 128, 128, 0, 1e4, 1.0, 2048, 512, 512, 2048, 64, 16,
+            16 * 512, 2, None, None)
+
+    assert append(0, 2, q=None, k=None) == 0
+    assert append(0, 0, q=None, k=None, kvl=None) == 0
+    assert append(4, 0, kvl=None) == 0
+    assert append(4, 2, kvl=None) == 2 and "null" in _err(lib)
+    assert append(4, 2, k=2 * FAR + 1) == 2 and "aligned" in _err(lib)
+    assert append(0, 2, max_pages=(1 << 27) - 15) == 2 and "num_pages" in _err(lib)
+    assert append(0, 2, max_pages=(1 << 27) - 16) == 0
+
+    def attend(tokens, batch, q=FAR, kvl=FAKE):
+        return lib.vl_paged_attention(
+            q, 5 * FAR, 6 * FAR, FAKE, kvl, kvl, tokens, batch, 1, 8, 8, 16, 4, 128, 0.0, 2048,
+            2048, 64, 16, 16 * 512, q and 2 * FAR, 2, None, 0, None, 0, None)
+
+    assert attend(0, 2, q=None) == 0 and attend(4, 0, kvl=None) == 0
+    assert attend(4, 2, kvl=None) == 2 and "null" in _err(lib)
+    eos = (ctypes.c_int64 * 1)(0)
+    assert lib.vl_beam_select(None, 0, 4, 100, 100, None, None, eos, 0, 0, None, None, None, None,
+                              2, None, 0, None) == 0
+    assert lib.vl_paged_beam_reorder(None, None, None, None, 4, 0, 4, 8, 8, None, 8, None,
+                                     5 * FAR, 6 * FAR, 2, 64, 16, 1024, 16384, 1 << 20, None,
+                                     None) == 0

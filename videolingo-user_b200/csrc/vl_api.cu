@@ -745,8 +745,9 @@ static int check_pages(const char* op, const void* k_cache, const void* v_cache,
                        int64_t tokens, int64_t batch, int64_t max_pages, int64_t table_stride,
                        int n_kv_heads, int head_dim, int64_t num_pages, int page_size,
                        int64_t page_stride) {
-  if (k_cache == nullptr || v_cache == nullptr || q_start == nullptr || kv_len == nullptr ||
-      page_table == nullptr)
+  // (an empty tensor's pointer is null)
+  if (k_cache == nullptr || v_cache == nullptr || q_start == nullptr ||
+      (batch != 0 && (kv_len == nullptr || page_table == nullptr)))
     return fail(VL_ERR_INVALID, "%s: null pointer", op);
   if (tokens < 0 || tokens > 0x7fffffff || batch < 0 || batch > (1 << 24) || n_kv_heads <= 0 ||
       n_kv_heads > 65535 || head_dim <= 0)
@@ -757,7 +758,7 @@ static int check_pages(const char* op, const void* k_cache, const void* v_cache,
     return fail(VL_ERR_INVALID, "%s: page_size must be a power of two in [16, 256], got %d", op,
                 page_size);
   if (num_pages <= 0 || num_pages > 0x7ffffffe || max_pages <= 0 || table_stride < max_pages ||
-      max_pages * page_size > 0x7fffffff)
+      max_pages > 0x7fffff00 / page_size)     // a tile's end stays below 2^31
     return fail(VL_ERR_INVALID, "%s: bad pages num_pages=%lld max_pages=%lld table_stride=%lld", op,
                 static_cast<long long>(num_pages), static_cast<long long>(max_pages),
                 static_cast<long long>(table_stride));
@@ -780,10 +781,11 @@ int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_ou
                              max_pages, table_stride, n_kv_heads, head_dim, num_pages, page_size,
                              page_stride);
   if (st != VL_OK) return st;
-  if (k == nullptr || v == nullptr) return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (tokens != 0 && (k == nullptr || v == nullptr))
+    return fail(VL_ERR_INVALID, "%s: null pointer", op);
   if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
-  if (n_q_heads < 0 || (q == nullptr) != (n_q_heads == 0) ||
-      (q_out == nullptr) != (n_q_heads == 0))
+  if (n_q_heads < 0 || (tokens != 0 && ((q == nullptr) != (n_q_heads == 0) ||
+                                        (q_out == nullptr) != (n_q_heads == 0))))
     return fail(VL_ERR_INVALID, "%s: q and q_out must be null exactly when n_q_heads is 0", op);
   if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim || rotary_dim > 256)
     return fail(VL_ERR_INVALID,
@@ -799,6 +801,10 @@ int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_ou
   if (q_row_stride < qw || q_out_row_stride < qw || k_row_stride < kw || v_row_stride < kw)
     return fail(VL_ERR_INVALID, "%s: row strides must cover heads * head_dim", op);
   const int64_t es = dtype_size(dtype);
+  for (const void* p : {q, k, v, static_cast<const void*>(q_out),
+                        static_cast<const void*>(k_cache), static_cast<const void*>(v_cache)})
+    if (reinterpret_cast<uintptr_t>(p) % es != 0)
+      return fail(VL_ERR_INVALID, "%s: buffers must be aligned to their type", op);
   if (n_q_heads > 0 &&
       rows_clash(q_out, q_out_row_stride * es, q, q_row_stride * es, tokens, qw * es))
     return fail(VL_ERR_INVALID, "%s: q_out overlaps q without being equal to it", op);
@@ -865,7 +871,8 @@ int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                              max_pages, table_stride, n_kv_heads, head_dim, num_pages, page_size,
                              page_stride);
   if (st != VL_OK) return st;
-  if (q == nullptr || out == nullptr) return fail(VL_ERR_INVALID, "%s: null pointer", op);
+  if (tokens != 0 && (q == nullptr || out == nullptr))
+    return fail(VL_ERR_INVALID, "%s: null pointer", op);
   if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
   if ((flags & ~VL_LAUNCH_PDL) != 0)
     return fail(VL_ERR_INVALID, "%s: unknown flags 0x%x", op, flags);
@@ -944,8 +951,8 @@ int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
                    int32_t* parents, float* scores_out, uint8_t* finished_out, int dtype,
                    void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "vl_beam_select";
-  if (logits == nullptr || scores == nullptr || tokens == nullptr || parents == nullptr ||
-      scores_out == nullptr)
+  if (batch != 0 && (logits == nullptr || scores == nullptr || tokens == nullptr ||
+                     parents == nullptr || scores_out == nullptr))
     return fail(VL_ERR_INVALID, "%s: null pointer", op);
   if (!valid_dtype(dtype)) return fail(VL_ERR_INVALID, "%s: unsupported dtype %d", op, dtype);
   if (batch > 65535 || !beam_select_shape(batch, beams, vocab))
@@ -997,8 +1004,8 @@ int vl_paged_beam_reorder(const int32_t* page_table, const int32_t* parents,
                           int page_size, int64_t row_bytes, int64_t page_stride_bytes,
                           int64_t layer_stride_bytes, int32_t* status, void* stream) {
   const char* op = "vl_paged_beam_reorder";
-  if (page_table == nullptr || parents == nullptr || kv_len == nullptr || pool_start == nullptr ||
-      table_out == nullptr || kv_len_out == nullptr ||
+  if ((batch != 0 && (page_table == nullptr || parents == nullptr || kv_len == nullptr ||
+                      pool_start == nullptr || table_out == nullptr || kv_len_out == nullptr)) ||
       (layers > 0 && (k_cache == nullptr || v_cache == nullptr)))
     return fail(VL_ERR_INVALID, "%s: null pointer", op);
   if (batch < 0 || batch > 65535 || beams < 1 || beams > VL_BEAM_MAX)
