@@ -636,16 +636,18 @@ VL_EXPORT size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batc
  * with kv head h / (n_q_heads / n_kv_heads); scale 0 means 1/sqrt(head_dim).
  * Scores, softmax and sums in fp32, one rounding of the output; in f16 / bf16
  * at head_dim 64 or 128 the probabilities are rounded to the storage type
- * before the second product.  A token that sees no position (kv_len < n)
- * gives a zero row.
+ * before the second product.  A token that sees no position (kv_len < n), or
+ * only scores of -inf, gives a zero row.
  * max_q_len bounds the new tokens of any sequence and chooses the kernel
  * (single tokens and a few tokens stream the cache once; longer chunks run
  * on the tcgen05 tensor cores); a sequence with more gives zero rows and
  * VL_STATUS_BAD_PAGE, as does a kv_len outside [0, max_pages * page_size].
  * out may be q itself; else it must overlap neither q nor a cache.
  * A page id outside [0, num_pages) reads as rows of zeros and sets the bit.
- * Cache rows at and beyond kv_len may hold anything.  A non-finite k or v
- * below kv_len may reach the output of any query of its sequence.
+ * Cache rows at and beyond kv_len may hold anything.  A NaN in k, or a score
+ * of +inf, makes the rows that see it non-finite and no others.  A non-finite
+ * v of one of the new tokens may reach the rows of its sequence's other new
+ * tokens too (weight 0 times infinity).
  * f32 / f16 / bf16; head_dim a multiple of 32 up to 256.
  * workspace: vl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * no initialisation; calls that may overlap on the GPU need their own.

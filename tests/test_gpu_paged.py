@@ -644,3 +644,62 @@ def test_empty_batches(dev):
     out, held = vlasr.paged_beam_reorder(torch.empty(0, 2, **i32), torch.empty(0, 4, **i32),
                                          torch.empty(0, **i32), torch.empty(0, **i32), 2, kc, vc)
     assert out.shape == (0, 2) and held.shape == (0,)
+
+
+@pytest.mark.parametrize("hd,new,past", [(128, 40, 300), (64, 40, 300), (128, 33, 2000),
+                                         (128, 3, 300)])
+def test_attention_keys_that_are_not_finite(dev, hd, new, past):
+    """A NaN in a key makes the rows that see it non-finite and leaves the
+    others alone; an infinite key is a weight of 0 where its score is -inf and
+    non-finite where it is +inf.  Positions at every place of a group of eight."""
+    p = Paged(dev, "bf16", [new], [past], 4, 1, hd, 16, seed=80)
+    late = past + new // 2
+    kc0 = p.kc.clone()
+    for at in (late, *range(16, 24)):
+        p.kc.copy_(kc0)
+        p.kc[int(p.table[0, at // 16]), at % 16, 0, 5] = float("nan")
+        got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new)
+        torch.cuda.synchronize()
+        sees = max(0, at - past)                     # the first token that does
+        assert not torch.isfinite(got[sees:]).any()
+        if sees:
+            qs, kl, tab = p.ints()
+            want, tol = paged_ref.attention(
+                f64(p.q).reshape(new, 4, hd)[:sees], f64(kc0), f64(p.vc), [0, sees],
+                [past + sees], tab, hd ** -0.5, np.zeros((sees, 4, hd)),
+                paged_ref.HALF_STEP["bf16"])
+            check_rows(got[:sees], want.reshape(sees, -1), tol.reshape(sees, -1), "bf16")
+    q = f64(p.q).reshape(new, 4, hd)
+    rows = (f64(kc0)[p.table[0].cpu().numpy()[:-(-(past + new) // 16)]].reshape(-1, hd)[:past + new],
+            f64(p.vc)[p.table[0].cpu().numpy()[:-(-(past + new) // 16)]].reshape(-1, hd)[:past + new])
+    for at in range(16, 24):
+        p.kc.copy_(kc0)
+        p.kc[int(p.table[0, at // 16]), at % 16, 0, 5] = float("inf")
+        got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new)
+        torch.cuda.synchronize()
+        got = got.view(new, 4, hd)
+        for t in range(new):
+            for h in range(4):
+                if q[t, h, 5] >= 0:
+                    assert not torch.isfinite(got[t, h]).any()
+                    continue
+                use = np.delete(np.arange(past + t + 1), at)
+                s = rows[0][use] @ q[t, h] * hd ** -0.5
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                mags = (np.abs(rows[0][use]) @ np.abs(q[t, h])).max() * hd ** -0.5
+                rel = 2 * hd * 2.0 ** -23 * mags + (len(use) + hd) * 2.0 ** -23 + 2.0 ** -20
+                tol = (rel + paged_ref.HALF_STEP["bf16"]) * (w @ np.abs(rows[1][use]))
+                check_rows(got[t, h], w @ rows[1][use], tol, "bf16")
+
+
+def test_attention_rows_of_minus_infinity(dev):
+    """Every score -inf: a row of zeros, as when nothing is seen."""
+    for new, past in ((40, 300), (2, 300), (33, 2000)):
+        p = Paged(dev, "bf16", [new], [past], 2, 1, 128, 16, seed=81)
+        seen = torch.isfinite(p.kc[..., 5])
+        p.kc[..., 5][seen] = float("inf")
+        p.q.view(new, 2, 128)[:, :, 5] = -1.0
+        got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new)
+        torch.cuda.synchronize()
+        assert int(got.count_nonzero()) == 0

@@ -404,12 +404,18 @@ __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
       : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
   return y;
 }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // 2^x of two values on the multiply-add pipe, beside the exponential unit:
 // x = n + f with |f| <= 1/2, a degree-5 polynomial of f fitted to the least
 // relative error (2.2e-7), n added to the exponent.  Values below -126 give
-// about 1e-38.
+// about 1e-38 (a row all of -inf is told by its maximum), NaN gives what rounds
+// to infinity in either type.
 __device__ __forceinline__ float2 ex2_pair(float2 z) {
-  const uint64_t t = pair_of(fmaxf(z.x, -126.0f), fmaxf(z.y, -126.0f));
+  const uint64_t t = pair_of(max_or_nan(z.x, -126.0f), max_or_nan(z.y, -126.0f));
   constexpr float kRound = 12582912.0f;   // 1.5 * 2^23: the sum's low bits are n
   const uint64_t r = add2(t, pair_of(kRound, kRound));
   const uint64_t f = fma2(add2(r, pair_of(-kRound, -kRound)), pair_of(-1.0f, -1.0f), t);
@@ -822,7 +828,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait_or_bad(&bars.o_done[i], n & 1, &bars.bad))) break;
           ++n;
           fence_after();
-          inv = ml.y > 0.0f || ml.y != ml.y ? 1.0f / ml.y : 0.0f;
+          // (a sum that is NaN stays so; a row all of -inf is a row of zeros)
+          inv = ml.y != ml.y || ml.x > -INFINITY ? 1.0f / ml.y : 0.0f;
         }
         const int64_t row256 =
             (2 * static_cast<int64_t>(blockIdx.x) + (p.j0 > 0 ? 0 : 1)) * 2 * kRows + i * kRows + r;
@@ -1063,7 +1070,7 @@ __global__ void __launch_bounds__(256)
         const float2 q = __ldcg(reinterpret_cast<const float2*>(w.part + row * HD) + lane);
         y[0] = q.x, y[1] = q.y;
       }
-      if (ml.x == -INFINITY) continue;    // the row sees nothing of it
+      if (ml.x == -INFINITY && ml.y == ml.y) continue;   // the row sees nothing of it
       const float m_new = fmaxf(M, ml.x);
       const float f0 = exp2f(M - m_new), f1 = exp2f(ml.x - m_new);
       M = m_new;
