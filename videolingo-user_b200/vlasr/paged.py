@@ -305,26 +305,34 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
     rows, vocab = logits.shape
     if rows != batch * beams:
         raise VlasrInputError("logits must have batch * beams rows")
-    device = logits.device
-
     def place(t, name, dtype):
-        if t is None:
-            return torch.empty_like(scores, dtype=dtype)     # half of torch.empty's time
         _packed(t, _U8 if dtype is _BOOL and t.dtype is _U8 else dtype, dev, name)
         if t.shape != shape:
             raise VlasrInputError(f"{name} must be [batch, beams]")
-        return t
 
     if finished is not None:
         place(finished, "finished", _BOOL)
-    tokens = place(tokens, "tokens", _I64)
-    parents = place(parents, "parents", _I32)
-    scores_out = place(scores_out, "scores_out", _F32)
-    finished_out = place(finished_out, "finished_out", _BOOL)
+    # (empty_like takes half of torch.empty's time)
+    if tokens is None:
+        tokens = torch.empty_like(scores, dtype=_I64)
+    else:
+        place(tokens, "tokens", _I64)
+    if parents is None:
+        parents = torch.empty_like(scores, dtype=_I32)
+    else:
+        place(parents, "parents", _I32)
+    if scores_out is None:
+        scores_out = torch.empty_like(scores)
+    else:
+        place(scores_out, "scores_out", _F32)
+    if finished_out is None:
+        finished_out = torch.empty_like(scores, dtype=_BOOL)
+    else:
+        place(finished_out, "finished_out", _BOOL)
     n_eos = len(eos_ids)
-    eos = (ctypes.c_int64 * max(n_eos, 1))(*eos_ids)
+    eos = (ctypes.c_int64 * n_eos)(*eos_ids) if n_eos else None
     lib = _lib.load()
-    ws, ws_bytes = _workspace(device, dev, workspace,
+    ws, ws_bytes = _workspace(logits.device, dev, workspace,
                               lib.vl_beam_select_workspace_bytes(batch, beams, vocab))
     rc = lib.vl_beam_select(
         logits.data_ptr(), batch, beams, vocab,
