@@ -16,7 +16,7 @@
 // then move 16-byte vectors: a task is the two vectors of a head that turn
 // together (one, when interleaved), or one that is only copied.
 //
-// 16 x 383 tokens, 16 / 4 heads of 128, bf16 (75 MB): 19.2 us, 0.60 of the
+// 16 x 383 tokens, 16 / 4 heads of 128, bf16 (75 MB): 18.6 us, 0.62 of the
 // measured copy rate; issue slots are 0.57 busy, the rest is what the short
 // blocks wait for (lookup, sincosf, first vectors).  16 x 1: 3.4 us.
 #include <cmath>
@@ -30,7 +30,12 @@ namespace vl {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendAhead = 4;   // tasks of a thread in flight
+// Tasks of a thread in flight: a task that turns two vectors holds twice the
+// registers.  With three of those five blocks fit on an SM (16 x 383 tokens:
+// 18.6 us, with four and four blocks 19.2).  Interleaved ones fit six with four
+// as they come (37 ragged sequences: 53.4 us, 62.8 with three; held to six
+// blocks 55.1).
+constexpr int append_ahead(bool interleaved) { return interleaved ? 4 : 3; }
 constexpr int kAppendTokens = 4;  // of a block, at most
 
 // n / d for n, d < 2^16 by the factor ceil(2^32 / d).
@@ -51,13 +56,13 @@ struct AppendTasks {
 };
 
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(kAppendThreads, kInterleaved ? 0 : 5)
     paged_append_kernel(const __grid_constant__ PagedAppendArgs a,
                         const __grid_constant__ InvFreq freq,
                         const __grid_constant__ AppendTasks tasks, int block_tokens) {
   using S = Storage<T>;
   constexpr int E = S::kVec;
-  constexpr int G = kAppendAhead;
+  constexpr int G = append_ahead(kInterleaved);
   constexpr int kPairs = kInterleaved ? E / 2 : E;   // of a task
   __shared__ __align__(16) float2 cs[kAppendTokens * kMaxHalfRot];
   __shared__ int64_t s_at[kAppendTokens];   // the cache row's offset, -1: not cached, -2: no token
@@ -65,7 +70,7 @@ __global__ void __launch_bounds__(kAppendThreads)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * block_tokens;
   const int nt = static_cast<int>(min(static_cast<int64_t>(block_tokens), a.tokens - t0));
-  const int half = a.rotary_dim / 2, half_vecs = half / E;
+  const int half = a.rotary_dim / 2;
   const int kv0 = a.n_q_heads;
   const int count = nt * static_cast<int>(tasks.token.d);
 
@@ -319,7 +324,8 @@ cudaError_t append_typed(const PagedAppendArgs& a, cudaStream_t stream) {
   tasks.whole = divisor(nv);
   // tokens of a block: enough for every thread to have its tasks in flight,
   // but one while there are few blocks
-  int block_tokens = kAppendAhead * kAppendThreads / static_cast<int>(tasks.token.d);
+  int block_tokens =
+      append_ahead(a.interleaved) * kAppendThreads / static_cast<int>(tasks.token.d);
   if (block_tokens > kAppendTokens) block_tokens = kAppendTokens;
   if (block_tokens < 1 || a.tokens <= 2 * sm_count()) block_tokens = 1;
   const int64_t blocks = (a.tokens + block_tokens - 1) / block_tokens;
