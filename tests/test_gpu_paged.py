@@ -703,3 +703,81 @@ def test_attention_rows_of_minus_infinity(dev):
         got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new)
         torch.cuda.synchronize()
         assert int(got.count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("name,nq,nkv,hd,new", [
+    ("bf16", 16, 4, 128, [1, 1, 1, 1]), ("f16", 5, 1, 64, [1, 3, 0, 2, 1]),
+    ("bf16", 4, 2, 128, [8, 1, 5, 0, 2]), ("f16", 16, 1, 128, [1, 1]), ("bf16", 3, 3, 64, [2, 16])])
+def test_few_tokens_by_cluster_and_along_the_line(dev, name, nq, nkv, hd, new):
+    """Short caches through narrow page tables (a cluster per pair) and through
+    wide ones (equal runs, joined by a second launch): lengths that leave some
+    of a cluster's blocks without tiles, none at all, rows that see nothing."""
+    for past in ([0, 1, 60, 500, 940], [700, 63, 0, 64, 2], [128, 1000, 900, 3, 190]):
+        p = Paged(dev, name, new, past[:len(new)], nq, nkv, hd, 16, seed=90)
+        narrow = p.table
+        a = run_attention(p, max(new))
+        p.table = torch.nn.functional.pad(narrow, (0, 100), value=-3)
+        b = run_attention(p, max(new))
+        tol = 4 * paged_ref.HALF_STEP[name]          # a rounding of P and of the output each
+        assert (a.float() - b.float()).abs().max() <= tol * a.float().abs().max() * 2
+        p.kv_len[0] = new[0] - 1                     # the first token sees nothing
+        for table in (narrow, p.table):
+            p.table = table
+            got = run_attention(p, max(new))
+            assert int(got[0].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("wide", [0, 100])
+def test_few_tokens_out_of_range(dev, wide):
+    """Bad lengths, pages and row ranges give the same in both forms."""
+    new = [1, 2, 3, 2, 1]
+    p = Paged(dev, "bf16", new, [50, 20, 90, 33, 7], 4, 2, 128, 16, seed=91)
+    if wide:
+        p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+    run_attention(p, 3)
+    starts = p.q_start.tolist()
+    p.kv_len[0] = -1
+    p.kv_len[1] = p.table.shape[1] * 16 + 1
+    p.table = p.table.clone()
+    p.table[3, 0] = p.kc.shape[0]
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.full_like(p.q, 9.0)
+    vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=2, out=out,
+                          status=status)
+    torch.cuda.synchronize()
+    assert int(status) == vlasr.VL_STATUS_BAD_PAGE
+    assert int(out[:starts[3]].count_nonzero()) == 0          # 2: more tokens than promised
+    qs, kl, tab = p.ints()
+    want, tol = paged_ref.attention(f64(p.q).reshape(p.tokens, 4, 128), f64(p.kc), f64(p.vc), qs,
+                                    np.array([0, 0, 0, kl[3], kl[4]]), tab, 128 ** -0.5,
+                                    np.zeros((p.tokens, 4, 128)), paged_ref.HALF_STEP["bf16"])
+    check_rows(out, want.reshape(p.tokens, -1), tol.reshape(p.tokens, -1), "bf16")
+
+
+@pytest.mark.parametrize("wide", [0, 100])
+def test_few_tokens_captured_at_once(dev, wide):
+    """Two graphs of the same form side by side, each with a workspace."""
+    ps = [Paged(dev, "f16", [1, 2, 1], [200, 700, 3], 8, 2, 64, 16, seed=92 + s) for s in range(2)]
+    graphs, outs, want = [], [], []
+    streams = [torch.cuda.Stream(dev) for _ in ps]
+    for p, st in zip(ps, streams):
+        if wide:
+            p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+        want.append(run_attention(p, 2).clone())
+        st.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(st):
+            out = torch.zeros_like(p.q)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=2,
+                                      out=out)
+        graphs.append(g)
+        outs.append(out)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert torch.equal(out, w)

@@ -16,7 +16,9 @@
 //     A pair that lies within one run is finished there; one that is cut
 //     leaves partial sums (at most two per CTA), and a second launch, ready
 //     before the first ends, joins them in order.  Neither grid nor
-//     workspace depends on the lengths.
+//     workspace depends on the lengths.  Short caches of few pairs take a
+//     cluster of CTAs per pair instead, joined through distributed shared
+//     memory, and no second launch.
 //   * A producer warp turns page ids into TMA boxes (64 dims x up to 64 rows
 //     of one page, 128-byte swizzle) and runs ahead of the four consumer
 //     warps, across pairs, through a ring of 64-position stages.
@@ -24,8 +26,9 @@
 //     maximum and sums; warps are joined once per pair.
 // 64 sequences of up to 4096 positions (269 MB), 16 / 4 heads of 128: 53.5 us,
 // 5.0 TB/s, 0.77 of the measured copy rate (0.82 when all are equally long);
-// what is left is the ring's start and the join.  4 sequences of 500: 8.8 us,
-// two launches' latency.
+// what is left is the ring's start and the join.  4 sequences of 500: 6.7 us,
+// the latency of a launch, of lengths, pages and rows one after the other, and of
+// the join.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -72,6 +75,7 @@ constexpr int kFewWarps = 4;              // consumer warps
 constexpr int kFewThreads = (kFewWarps + 1) * 32;
 constexpr int kFewStages = 3;
 constexpr int kFewCtasPerSm = 2;
+constexpr int kFewCluster = 4;            // CTAs of a pair, where a cluster takes one
 
 __host__ __device__ constexpr int few_partial_floats(int hd) { return kFewRows * hd + 2 * kFewRows; }
 
@@ -202,11 +206,37 @@ __device__ __forceinline__ void few_next(const PagedAttnArgs& a, int shift, Curs
   } while (c.tiles == 0);
 }
 
-template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
-    paged_few_kernel(const __grid_constant__ PagedAttnArgs a,
-                     const __grid_constant__ CUtensorMap kmap,
-                     const __grid_constant__ CUtensorMap vmap, FewWork work, int box_shift) {
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The shared-memory address of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t y;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(addr), "r"(rank));
+  return y;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 y;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+               : "r"(addr)
+               : "memory");
+  return y;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+  float2 y;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(addr)
+               : "memory");
+  return y;
+}
+
+// C = 1: a run of the line of units.  C > 1: a cluster of C CTAs per pair, an
+// equal share of its tiles each, joined through distributed shared memory.
+template <typename T, int HD, int NT, int C>
+__device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorMap& kmap,
+                                         const CUtensorMap& vmap, const FewWork& work,
+                                         int box_shift) {
   using S = Storage<T>;
   constexpr int KS = HD / 16;             // k-steps of q.k, m-tiles of p.v
   constexpr int kHalves = HD / 64;        // 128-byte columns of a row
@@ -240,14 +270,27 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
        i * 32 < a.batch * a.table_stride - (a.table_stride - a.max_pages);
        i += static_cast<int64_t>(gridDim.x) * kFewThreads)
     asm volatile("prefetch.global.L2 [%0];" ::"l"(a.page_table + i * 32));
-  int64_t before;
-  const bool note = blockIdx.x == 0 && warp == 0;
-  const int64_t total = few_total(a, shift, lane, &before, nullptr);
-  const int64_t share = max(int64_t(1), divide(total + gridDim.x - 1, gridDim.x));
-  const int64_t u0 = blockIdx.x * share, u1 = min(total, u0 + share);
+  int64_t before = 0, total = 0, share = 0, u0, u1;
+  const bool note = C == 1 && blockIdx.x == 0 && warp == 0;
+  const int rank = C == 1 ? 0 : static_cast<int>(blockIdx.x % C);
   Cursor c;
-  c.b = a.batch;
-  if (u0 < u1) c = few_locate(a, shift, lane, before, u0);
+  if (C == 1) {
+    total = few_total(a, shift, lane, &before, nullptr);
+    share = max(int64_t(1), divide(total + gridDim.x - 1, gridDim.x));
+    u0 = blockIdx.x * share;
+    u1 = min(total, u0 + share);
+    c.b = a.batch;
+    if (u0 < u1) c = few_locate(a, shift, lane, before, u0);
+  } else {
+    const int pair = blockIdx.x / C;
+    c.b = pair / a.n_kv_heads;
+    c.base = 0;
+    c.s = sequence_view(a, c.b, shift);
+    c.tiles = few_tiles(c.s);
+    const int64_t first = static_cast<int64_t>(pair - c.b * a.n_kv_heads) * c.tiles;
+    u0 = first + c.tiles * rank / C;
+    u1 = first + c.tiles * (rank + 1) / C;
+  }
   // the first tile's pages, for the producer
   const int box_rows = 1 << box_shift;
   auto pages_of = [&](int64_t u) {        // lane l: the l-th box's page
@@ -275,7 +318,22 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       work.base[a.batch + 1] = share;
     }
   }
-  if (u0 >= u1) return;
+  if (C > 1) {
+    const int h = static_cast<int>(blockIdx.x / C) - c.b * a.n_kv_heads;
+    if (c.s.bad && h == 0 && rank == 0 && tid == 0 && a.status)
+      atomicOr(a.status, VL_STATUS_BAD_PAGE);
+    if (c.tiles == 0) {                   // (the whole cluster)
+      T* out = static_cast<T*>(a.out) + static_cast<int64_t>(c.s.start) * a.out_row_stride +
+               static_cast<int64_t>(h) * G * HD;
+      const int64_t vecs = static_cast<int64_t>(c.s.rows) * G * (HD / 8);
+      for (int64_t i = rank * kFewThreads + tid; i < vecs; i += C * kFewThreads)
+        st_vec(out + i / (G * (HD / 8)) * a.out_row_stride + i % (G * (HD / 8)) * 8,
+               make_uint4(0, 0, 0, 0));
+      return;
+    }
+  } else if (u0 >= u1) {
+    return;
+  }
 
   if (warp == kFewWarps) {
     // ---- producer ----
@@ -489,9 +547,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     if (tid == 0) sm.stop = *reinterpret_cast<volatile int*>(&sm.bad);
     few_sync();
     const bool failed = sm.stop != 0;
-    const bool whole = t0 == 0 && t1 == c.tiles;
-    float* part = work.part + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) *
-                                  few_partial_floats(HD);
+    const bool whole = C == 1 && t0 == 0 && t1 == c.tiles;
+    // (a cluster's lie where the ring was: its last stage has been read)
+    float* part = C > 1 ? reinterpret_cast<float*>(smem_raw + (ring - raw0))
+                        : work.part + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) *
+                                          few_partial_floats(HD);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {     // eight rows at a time
 #pragma unroll
@@ -558,11 +618,66 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     if (failed) {
       if (tid == 0 && a.status) atomicOr(a.status, VL_STATUS_TIMEOUT);
-      return;
+      if (C == 1) return;
     }
     first_piece = false;
     u += t1 - t0;
   }
+  if (C > 1) {
+    // ---- join the cluster's pieces, in order: four dims of a row a thread ----
+    const int h = static_cast<int>(blockIdx.x / C) - c.b * a.n_kv_heads, R = c.s.rows * G;
+    if (u0 >= u1 && tid < kFewRows)
+      reinterpret_cast<float2*>(smem_raw + (ring - raw0) + kFewRows * HD * 4)[tid] =
+          make_float2(-INFINITY, 0.0f);
+    cluster_sync();
+    for (int i = tid * C + rank; i < R * (HD / 4); i += kFewWarps * 32 * C) {
+      const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+      float2 ml[C];
+      float4 x[C];
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const uint32_t at = cluster_addr(ring, k);
+        ml[k] = cluster_load2(at + (kFewRows * HD + 2 * row) * 4);
+        x[k] = cluster_load4(at + (row * HD + d) * 4);
+      }
+      float M = ml[0].x, L = 0.0f;
+#pragma unroll
+      for (int k = 1; k < C; ++k) M = fmaxf(M, ml[k].x);
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;   // nothing seen, or no tiles
+        const float w = ml[k].x == -INFINITY ? 1.0f : exp2f(ml[k].x - M);
+        L = fmaf(ml[k].y, w, L);
+        f.x = fmaf(x[k].x, w, f.x);
+        f.y = fmaf(x[k].y, w, f.y);
+        f.z = fmaf(x[k].z, w, f.z);
+        f.w = fmaf(x[k].w, w, f.w);
+      }
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const uint2 y = make_uint2(pack16(f.x * inv, f.y * inv, T()), pack16(f.z * inv, f.w * inv, T()));
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) +
+                                static_cast<int64_t>(c.s.start + row / G) * a.out_row_stride +
+                                static_cast<int64_t>(h * G + row % G) * HD + d) = y;
+    }
+    cluster_sync();                       // nobody leaves while its sums are being read
+  }
+}
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
+    paged_few_kernel(const __grid_constant__ PagedAttnArgs a,
+                     const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap, FewWork work, int box_shift) {
+  few_body<T, HD, NT, 1>(a, kmap, vmap, work, box_shift);
+}
+template <typename T, int HD, int NT, int C>
+__global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(kFewThreads, kFewCtasPerSm)
+    paged_few_cluster_kernel(const __grid_constant__ PagedAttnArgs a,
+                             const __grid_constant__ CUtensorMap kmap,
+                             const __grid_constant__ CUtensorMap vmap, FewWork work,
+                             int box_shift) {
+  few_body<T, HD, NT, C>(a, kmap, vmap, work, box_shift);
 }
 
 // Joins the partial sums of the pairs that were cut, in CTA order, and
@@ -667,6 +782,17 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
+// Few pairs and tables of at most 1024 positions: one launch of clusters,
+// instead of the line and its join.  4 sequences of 500, G = 4: 6.6 us against
+// 7.9 (4 tokens each 9.0 against 12.2); of 1000: 8.0 against 8.6; of 2000 the
+// line is better, 9.5 against 10.9.  Clusters of eight: 6.5 us at 500, 6.3
+// against 5.8 at 200, and fewer of them fit.
+bool few_by_cluster(const PagedAttnArgs& a) {
+  const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv_heads;
+  const int64_t tiles = (static_cast<int64_t>(a.max_pages) * a.page_size + kFewTile - 1) / kFewTile;
+  return pairs * kFewCluster <= 2 * sm_count() && tiles <= 4 * kFewCluster;
+}
+
 int few_grid() {
   const int n = sm_count() * kFewCtasPerSm;
   return n < kFewGridMax ? n : kFewGridMax;
@@ -696,6 +822,7 @@ cudaError_t few_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cudaSt
   constexpr size_t smem = 1024 + static_cast<size_t>(kFewStages) * 2 * kFewTile * HD * sizeof(T) +
                           sizeof(FewSmem<T, HD, NT>);
   auto kernel = paged_few_kernel<T, HD, NT>;
+  auto by_cluster = paged_few_cluster_kernel<T, HD, NT, kFewCluster>;
   static std::atomic<bool> configured[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -703,9 +830,16 @@ cudaError_t few_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cudaSt
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(by_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
+  if (few_by_cluster(a))
+    return launch_kernel(by_cluster,
+                         dim3(static_cast<unsigned>(a.batch * a.n_kv_heads * kFewCluster)),
+                         dim3(kFewThreads), smem, stream, pdl, a, kmap, vmap, work, box_shift);
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(few_grid())), dim3(kFewThreads), smem,
                     stream, pdl, a, kmap, vmap, work, box_shift);
   if (e != cudaSuccess) return e;
