@@ -549,9 +549,9 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorM
     const bool failed = sm.stop != 0;
     const bool whole = C == 1 && t0 == 0 && t1 == c.tiles;
     // (a cluster's lie where the ring was: its last stage has been read)
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1);
     float* part = C > 1 ? reinterpret_cast<float*>(smem_raw + (ring - raw0))
-                        : work.part + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) *
-                                          few_partial_floats(HD);
+                        : work.part + slot * few_partial_floats(HD);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {     // eight rows at a time
 #pragma unroll
@@ -655,7 +655,8 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorM
         f.w = fmaf(x[k].w, w, f.w);
       }
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const uint2 y = make_uint2(pack16(f.x * inv, f.y * inv, T()), pack16(f.z * inv, f.w * inv, T()));
+      const uint2 y =
+          make_uint2(pack16(f.x * inv, f.y * inv, T()), pack16(f.z * inv, f.w * inv, T()));
       *reinterpret_cast<uint2*>(static_cast<T*>(a.out) +
                                 static_cast<int64_t>(c.s.start + row / G) * a.out_row_stride +
                                 static_cast<int64_t>(h * G + row % G) * HD + d) = y;

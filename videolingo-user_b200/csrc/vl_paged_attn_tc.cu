@@ -117,17 +117,19 @@ struct CutCell {
 };
 
 // A cell is a pair of blocks of one sequence and kv head against the n tiles
-// of positions that they see.  All cells lie on one line, (sequence, head,
-// pair) in order, each as long as the positions it sees plus what a cell
+// of positions that they see.  All cells lie on one line, by sequence and head
+// (a head's pairs in the order of cells_before), each as long as the positions it sees plus what a cell
 // costs by itself, so that places are sums in closed form; CTAs take equal
 // runs of the line.  Where a run ends inside a cell the cell is cut, at a
 // whole tile, if both ends are worth a piece; else it goes to the side that
 // has more of it.
-constexpr int kCellCost = 256;     // of a cell by itself, in positions
+constexpr int kCellCost = 2 * kTile;      // of a cell by itself, in positions
 // A run of this many positions sets its blocks half a tile apart, which costs
 // it 1.5 us at the start: 16 x 383 tokens (1245 a run) 34.1 us set apart, 33.3
 // in step; 23 ragged sequences (4000) 88 and 95 us.
 constexpr int64_t kApart = 16 * kTile;
+// Shortest piece of a cut cell.  23 ragged sequences: 93.5 us with three tiles,
+// 95.4 with four, 93.9 with two (and 104 with cells that cost 192 positions).
 constexpr int kMinPiece = 3;              // tiles
 
 // Where a walk along the line stands.
@@ -365,14 +367,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
       "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
       "r"(r[30]), "r"(r[31]), "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
 // Loads issued so far have arrived; ties the registers to the wait, so that
@@ -1124,7 +1118,8 @@ cudaError_t chunk_launch(const PagedAttnArgs& a, void* workspace, bool pdl, cuda
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, stream, pdl, a,
                     qmap, kmap, vmap, w, box_shift);
   // a table too short for a cell that could be cut needs no join
-  if (e != cudaSuccess || static_cast<int64_t>(a.max_pages) * a.page_size <= (2 * kMinPiece - 1) * kTile)
+  if (e != cudaSuccess ||
+      static_cast<int64_t>(a.max_pages) * a.page_size <= (2 * kMinPiece - 1) * kTile)
     return e;
   return launch_kernel(paged_chunk_join_kernel<T, HD>,
                        dim3(static_cast<unsigned>(grid), kJoinBlocks), dim3(256), 0, stream, true,
