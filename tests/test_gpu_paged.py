@@ -781,3 +781,40 @@ def test_few_tokens_captured_at_once(dev, wide):
     torch.cuda.synchronize()
     for out, w in zip(outs, want):
         assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("wide", [0, 100])
+@pytest.mark.parametrize("new", [1, 3])
+def test_few_tokens_that_are_not_a_number(dev, new, wide):
+    """A NaN query row, and NaN keys that fill what a warp, a tile or a whole
+    share of the tiles sees: the rows that see one are not finite, whichever
+    form the table's width chooses, and the other rows are right."""
+    past = [0, 64, 300, 255, 130, 700]
+    # first and last NaN position of each sequence (none: its query is NaN)
+    spans = [(0, 0), (64, 64), None, (64, 127), (0, 130), (650, 650)]
+    p = Paged(dev, "bf16", [new] * len(past), past, 4, 1, 128, 16, seed=95)
+    if wide:
+        p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+    sees = torch.zeros(p.tokens, dtype=torch.bool)
+    for b, span in enumerate(spans):
+        rows = torch.arange(b * new, (b + 1) * new)
+        if span is None:
+            p.q[rows[0]] = float("nan")
+            sees[rows[0]] = True
+            continue
+        for at in range(span[0], span[1] + 1):
+            p.kc[int(p.table[b, at // 16]), at % 16] = float("nan")
+        sees[rows] = past[b] + torch.arange(new) >= span[0]
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new,
+                                status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and not torch.isfinite(got[sees.to(dev)]).any()
+    fine = (~sees).numpy()
+    if fine.any():
+        with np.errstate(invalid="ignore"):
+            want, tol = paged_ref.attention(
+                f64(p.q).reshape(p.tokens, 4, 128), f64(p.kc), f64(p.vc), *p.ints(), 128 ** -0.5,
+                np.zeros((p.tokens, 4, 128)), paged_ref.HALF_STEP["bf16"])
+        check_rows(got[(~sees).to(dev)], want[fine].reshape(fine.sum(), -1),
+                   tol[fine].reshape(fine.sum(), -1), "bf16")

@@ -597,6 +597,7 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorM
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w)
           if (sm.wm[w][n] != -INFINITY) L = fmaf(sm.wl[w][n], exp2f(sm.wm[w][n] - M), L);
+          else L += sm.wl[w][n];          // 0, or NaN where every score seen was NaN
         if (failed) L = __int_as_float(0x7fc00000);
         if (whole) {
           const float inv = L == 0.0f ? 0.0f : 1.0f / L;
