@@ -818,3 +818,33 @@ def test_few_tokens_that_are_not_a_number(dev, new, wide):
                 np.zeros((p.tokens, 4, 128)), paged_ref.HALF_STEP["bf16"])
         check_rows(got[(~sees).to(dev)], want[fine].reshape(fine.sum(), -1),
                    tol[fine].reshape(fine.sum(), -1), "bf16")
+
+
+@pytest.mark.parametrize("new", [40, 1])
+def test_attention_at_the_longest_length(dev, new):
+    """kv_len 2^31 - 256, the longest that the calls take, through a table that
+    repeats one page; the keys of that page weigh nothing (score -512 below
+    the others), so the rows are those of the last two pages alone."""
+    ps, hd = 256, 64
+    pages = ((1 << 31) - 256) // ps
+    g = torch.Generator(device="cpu").manual_seed(96)
+    kc = torch.randn(3, ps, 1, hd, generator=g)
+    kc[..., 0] = 0.0
+    kc[0, :, 0, 0] = -512.0
+    kc = kc.to(torch.bfloat16).to(dev)
+    vc = torch.randn(3, ps, 1, hd, generator=g).to(torch.bfloat16).to(dev)
+    q = torch.randn(new, 4, hd, generator=g)
+    q[..., 0] = 8.0
+    q = q.to(torch.bfloat16).to(dev).view(new, 4 * hd)
+    table = torch.zeros(1, pages, dtype=torch.int32, device=dev)
+    table[0, -2:] = torch.tensor([2, 1], dtype=torch.int32, device=dev)
+    start = torch.tensor([0, new], dtype=torch.int32, device=dev)
+    length = torch.tensor([pages * ps], dtype=torch.int32, device=dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    got = vlasr.paged_attention(q, kc, vc, start, length, table, max_q_len=new, status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    want, tol = paged_ref.attention(f64(q).reshape(new, 4, hd), f64(kc), f64(vc), [0, new],
+                                    [2 * ps], np.array([[2, 1]]), hd ** -0.5,
+                                    np.zeros((new, 4, hd)), paged_ref.HALF_STEP["bf16"])
+    check_rows(got, want.reshape(new, -1), tol.reshape(new, -1), "bf16")

@@ -633,9 +633,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int pos0 = j * kTile;
         if (at_box == 32) {
           at_box = 0;
-          const int pos = pos0 + (lane << box_shift);
-          if (pos < min(p.len, p.j1 * kTile)) {
-            page = a.page_table[p.b * a.table_stride + (pos >> shift)];
+          // (a box that far ahead may begin past 2^31: only its distance is formed)
+          const int ahead = lane << box_shift;
+          if (ahead < min(p.len, p.j1 * kTile) - pos0) {
+            page = a.page_table[p.b * a.table_stride + ((pos0 + ahead) >> shift)];
             if (page < 0 || page >= a.num_pages) {     // read as rows of zeros
               page = static_cast<int>(a.num_pages);
               if (a.status) atomicOr(a.status, VL_STATUS_BAD_PAGE);
