@@ -648,7 +648,8 @@ VL_EXPORT size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batc
  * of +inf, makes the rows that see it non-finite and no others.  A non-finite
  * v of one of the new tokens may reach the rows of its sequence's other new
  * tokens too (weight 0 times infinity).
- * f32 / f16 / bf16; head_dim a multiple of 32 up to 256.
+ * f32 / f16 / bf16; head_dim a multiple of 32 up to 256; n_kv_heads *
+ * max_pages * page_size / 64 below 2^31.
  * workspace: vl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * no initialisation; calls that may overlap on the GPU need their own.
  * flags: 0 or VL_LAUNCH_PDL (the kernel before it in the stream must not

@@ -287,3 +287,16 @@ def test_empty_calls_and_what_is_not_aligned(lib):
     assert lib.vl_paged_beam_reorder(None, None, None, None, 4, 0, 4, 8, 8, None, 8, None,
                                      5 * FAR, 6 * FAR, 2, 64, 16, 1024, 16384, 1 << 20, None,
                                      None) == 0
+
+
+def test_attention_rejects_more_tiles_than_are_counted(lib):
+    """64-position tiles times kv heads of a sequence are counted in 31 bits."""
+    def call(nkv, max_pages):
+        return lib.vl_paged_attention(
+            FAR, 5 << 40, 6 << 40, FAKE, FAKE, FAKE, 1, 1, 1, max_pages, max_pages, nkv, nkv, 64,
+            0.0, nkv * 64, nkv * 64, 4, 256, 256 * nkv * 64, 2 * FAR, 2, None, 0, None, 0, None)
+
+    most = ((1 << 31) - 1) // (4 * 128)            # pages of four tiles, 128 kv heads
+    assert call(128, most + 1) == 2 and "tiles" in _err(lib)
+    assert call(128, most) == 2 and "workspace" in _err(lib)
+    assert call(63, (1 << 23) - 1) == 2 and "workspace" in _err(lib)

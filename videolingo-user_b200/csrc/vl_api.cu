@@ -881,6 +881,10 @@ int vl_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                 "%s: unsupported shape: heads %d / %d (a multiple, at most 128 per kv head), "
                 "head_dim %d (a multiple of 32 up to 256), max_q_len %lld", op, n_q_heads,
                 n_kv_heads, head_dim, static_cast<long long>(max_q_len));
+  // a sequence's 64-position tiles of all kv heads are counted in an int
+  if ((max_pages * page_size + 63) / 64 * n_kv_heads > 0x7fffffff)
+    return fail(VL_ERR_INVALID, "%s: max_pages * page_size / 64 tiles of %d kv heads exceed 2^31 - 1",
+                op, n_kv_heads);
   if (!std::isfinite(scale) || scale < 0.0f)
     return fail(VL_ERR_INVALID, "%s: scale must be finite and >= 0", op);
   const int64_t qw = static_cast<int64_t>(n_q_heads) * head_dim;
