@@ -300,3 +300,17 @@ def test_attention_rejects_more_tiles_than_are_counted(lib):
     assert call(128, most + 1) == 2 and "tiles" in _err(lib)
     assert call(128, most) == 2 and "workspace" in _err(lib)
     assert call(63, (1 << 23) - 1) == 2 and "workspace" in _err(lib)
+
+
+def test_append_rejects_rows_past_31_bits(lib):
+    """A token's elements, q, k and v together, are counted in an int."""
+    def call(nq, nkv=4, hd=128):
+        return lib.vl_paged_rope_append(
+            1 << 56, 1 << 57, 1 << 58, 1 << 59, 1 << 60, 1 << 61, FAKE, FAKE, FAKE, 1, 0, 8, 8, nq,
+            nkv, hd, 0, 0, 1e4, 1.0, 1 << 40, 1 << 40, 1 << 40, 1 << 40, 64, 16, 1 << 40, 2, None,
+            None)
+
+    assert call((1 << 24) - 8) == 2 and "elements" in _err(lib)
+    assert call(1, 65535, 1 << 15) == 2 and "elements" in _err(lib)
+    assert call((1 << 24) - 9) == 2 and "elements" in _err(lib)
+    assert call((1 << 24) - 10) == 0

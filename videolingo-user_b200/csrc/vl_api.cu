@@ -787,6 +787,10 @@ int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_ou
   if (n_q_heads < 0 || (tokens != 0 && ((q == nullptr) != (n_q_heads == 0) ||
                                         (q_out == nullptr) != (n_q_heads == 0))))
     return fail(VL_ERR_INVALID, "%s: q and q_out must be null exactly when n_q_heads is 0", op);
+  // (a block's threads step through them with an int)
+  if ((static_cast<int64_t>(n_q_heads) + 2 * static_cast<int64_t>(n_kv_heads)) * head_dim >
+      0x7fffff00)
+    return fail(VL_ERR_INVALID, "%s: a token's q, k and v are more than 2^31 - 256 elements", op);
   if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim || rotary_dim > 256)
     return fail(VL_ERR_INVALID,
                 "%s: rotary_dim must be even, in [0, min(head_dim, 256)] (head_dim=%d "
