@@ -602,8 +602,10 @@ VL_EXPORT int vl_argmax_eos(const void* logits, int64_t rows, int64_t vocab, int
  *   x1' = x1*cos - x2*sin,  x2' = x2*cos + x1*sin     (fp32, one rounding)
  * over the pairs (d, d + rotary_dim/2) of every head, or with interleaved != 0
  * over the pairs (2d, 2d + 1).  Dims from rotary_dim on are copied.
- *   q_out[t] = rotated q[t]   (q_out may be q itself; else it must not overlap)
- *   cache rows of the position = rotated k[t], v[t]; k and v are only read.
+ *   q_out[t] = rotated q[t]   (q_out may be q itself; else it must not overlap
+ *   q, and never k or v)
+ *   cache rows of the position = rotated k[t], v[t]; k and v are only read, and
+ *   no row buffer may overlap a cache.
  * q may be NULL with n_q_heads 0.  rotary_dim 0 copies without rotation.
  * position_scale < 1 compresses positions for contexts beyond the trained
  * length (linear interpolation); a changed base does the rest.

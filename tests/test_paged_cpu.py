@@ -314,3 +314,29 @@ def test_append_rejects_rows_past_31_bits(lib):
     assert call(1, 65535, 1 << 15) == 2 and "elements" in _err(lib)
     assert call((1 << 24) - 9) == 2 and "elements" in _err(lib)
     assert call((1 << 24) - 10) == 0
+
+
+def test_append_rejects_outputs_over_inputs(lib):
+    """q_out may be q; over k, v or a cache it would be read back or appended
+    over, and so would a cache that lies over q, k or v."""
+    def call(q=FAR, k=2 * FAR, v=3 * FAR, qo=4 * FAR, kc=5 * FAR, vc=6 * FAR, tokens=4, batch=0,
+             qs=2048, ks=512, os_=2048):
+        return lib.vl_paged_rope_append(
+            q, k, v, qo, kc, vc, FAKE, FAKE, FAKE, tokens, batch, 8, 8, 16 if q else 0, 4, 128, 128,
+            0, 1e4, 1.0, qs, ks, ks, os_, 64, 16, 16 * 512, 2, None, None)
+
+    assert call() == 0 and call(qo=FAR) == 0
+    for over in (2, 3, 5, 6):
+        assert call(qo=over * FAR) == 2 and "overlap" in _err(lib)
+        assert call(qo=over * FAR + 1024) == 2 and "overlap" in _err(lib)
+    for name in ("q", "k", "v"):
+        for cache in (5, 6):
+            assert call(**{name: cache * FAR + 4096}) == 2 and "overlap" in _err(lib)
+    # the columns of one projection, rotated in place
+    packed = dict(q=FAR, k=FAR + 4096, v=FAR + 5120, qo=FAR, qs=3080, ks=3080, os_=3080)
+    assert call(**packed) == 0
+    assert call(**{**packed, "qo": FAR + 4096, "tokens": 1}) == 2 and "overlap" in _err(lib)
+    # k and v may be the same rows; a last row of q_out that ends where k begins is apart
+    assert call(k=3 * FAR) == 0
+    assert call(k=4 * FAR + 4 * 4096) == 0 and call(k=4 * FAR + 4 * 4096 - 16) == 2
+    assert call(q=None, qo=None) == 0

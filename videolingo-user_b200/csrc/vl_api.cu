@@ -727,17 +727,23 @@ static bool pow2_in(int64_t x, int64_t lo, int64_t hi) {
   return x >= lo && x <= hi && (x & (x - 1)) == 0;
 }
 
-// Whether rows of `width` bytes at two row strides share memory, other than
-// by being the same rows.
-static bool rows_clash(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
-                       int64_t rows, int64_t width) {
-  if (rows == 0 || (x == y && x_stride == y_stride)) return false;
-  if (!overlaps(x, (rows - 1) * x_stride + width, y, (rows - 1) * y_stride + width)) return false;
+// Whether rows of x_width and of y_width bytes at two row strides share memory.
+static bool rows_overlap(const void* x, int64_t x_stride, int64_t x_width, const void* y,
+                         int64_t y_stride, int64_t y_width, int64_t rows) {
+  if (rows == 0) return false;
+  if (!overlaps(x, (rows - 1) * x_stride + x_width, y, (rows - 1) * y_stride + y_width))
+    return false;
   if (x_stride != y_stride) return true;
   // equal strides: apart if they are disjoint columns of one buffer
-  const int64_t off = std::llabs(static_cast<const char*>(x) - static_cast<const char*>(y)) %
-                      x_stride;
-  return off < width || x_stride - off < width;
+  const int64_t d = static_cast<const char*>(y) - static_cast<const char*>(x);
+  const int64_t off = (d % x_stride + x_stride) % x_stride;   // y's column behind x's
+  return off < x_width || x_stride - off < y_width;
+}
+// The same for rows of one width, which may be the same rows.
+static bool rows_clash(const void* x, int64_t x_stride, const void* y, int64_t y_stride,
+                       int64_t rows, int64_t width) {
+  if (x == y && x_stride == y_stride) return false;
+  return rows_overlap(x, x_stride, width, y, y_stride, width, rows);
 }
 
 static int check_pages(const char* op, const void* k_cache, const void* v_cache,
@@ -812,6 +818,22 @@ int vl_paged_rope_append(const void* q, const void* k, const void* v, void* q_ou
   if (n_q_heads > 0 &&
       rows_clash(q_out, q_out_row_stride * es, q, q_row_stride * es, tokens, qw * es))
     return fail(VL_ERR_INVALID, "%s: q_out overlaps q without being equal to it", op);
+  const struct {
+    const void* at;
+    int64_t stride, width;
+  } rows[4] = {{q_out, q_out_row_stride * es, qw * es}, {q, q_row_stride * es, qw * es},
+               {k, k_row_stride * es, kw * es}, {v, v_row_stride * es, kw * es}};
+  const int64_t cache_bytes = ((num_pages - 1) * page_stride + page_size * kw) * es;
+  for (int i = n_q_heads > 0 ? 0 : 2; i < 4 && tokens > 0; ++i) {
+    if (i >= 2 && n_q_heads > 0 &&
+        rows_overlap(q_out, q_out_row_stride * es, qw * es, rows[i].at, rows[i].stride,
+                     rows[i].width, tokens))
+      return fail(VL_ERR_INVALID, "%s: q_out overlaps k or v", op);
+    const int64_t bytes = (tokens - 1) * rows[i].stride + rows[i].width;
+    if (overlaps(rows[i].at, bytes, k_cache, cache_bytes) ||
+        overlaps(rows[i].at, bytes, v_cache, cache_bytes))
+      return fail(VL_ERR_INVALID, "%s: q, k, v or q_out overlaps a cache", op);
+  }
   if (tokens == 0 || batch == 0) return ok();
   vl::PagedAppendArgs a{};
   a.q = q;
