@@ -691,6 +691,9 @@ VL_EXPORT size_t vl_beam_select_workspace_bytes(int64_t batch, int beams, int64_
  * be NULL.  Sums in fp32 per thread and fp64 across threads, values in fp64,
  * rounded to f32 once.  beams <= 32, vocab <= 2^24, f32 / f16 / bf16; any
  * vocab and row_stride.  workspace as in vl_paged_attention.
+ * vl_beam_select_status does the same and takes a status word (or NULL): a
+ * bounded wait that runs out inside the kernel makes its beam offer nothing,
+ * and VL_STATUS_TIMEOUT tells that from a masked row.
  */
 #define VL_BEAM_MAX 32
 VL_EXPORT int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
@@ -699,6 +702,13 @@ VL_EXPORT int vl_beam_select(const void* logits, int64_t batch, int beams, int64
                              int64_t* tokens, int32_t* parents, float* scores_out,
                              uint8_t* finished_out, int dtype, void* workspace,
                              size_t workspace_bytes, void* stream);
+VL_EXPORT int vl_beam_select_status(const void* logits, int64_t batch, int beams, int64_t vocab,
+                                    int64_t row_stride, const float* scores,
+                                    const uint8_t* finished, const int64_t* eos_ids, int n_eos,
+                                    int64_t pad_id, int64_t* tokens, int32_t* parents,
+                                    float* scores_out, uint8_t* finished_out, int dtype,
+                                    void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream);
 
 /*
  * Page tables after a selection: row (e, i) of the new tables continues row

@@ -364,3 +364,19 @@ def test_reorder_refusals(dev):
         vlasr.paged_beam_reorder(t, par, n, f, 4, kc, vc[:, :4])
     with pytest.raises(vlasr.VlasrInputError, match="pool_start"):
         vlasr.paged_beam_reorder(t, par, n, f[:1].contiguous(), 4, kc, vc)
+
+
+def test_select_status_stays_clear(dev):
+    """A masked row is no failure: the word is set only by a wait that ran out."""
+    logits, scores = make(dev, "bf16", 2, 3, 5000, seed=18)
+    logits[1] = -float("inf")
+    logits[4, 7] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    want = vlasr.beam_select(logits, scores.to(dev))
+    got = vlasr.beam_select(logits, scores.to(dev), status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    with pytest.raises(vlasr.VlasrInputError, match="status"):
+        vlasr.beam_select(logits, scores.to(dev), status=status.long())

@@ -340,3 +340,35 @@ def test_append_rejects_outputs_over_inputs(lib):
     assert call(k=3 * FAR) == 0
     assert call(k=4 * FAR + 4 * 4096) == 0 and call(k=4 * FAR + 4 * 4096 - 16) == 2
     assert call(q=None, qo=None) == 0
+
+
+def test_select_status_word(lib, monkeypatch):
+    """vl_beam_select_status refuses what vl_beam_select does, and the wrapper
+    hands its status word over."""
+    eos = (ctypes.c_int64 * 1)(1)
+
+    def call(pad=0, batch=2, ws=6 * FAR):
+        return lib.vl_beam_select_status(FAR, batch, 4, 1000, 1000, FAKE, None, eos, 1, pad,
+                                         2 * FAR, 3 * FAR, 4 * FAR, None, 2, ws, 1 << 30,
+                                         7 * FAR, None)
+
+    assert call(pad=1000) == 2 and "pad_id" in _err(lib)
+    assert call(ws=None) == 2 and "workspace" in _err(lib)
+    assert call(batch=0) == 0
+
+    seen = []
+
+    class Fake:
+        vl_beam_select_workspace_bytes = staticmethod(lambda *a: 16)
+        vl_beam_select_status = staticmethod(lambda *a: seen.append(a) or 0)
+
+    from vlasr import paged
+    monkeypatch.setattr(paged, "_lead", lambda t, name: (0, t.dtype, t.get_device()))
+    monkeypatch.setattr(paged, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(paged._lib, "load", lambda: Fake)
+    status = torch.zeros(1, dtype=torch.int32)
+    paged.beam_select(torch.zeros(2, 9), torch.zeros(1, 2), status=status)
+    paged.beam_select(torch.zeros(2, 9), torch.zeros(1, 2))
+    assert seen[0][-2] == status.data_ptr() and seen[1][-2] is None
+    with pytest.raises(vlasr.VlasrInputError, match="status"):
+        paged.beam_select(torch.zeros(2, 9), torch.zeros(1, 2), status=status.long())

@@ -980,6 +980,17 @@ int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
                    const int64_t* eos_ids, int n_eos, int64_t pad_id, int64_t* tokens,
                    int32_t* parents, float* scores_out, uint8_t* finished_out, int dtype,
                    void* workspace, size_t workspace_bytes, void* stream) {
+  return vl_beam_select_status(logits, batch, beams, vocab, row_stride, scores, finished, eos_ids,
+                               n_eos, pad_id, tokens, parents, scores_out, finished_out, dtype,
+                               workspace, workspace_bytes, nullptr, stream);
+}
+
+int vl_beam_select_status(const void* logits, int64_t batch, int beams, int64_t vocab,
+                          int64_t row_stride, const float* scores, const uint8_t* finished,
+                          const int64_t* eos_ids, int n_eos, int64_t pad_id, int64_t* tokens,
+                          int32_t* parents, float* scores_out, uint8_t* finished_out, int dtype,
+                          void* workspace, size_t workspace_bytes, int32_t* status,
+                          void* stream) {
   const char* op = "vl_beam_select";
   if (batch != 0 && (logits == nullptr || scores == nullptr || tokens == nullptr ||
                      parents == nullptr || scores_out == nullptr))
@@ -1022,6 +1033,7 @@ int vl_beam_select(const void* logits, int64_t batch, int beams, int64_t vocab,
   a.parents = parents;
   a.scores_out = scores_out;
   a.finished_out = finished_out;
+  a.status = status;
   return exec_status(
       vl::launch_beam_select(a, dtype, workspace, static_cast<cudaStream_t>(stream)), op);
 }

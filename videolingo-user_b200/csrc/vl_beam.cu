@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(kSelBlock, 2)
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) cs += __shfl_xor_sync(0xffffffffu, cs, o);
   // (a failed piece offers nothing)
+  if (lane == 0 && s_bad && a.status) atomicOr(a.status, VL_STATUS_TIMEOUT);
   if (lane == 0) sums[at] = PieceSum{s_bad ? static_cast<double>(NAN) : cs, top, 0.0f};
 }
 

@@ -260,6 +260,7 @@ struct BeamSelectArgs {
   int32_t* parents;
   float* scores_out;
   uint8_t* finished_out;
+  int32_t* status;
 };
 size_t beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab);
 cudaError_t launch_beam_select(const BeamSelectArgs& args, int dtype, void* workspace,

@@ -82,6 +82,10 @@ SIGNATURES = {
     "vl_beam_select": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p,
                                ctypes.POINTER(c_int64), c_int, c_int64, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "vl_beam_select_status": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p,
+                                      c_void_p, ctypes.POINTER(c_int64), c_int, c_int64, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t,
+                                      c_void_p, c_void_p]),
     "vl_paged_beam_reorder": (c_int, [c_void_p] * 4 + [c_int64, c_int64, c_int, c_int64, c_int64,
                                                        c_void_p, c_int64, c_void_p, c_void_p,
                                                        c_void_p, c_int64, c_int64, c_int]

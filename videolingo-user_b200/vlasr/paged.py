@@ -283,7 +283,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
                 tokens: torch.Tensor | None = None, parents: torch.Tensor | None = None,
                 scores_out: torch.Tensor | None = None,
                 finished_out: torch.Tensor | None = None,
-                workspace: torch.Tensor | None = None):
+                workspace: torch.Tensor | None = None, status: torch.Tensor | None = None):
     """One step's selection of beam search (vl_beam_select).
 
     logits [batch * beams, vocab] (a row stride is allowed), scores float32
@@ -293,7 +293,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
     best `beams` values of an entry are taken, ties to the lower
     beam * vocab + token.  Returns (tokens int64, parents int32, scores
     float32, finished bool), each [batch, beams]; scores_out may be scores and
-    finished_out may be finished."""
+    finished_out may be finished.  A wait that ran out inside the kernel makes
+    its beam offer nothing and sets VL_STATUS_TIMEOUT in `status`."""
     code, _, dev = _lead(logits, "logits")
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise VlasrInputError("logits must be a 2-D tensor with contiguous rows")
@@ -334,12 +335,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *,
     lib = _lib.load()
     ws, ws_bytes = _workspace(logits.device, dev, workspace,
                               lib.vl_beam_select_workspace_bytes(batch, beams, vocab))
-    rc = lib.vl_beam_select(
+    rc = lib.vl_beam_select_status(
         logits.data_ptr(), batch, beams, vocab,
         logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
         None if finished is None else finished.data_ptr(), eos, n_eos, pad_id,
         tokens.data_ptr(), parents.data_ptr(), scores_out.data_ptr(), finished_out.data_ptr(),
-        code, ws.data_ptr(), ws_bytes, _raw_stream(dev))
+        code, ws.data_ptr(), ws_bytes, _status_ptr(status, dev), _raw_stream(dev))
     if rc:
         check(rc, "vl_beam_select")
     return tokens, parents, scores_out, finished_out
