@@ -200,3 +200,22 @@ def test_refusals(model):
         dec.generate_beam(audio, PROMPT, max_new_tokens=200)
     with pytest.raises(vlasr.VlasrInputError, match="page_size"):
         dec.generate_beam(audio, PROMPT, max_new_tokens=4, page_size=48)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_a_failure_inside_a_step_is_raised(model, monkeypatch, graphs):
+    """A page id out of range in the tables that a step's attention is given
+    (read as zeros, and reported) ends the search with an error."""
+    dec, _, audio = model
+    attend = vlasr.decoder.paged.paged_attention
+
+    def bad(q, kc, vc, start, length, table, **kw):
+        return attend(q, kc, vc, start, length, torch.full_like(table, kc.shape[0]), **kw)
+
+    dec._states.clear()
+    monkeypatch.setattr(vlasr.decoder.paged, "paged_attention", bad)
+    try:
+        with pytest.raises(vlasr.VlasrExecutionError, match="status 8"):
+            dec.generate_beam(audio, PROMPT, beams=2, max_new_tokens=4, graphs=graphs)
+    finally:
+        dec._states.clear()

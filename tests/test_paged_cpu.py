@@ -372,3 +372,49 @@ def test_select_status_word(lib, monkeypatch):
     assert seen[0][-2] == status.data_ptr() and seen[1][-2] is None
     with pytest.raises(vlasr.VlasrInputError, match="status"):
         paged.beam_select(torch.zeros(2, 9), torch.zeros(1, 2), status=status.long())
+
+
+def _stub_decoder(monkeypatch, layers=2):
+    """A TextDecoder of CPU tensors whose operators are stand-ins."""
+    from types import SimpleNamespace
+
+    from vlasr import decoder
+    dec = object.__new__(decoder.TextDecoder)
+    dec.shape = SimpleNamespace(heads=2, kv_heads=1, head_dim=64, hidden=64, eps=1e-5, layers=layers,
+                                rope_base=1e4)
+    dec.fused, dec.device, dec.eos_ids, dec.embed = False, torch.device("cpu"), (3,), None
+    dec.layer_w = [{"ln1": None, "qkv_t": torch.zeros(64, 256), "o_t": torch.zeros(128, 64)}
+                   for _ in range(layers)]
+    dec._mlp = lambda lw, h, a: a
+    monkeypatch.setattr(decoder.ops, "add_rmsnorm", lambda h, d, w, eps: h)
+    return dec, decoder
+
+
+def test_beam_search_hands_its_status_to_every_call(monkeypatch):
+    """What the operators of a step report reaches the word that
+    generate_beam looks at."""
+    dec, decoder = _stub_decoder(monkeypatch)
+    seen = []
+
+    def op(name, result):
+        def call(*args, **kw):
+            seen.append((name, kw.get("status")))
+            return result(*args)
+        return call
+
+    monkeypatch.setattr(decoder.paged, "paged_rope_append", op("append", lambda q, *a: q))
+    monkeypatch.setattr(decoder.paged, "paged_attention", op("attend", lambda q, *a: q))
+    monkeypatch.setattr(decoder.paged, "beam_select", op("select", lambda *a: None))
+    monkeypatch.setattr(decoder.paged, "paged_beam_reorder", op("reorder", lambda *a: None))
+    i32 = torch.zeros(1, 2, dtype=torch.int32)
+    st = {k: i32 for k in ("table", "next_table", "held", "next_held", "parents", "scores",
+                           "finished", "tokens", "pool_start")}
+    st.update(k_cache=[None] * 2, v_cache=[None] * 2, pool_pages=1, status=torch.zeros(1),
+              step=torch.zeros(1, dtype=torch.int64), all_tokens=torch.zeros(3, 1, 2),
+              all_parents=torch.zeros(3, 1, 2))
+    st["all_tokens"], st["all_parents"] = (t.to(torch.int32) for t in (st["all_tokens"],
+                                                                       st["all_parents"]))
+    dec._paged_layers(torch.zeros(2, 64), st, i32, i32, i32, 1)
+    dec._beam_select(st, torch.zeros(2, 9))
+    assert [n for n, _ in seen] == ["append", "attend"] * 2 + ["select", "reorder"]
+    assert all(s is st["status"] for _, s in seen)

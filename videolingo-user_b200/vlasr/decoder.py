@@ -451,9 +451,10 @@ class TextDecoder:
                                         eps=s.eps, pdl=True)
             q = paged.paged_rope_append(
                 qkv[:, :qw], qkv[:, qw:qw + kw], qkv[:, qw + kw:], st["k_cache"][l],
-                st["v_cache"][l], q_start, kv_len, table, base=s.rope_base)
+                st["v_cache"][l], q_start, kv_len, table, base=s.rope_base, status=st["status"])
             a = paged.paged_attention(q, st["k_cache"][l], st["v_cache"][l], q_start, kv_len,
-                                      table, max_q_len=max_q_len, out=q, pdl=True)
+                                      table, max_q_len=max_q_len, out=q, pdl=True,
+                                      status=st["status"])
             if not fused:
                 delta = self._mlp(lw, h, a @ lw["o_t"])
                 continue
@@ -515,7 +516,8 @@ class TextDecoder:
         their page tables, each with a page of its own to write next."""
         paged.beam_select(logits, st["scores"], finished=st["finished"], eos_ids=self.eos_ids,
                           pad_id=self.eos_ids[0], tokens=st["tokens"], parents=st["parents"],
-                          scores_out=st["scores"], finished_out=st["finished"])
+                          scores_out=st["scores"], finished_out=st["finished"],
+                          status=st["status"])
         st["all_tokens"].index_copy_(0, st["step"], st["tokens"][None])
         st["all_parents"].index_copy_(0, st["step"], st["parents"][None])
         st["step"].add_(1)
@@ -555,6 +557,7 @@ class TextDecoder:
         if L + max_new_tokens > self.max_seq_len:
             raise VlasrInputError("prompt plus budget exceeds the decoder's max_seq_len")
         st = self._beam_state(chunks, beams, L, L + max_new_tokens, page_size)
+        st["status"].zero_()
         # prefill, all chunks together
         h = ops.embed_gather(prompt, self.embed, audio=audio, audio_token_id=self.audio_token_id,
                              shared_ids=True, batch=chunks).view(chunks * L, s.hidden)
@@ -570,7 +573,6 @@ class TextDecoder:
         st["scores"][:, 0] = 0.0
         st["finished"].zero_()
         st["step"].zero_()
-        st["status"].zero_()
         self._beam_select(st, logits.repeat_interleave(beams, 0))
         steps = 1
         if graphs and st["graph"] is None and max_new_tokens > 1:
@@ -593,7 +595,8 @@ class TextDecoder:
                 self._beam_step(st)
         steps = int(st["step"].item())
         if int(st["status"].item()):
-            raise VlasrExecutionError(f"beam search: page status {int(st['status'].item())}")
+            raise VlasrExecutionError("beam search: a kernel reported status "
+                                      f"{int(st['status'].item())}")
         return BeamResult(*self._beam_collect(st, steps, length_penalty))
 
     def _beam_collect(self, st: dict, steps: int, length_penalty: float):
