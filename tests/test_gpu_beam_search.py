@@ -219,3 +219,14 @@ def test_a_failure_inside_a_step_is_raised(model, monkeypatch, graphs):
             dec.generate_beam(audio, PROMPT, beams=2, max_new_tokens=4, graphs=graphs)
     finally:
         dec._states.clear()
+
+
+def test_audio_that_is_not_finite_is_an_error(model):
+    dec, _, audio = model
+    bad = audio.clone()
+    bad[1, 3] = float("nan")
+    for graphs in (False, True):
+        with pytest.raises(vlasr.VlasrExecutionError, match=r"chunks \[1\]"):
+            dec.generate_beam(bad, PROMPT, beams=2, max_new_tokens=4, graphs=graphs)
+    good = dec.generate_beam(audio, PROMPT, beams=2, max_new_tokens=4)
+    assert all(math.isfinite(h[0][1]) for h in good.hypotheses)

@@ -418,3 +418,16 @@ def test_beam_search_hands_its_status_to_every_call(monkeypatch):
     dec._beam_select(st, torch.zeros(2, 9))
     assert [n for n, _ in seen] == ["append", "attend"] * 2 + ["select", "reorder"]
     assert all(s is st["status"] for _, s in seen)
+
+
+def test_a_chunk_without_a_hypothesis_is_an_error(monkeypatch):
+    """Beams that all ended at -inf (logits that are not finite) are no
+    transcription."""
+    dec, _ = _stub_decoder(monkeypatch)
+    st = {"all_tokens": torch.tensor([[[5, 6], [7, 3]]]), "all_parents": torch.zeros(1, 2, 2).int(),
+          "scores": torch.tensor([[-1.0, -2.0], [-0.5, -math.inf]])}
+    ids, steps, hyps = dec._beam_collect(st, 1, 1.0)
+    assert ids == [[5], [7]] and steps == 1 and [len(h) for h in hyps] == [2, 1]
+    st["scores"][1, 0] = -math.inf
+    with pytest.raises(vlasr.VlasrExecutionError, match=r"chunks \[1\]"):
+        dec._beam_collect(st, 1, 1.0)

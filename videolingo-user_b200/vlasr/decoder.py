@@ -36,6 +36,7 @@ of a host round trip and a re-compaction per step.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -542,7 +543,9 @@ class TextDecoder:
         """Beam search of up to max_new_tokens ids per chunk; arguments as in
         generate().  Hypotheses are ranked by log-probability /
         length ** length_penalty, length counting the EOS; a finished
-        hypothesis stays in its beam and competes with its log-probability."""
+        hypothesis stays in its beam and competes with its log-probability.
+        A kernel's reported failure, or a chunk none of whose hypotheses has a
+        finite log-probability, raises VlasrExecutionError."""
         s = self.shape
         prompt = torch.as_tensor(prompt_ids, dtype=torch.int64).to(self.device).contiguous()
         L = prompt.numel()
@@ -604,6 +607,10 @@ class TextDecoder:
         parents = st["all_parents"][:steps].tolist()
         hypotheses = trace_beams(tokens, parents, st["scores"].tolist(), self.eos_ids,
                                  length_penalty)
+        lost = [c for c, h in enumerate(hypotheses) if not math.isfinite(h[0][1])]
+        if lost:
+            raise VlasrExecutionError(f"beam search: chunks {lost} have no hypothesis of finite "
+                                      "log-probability (logits that are not finite)")
         return [h[0][0] for h in hypotheses], steps, hypotheses
 
     def _collect(self, out: torch.Tensor, chunks: int) -> list[list[int]]:
