@@ -380,3 +380,34 @@ def test_select_status_stays_clear(dev):
         assert torch.equal(a, b)
     with pytest.raises(vlasr.VlasrInputError, match="status"):
         vlasr.beam_select(logits, scores.to(dev), status=status.long())
+
+
+def test_select_values_over_the_longest_rows(dev):
+    """2^24 tokens a row, so many rows that each is one piece: the value keeps
+    VALUE_TOL where every round adds the same to a lane's sum (roundings all
+    one way), and where the lanes' maxima grow from round to round."""
+    batch, vocab = 296, 1 << 24
+    logits = torch.empty(batch, vocab, device=dev)
+    scores = torch.zeros(batch, 1, device=dev)
+    best = torch.arange(batch, device=dev) * 50021 % vocab
+    row = torch.arange(batch, device=dev)
+
+    def check(first):
+        tok, par, val, _ = vlasr.beam_select(logits, scores)
+        torch.cuda.synchronize()
+        assert torch.equal(tok[:, 0], first) and int(par.count_nonzero()) == 0
+        want = torch.stack([logits[i, first[i]].double() - torch.logsumexp(logits[i].double(), 0)
+                            for i in range(batch)])
+        off = (val[:, 0].double() - want).abs()
+        assert (off <= VALUE_TOL + 2.0 ** -24 * want.abs()).all(), float(off.max())
+
+    rounds = vocab // 8192
+    logits[:] = -torch.linspace(0.1, 8.0, batch, device=dev).view(-1, 1)
+    logits[:, :1024:4] = 0.0                 # a maximum for every lane, in the first round
+    check(torch.zeros_like(best))
+    # one value a lane and round climbs, by 0.00005 to 0.005 a round
+    logits.view(batch, rounds, 8192)[:, :, :1024:4] = \
+        (torch.linspace(0.1, 10.0, batch, device=dev).view(-1, 1)
+         * torch.linspace(0.0, 1.0, rounds, device=dev)).unsqueeze(2)
+    logits[row, best] = 11.0
+    check(best)

@@ -20,9 +20,14 @@
 //     values come in index order, so equal ones keep it.  Inserting into a
 //     list takes a warp some 700 cycles, a place on the heap a lane 100.
 //   * Lists are merged pairwise as bitonic sequences, five exchanges each.
-//   * exp is taken of l - max (of the lane's values so far), summed in fp32
-//     per lane and in fp64 above that; values are compared in fp64: beams are
-//     told apart to about 1e-7.
+//   * exp is taken of l - m, m the lane's maximum at its last rescaling, summed
+//     in fp32 over a round (chains of 16 values) and in fp64 above that; values
+//     are compared in fp64.  Two beams are told apart to 1e-5, the error of
+//     their lse at any vocab: 20 * 2^-24 by a round's additions, 2^-22 by ex2,
+//     and for its argument 2.5 * 2^-24 times the distance from m, which is 17
+//     where 2^24 values share a row's mass, and the last two once more for a
+//     lane's three rescalings that weigh (kSelLag) and the joins of lanes and
+//     pieces: 6e-6 together.  Within a row the order is exact.
 //
 // Reordering.  See vl_paged_beam_reorder in vl_api.h for the rule.  Every
 // CTA of an entry works the small plan out for itself (a bitmap of the
@@ -102,6 +107,10 @@ constexpr int kSelStage = kSelThreads * kSelVecs * 16;   // bytes of all threads
 constexpr int kHeap = 512;               // candidates of a piece outside the lists
 constexpr int kSelStages = 3;            // on their way, or being read
 constexpr float kLog2e = 1.4426950408889634f;
+// A lane's sum is rescaled when its maximum has grown by this much: what was
+// summed before then soon weighs nothing, and with it its rescalings' errors (a
+// row in ascending order would rescale every round, 4e-5 over 2^24 values).
+constexpr float kSelLag = 4.0f;
 
 // A piece's sum of exp(l - max).
 struct PieceSum {
@@ -158,7 +167,8 @@ __global__ void __launch_bounds__(kSelBlock, 2)
   const int v1 = static_cast<int>(static_cast<int64_t>(vecs) * (piece + 1) / pieces);
   const uint4* whole = reinterpret_cast<const uint4*>(base + head);
 
-  float m = kNegInf, l = 0.0f;             // this lane's maximum and sum about it
+  float m = kNegInf;                       // this lane's maximum, or up to kSelLag less
+  double l = 0.0;                          // its sum about m
   float lv = kNegInf, worst = kNegInf;     // the warp's list: value, index of entry `lane`
   int li = kNoIndex;
   uint4 nothing;
@@ -184,8 +194,8 @@ __global__ void __launch_bounds__(kSelBlock, 2)
       top = fmaxf(top, vmax[i]);
     }
     // a NaN makes the sum NaN, and so does +inf (inf - inf)
-    if (top > m) {
-      l = m == kNegInf ? l : l * ex2((m - top) * kLog2e);
+    if (top > m + kSelLag) {
+      l = m == kNegInf ? l : l * static_cast<double>(ex2((m - top) * kLog2e));
       m = top;
     }
     const float about = m == kNegInf ? 0.0f : m;
@@ -202,7 +212,7 @@ __global__ void __launch_bounds__(kSelBlock, 2)
       }
     }
     const float2 sum2 = halves_of(add2(part[0], part[1]));
-    l += sum2.x + sum2.y;
+    l += static_cast<double>(sum2.x + sum2.y);
     if (first) {
       // The K-th largest of all lanes' maxima: every warp's K largest, then
       // every warp the K-th of those.
@@ -398,7 +408,7 @@ __global__ void __launch_bounds__(kSelBlock, 2)
 
   // the warp's maximum and sum
   const float wm = key_float(__reduce_max_sync(0xffffffffu, float_key(m)));
-  double sum = l == 0.0f ? 0.0 : static_cast<double>(l * ex2((m - wm) * kLog2e));
+  double sum = l == 0.0 ? 0.0 : l * static_cast<double>(ex2((m - wm) * kLog2e));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {
