@@ -431,3 +431,25 @@ def test_a_chunk_without_a_hypothesis_is_an_error(monkeypatch):
     st["scores"][1, 0] = -math.inf
     with pytest.raises(vlasr.VlasrExecutionError, match=r"chunks \[1\]"):
         dec._beam_collect(st, 1, 1.0)
+
+
+def test_wrappers_tell_their_own_errors_from_wrong_arguments(monkeypatch):
+    """An argument that is no tensor is an input error; an AttributeError with
+    tensors in every place is not called one."""
+    from vlasr import paged
+    x = torch.zeros(4, 8)
+    for bad in (None, 3, [1.0]):
+        with pytest.raises(vlasr.VlasrInputError, match="k is not a torch.Tensor"):
+            vlasr.paged_rope_append(None, bad, x, x, x, x, x, x)
+    with pytest.raises(vlasr.VlasrInputError, match="scores is not a torch.Tensor"):
+        monkeypatch.setattr(paged, "_lead", lambda t, name: (0, t.dtype, t.get_device()))
+        vlasr.beam_select(x, scores=[[0.0, 0.0]] * 2)
+
+    def broken(t, name):
+        raise AttributeError("no such helper")
+
+    monkeypatch.setattr(paged, "_lead", broken)
+    with pytest.raises(AttributeError, match="no such helper"):
+        vlasr.beam_select(x, torch.zeros(2, 2))
+    with pytest.raises(AttributeError, match="no such helper"):
+        vlasr.paged_rope_append(None, x, x, x, x, x, x, x)

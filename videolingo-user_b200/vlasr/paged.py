@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 
 import torch
 
@@ -56,6 +57,11 @@ def _operator(fn):
     """Launches go to the tensors' device, whatever the current one is (the
     first CUDA tensor among the arguments names it), and an argument that is
     no tensor is an input error."""
+    signature = inspect.signature(fn)
+    # what a parameter must be: True a tensor, False a tensor or None
+    tensors = {name: "None" not in p.annotation for name, p in signature.parameters.items()
+               if "torch.Tensor" in str(p.annotation)}
+
     @functools.wraps(fn)
     def call(*args, **kwargs):
         try:
@@ -63,8 +69,13 @@ def _operator(fn):
         except _OtherDevice as e:
             with torch.cuda.device(e.device):
                 return fn(*args, **kwargs)
-        except AttributeError as e:
-            raise VlasrInputError(f"{fn.__name__}: an argument is not a torch.Tensor ({e})") from e
+        except AttributeError:
+            for name, value in signature.bind(*args, **kwargs).arguments.items():
+                if name in tensors and not isinstance(value, torch.Tensor) and (
+                        tensors[name] or value is not None):
+                    raise VlasrInputError(
+                        f"{fn.__name__}: {name} is not a torch.Tensor") from None
+            raise
     return call
 
 
