@@ -577,8 +577,9 @@ VL_EXPORT int vl_argmax_eos(const void* logits, int64_t rows, int64_t vocab, int
  *               be passed).  page_size is a power of two in [16, 256].
  *   q_start     int32 [batch + 1], ascending: sequence b's new tokens are the
  *               rows q_start[b] .. q_start[b+1] - 1 of q / k / v / out.  Rows
- *               from q_start[batch] on (a padded batch) are neither read nor
- *               written.
+ *               from q_start[batch] to tokens (a padded batch) are not
+ *               written; they may be read and must be readable, but what
+ *               they hold does not matter.
  *   kv_len      int32 [batch]: positions of the sequence once its new tokens
  *               are counted; the new tokens are the last ones, so token i of
  *               n sits at position kv_len - n + i.

@@ -848,3 +848,29 @@ def test_attention_at_the_longest_length(dev, new):
                                     [2 * ps], np.array([[2, 1]]), hd ** -0.5,
                                     np.zeros((new, 4, hd)), paged_ref.HALF_STEP["bf16"])
     check_rows(got, want.reshape(new, -1), tol.reshape(new, -1), "bf16")
+
+
+@pytest.mark.parametrize("name,nq,nkv,hd,new,wide", [
+    ("bf16", 8, 2, 128, [1, 1, 1], 0), ("bf16", 8, 2, 128, [1, 1, 1], 100),
+    ("f16", 5, 1, 64, [40, 3, 17], 0), ("f32", 4, 2, 96, [5, 1, 2], 0)])
+def test_what_padding_rows_hold_does_not_matter(dev, name, nq, nkv, hd, new, wide):
+    """Rows behind the last sequence: the same bits whatever they hold, and
+    they are left as they were."""
+    p = Paged(dev, name, new, [30, 700, 3], nq, nkv, hd, 16, seed=97, pad=9, packed=True)
+    if wide:
+        p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+    real, got = p.tokens - p.pad, []
+    for value in (0.0, float("inf"), float("nan"), 3.0):
+        for x in (p.q, p.k, p.v):
+            x[real:] = value
+        kc, vc = p.kc.clone(), p.vc.clone()
+        out = torch.full((p.tokens, nq * hd), 7.0, dtype=p.q.dtype, device=dev)
+        rot = vlasr.paged_rope_append(p.q, p.k, p.v, kc, vc, p.q_start, p.kv_len, p.table,
+                                      q_out=out.clone())
+        vlasr.paged_attention(rot, kc, vc, p.q_start, p.kv_len, p.table, max_q_len=max(new), out=out)
+        torch.cuda.synchronize()
+        assert (rot[real:] == 7.0).all() and (out[real:] == 7.0).all()
+        got.append([t.nan_to_num(99.0) for t in (rot[:real], out[:real], kc, vc)])
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
