@@ -874,3 +874,27 @@ def test_what_padding_rows_hold_does_not_matter(dev, name, nq, nkv, hd, new, wid
     for other in got[1:]:
         for a, b in zip(got[0], other):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("at", [129, 130, 131, 133])
+@pytest.mark.parametrize("name,hd", [("bf16", 128), ("f16", 64)])
+def test_attention_nan_among_minus_infinity(dev, name, hd, at):
+    """A NaN key in a long stretch whose other scores are -inf: a cut cell's
+    piece has no finite maximum, and its rows are not finite all the same."""
+    new, past = 33, 2000
+    p = Paged(dev, name, [new], [past], 4, 1, hd, 16, seed=98)
+    ids = p.table[0].cpu().long()
+    for page in range(94):                       # positions 0 .. 1503
+        p.kc[ids[page], :, 0, 5] = -float("inf")
+    p.q.view(new, 4, hd)[:, :, 5] = 1.0
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def run():
+        got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new,
+                                    status=status)
+        torch.cuda.synchronize()
+        return got
+
+    assert torch.isfinite(run()).all()
+    p.kc[ids[at // 16], at % 16, 0] = float("nan")
+    assert not torch.isfinite(run()).any() and int(status) == 0

@@ -1065,7 +1065,9 @@ __global__ void __launch_bounds__(256)
         const float2 q = __ldcg(reinterpret_cast<const float2*>(w.part + row * HD) + lane);
         y[0] = q.x, y[1] = q.y;
       }
-      if (ml.x == -INFINITY && ml.y == ml.y) continue;   // the row sees nothing of it
+      // The row sees nothing of it, or scores of -inf alone; a NaN beside those
+      // leaves a sum of NaN or, by the polynomial, one of 3e38.
+      if (ml.x == -INFINITY && ml.y < 1.0f) continue;
       const float m_new = fmaxf(M, ml.x);
       const float f0 = exp2f(M - m_new), f1 = exp2f(ml.x - m_new);
       M = m_new;
