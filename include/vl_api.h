@@ -639,7 +639,8 @@ VL_EXPORT size_t vl_paged_attention_workspace_bytes(int64_t tokens, int64_t batc
  * with kv head h / (n_q_heads / n_kv_heads); scale 0 means 1/sqrt(head_dim).
  * Scores, softmax and sums in fp32, one rounding of the output; in f16 / bf16
  * at head_dim 64 or 128 the probabilities are rounded to the storage type
- * before the second product.  A token that sees no position (kv_len < n), or
+ * before the second product (f16 ones scaled by a power of two, so that those
+ * below 2^-24 of a row's largest still count).  A token that sees no position (kv_len < n), or
  * only scores of -inf, gives a zero row.
  * max_q_len bounds the new tokens of any sequence and chooses the kernel
  * (single tokens and a few tokens stream the cache once; longer chunks run

@@ -898,3 +898,19 @@ def test_attention_nan_among_minus_infinity(dev, name, hd, at):
     assert torch.isfinite(run()).all()
     p.kc[ids[at // 16], at % 16, 0] = float("nan")
     assert not torch.isfinite(run()).any() and int(status) == 0
+
+
+@pytest.mark.parametrize("new,past,wide", [(1, 1000, 0), (1, 1000, 100), (3, 900, 0),
+                                           (40, 1400, 0), (300, 0, 0)])
+@pytest.mark.parametrize("name,hd", [("f16", 64), ("f16", 128), ("bf16", 128)])
+def test_attention_of_many_small_weights(dev, name, hd, new, past, wide):
+    """One key takes nearly all of a row's weight and its value is 0; what is
+    left are weights of 2^-26 each, which sum to the result."""
+    p = Paged(dev, name, [new], [past], 4, 1, hd, 16, seed=99)
+    if wide:
+        p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+    ids = p.table[0, :-(-(new + past) // 16)].cpu().long()
+    p.kc[ids], p.q[:] = 0.0, 0.0
+    p.kc[ids[0], 0, 0, 5], p.vc[ids[0], 0] = 8.0, 0.0
+    p.q.view(new, 4, hd)[:, :, 5] = 2.25         # a score of 18 against 0
+    run_attention(p, new, scale=1.0)

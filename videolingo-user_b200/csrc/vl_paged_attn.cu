@@ -76,6 +76,11 @@ constexpr int kFewThreads = (kFewWarps + 1) * 32;
 constexpr int kFewStages = 3;
 constexpr int kFewCtasPerSm = 2;
 constexpr int kFewCluster = 4;            // CTAs of a pair, where a cluster takes one
+// Weights are held times 2^15 in f16, the largest that it takes: small ones keep
+// their bits down to 2^-29 of the largest and some down to 2^-39, where sums of
+// thousands of them count beside one large weight.  bf16 has fp32's exponents.
+template <typename T>
+constexpr float kFewLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
 __host__ __device__ constexpr int few_partial_floats(int hd) { return kFewRows * hd + 2 * kFewRows; }
 
@@ -490,8 +495,9 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorM
             alpha[nt][e] = m_new == -INFINITY ? 1.0f : exp2f(m_run[nt][e] - m_new);
             rescale |= alpha[nt][e] != 1.0f;
             m_run[nt][e] = m_new;
-            sv[e] = sv[e] == -INFINITY ? 0.0f : exp2f(sv[e] - m_new);
-            sv[e + 2] = sv[e + 2] == -INFINITY ? 0.0f : exp2f(sv[e + 2] - m_new);
+            const float about = m_new - kFewLift<T>;
+            sv[e] = sv[e] == -INFINITY ? 0.0f : exp2f(sv[e] - about);
+            sv[e + 2] = sv[e + 2] == -INFINITY ? 0.0f : exp2f(sv[e + 2] - about);
             l_run[nt][e] = fmaf(l_run[nt][e], alpha[nt][e], sv[e] + sv[e + 2]);
           }
           // P rounds to the storage type, as its tensor-core operand: half a

@@ -19,9 +19,9 @@
 //     that share a kv head share its tiles, and a TMA box of [tokens][G][64]
 //     brings them in that order;
 //   * O stays in tensor memory.  It is rescaled only when a row's maximum
-//     has grown by more than 2^8 since the last time: until then weights are
-//     taken about the old maximum, which fp32 sums and both 16-bit types
-//     hold (P <= 2^8).
+//     has grown by more than 2^8 since the last time (2^4 in f16): until then
+//     weights are taken about the old maximum, which fp32 sums and both 16-bit
+//     types hold (see kLift).
 //   * a warp each turns page ids into TMA boxes of K and of V, one thread
 //     issues the MMAs, four warps scale and store finished rows while the
 //     others are at the next cell, one warp walks along the cells.
@@ -60,7 +60,16 @@ constexpr int kPlanWarp = 14;
 constexpr int kVWarp = 15;
 constexpr int kThreads = 512;
 constexpr int kPlans = 4;                 // pieces that the walk is ahead
-constexpr float kRescaleLog2 = 8.0f;
+// How far a row's maximum may grow before O is rescaled, and what weights are
+// held times of (log2): with both they reach 2^15 of the 65504 that f16 takes.
+// So small ones keep their bits there down to 2^-25 of the largest and some
+// down to 2^-35, where sums of thousands of them count beside one large
+// weight.  Growth of 2^4 costs nothing against 2^8 (f16, 2048 tokens after 14336:
+// 231.8 and 232.4 us), 2^2 some (236.8).  bf16 has fp32's exponents.
+template <typename T>
+constexpr float kRescaleLog2 = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 11.0f : 0.0f;
 
 template <int HD>
 struct Shape {
@@ -941,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mx = fmaxf(mx, my);
         mx *= scale;
-        if (__any_sync(0xffffffffu, mine && mx > m + kRescaleLog2)) {
+        if (__any_sync(0xffffffffu, mine && mx > m + kRescaleLog2<T>)) {
           const float m_new = fmaxf(m, mx);
           const float f = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
           l *= f;
@@ -960,7 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float off = m == -INFINITY ? 0.0f : -m;
+        const float off = m == -INFINITY ? 0.0f : kLift<T> - m;
         const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
         // P rounds to the storage type, as its tensor-core operand: half a
         // step per weight, against a sum that stays in fp32
