@@ -106,7 +106,6 @@ constexpr int kSelVecs = 8;              // 16-byte vectors of a thread at a tim
 constexpr int kSelStage = kSelThreads * kSelVecs * 16;   // bytes of all threads'
 constexpr int kHeap = 512;               // candidates of a piece outside the lists
 constexpr int kSelStages = 3;            // on their way, or being read
-constexpr float kLog2e = 1.4426950408889634f;
 // A lane's sum is rescaled when its maximum has grown by this much: what was
 // summed before then soon weighs nothing, and with it its rescalings' errors (a
 // row in ascending order would rescale every round, 4e-5 over 2^24 values).

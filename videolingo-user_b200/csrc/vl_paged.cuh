@@ -16,6 +16,16 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
   return x / y;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Two values as 16-bit ones of a type, the first in the low half.
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
+  return pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, __half) {
+  return pack_f16x2(lo, hi);
+}
+
 // The exponential unit's 2^x (relative error below 2^-22).
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -42,8 +42,6 @@
 namespace vl {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 // ---------------------------------------------------------------------------
 // tensor maps
 // ---------------------------------------------------------------------------
@@ -144,12 +142,6 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
-  return pack_bf16x2(lo, hi);
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __half) {
-  return pack_f16x2(lo, hi);
 }
 
 __device__ __forceinline__ int few_tiles(const SeqView& s) {

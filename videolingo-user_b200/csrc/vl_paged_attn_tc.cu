@@ -48,7 +48,6 @@
 namespace vl {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;                // rows of a block (MMA M)
 constexpr int kTile = 128;                // positions of a tile
 constexpr int kStages = 2;                // of K and of V
@@ -436,12 +435,6 @@ __device__ __forceinline__ float2 ex2_pair(float2 z) {
 // with two, against 1360 and 2240 with none, 1350 and 2040 with three of
 // eight.
 __device__ constexpr bool by_polynomial(int pair) { return pair % 4 == 1; }
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
-  return pack_bf16x2(lo, hi);
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __half) {
-  return pack_f16x2(lo, hi);
-}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
