@@ -914,3 +914,35 @@ def test_attention_of_many_small_weights(dev, name, hd, new, past, wide):
     p.kc[ids[0], 0, 0, 5], p.vc[ids[0], 0] = 8.0, 0.0
     p.q.view(new, 4, hd)[:, :, 5] = 2.25         # a score of 18 against 0
     run_attention(p, new, scale=1.0)
+
+
+@pytest.mark.parametrize("new,past,wide", [(3, 500, 0), (3, 500, 100), (70, 500, 0), (70, 3000, 0)])
+@pytest.mark.parametrize("name,hd", [("f16", 64), ("f16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("peak", [2000, 4000])
+def test_attention_of_enormous_scores(dev, name, hd, new, past, wide, peak):
+    """Scores of 10^7 and more, where fp32 no longer holds their fractions: a
+    row is its best key's value (the next is 10^6 below), and finite."""
+    p = Paged(dev, name, [new], [past], 4, 1, hd, 16, seed=101)
+    if wide:
+        p.table = torch.nn.functional.pad(p.table, (0, wide), value=-3)
+    ids = p.table[0, :-(-(new + past) // 16)].cpu().long()
+    p.kc[ids], p.q[:] = 0.0, 0.0
+    g = torch.Generator(device="cpu").manual_seed(102)
+    rising = torch.arange(past + new) % 400 * 8.0 + 128.0       # 128 .. 3320, in many tiles
+    best = past - 77
+    rising[best] = 16000.0
+    flat = torch.zeros(len(ids) * 16)
+    flat[:past + new] = rising
+    p.kc[ids, :, 0, 5] = flat.view(-1, 16).to(p.kc.dtype).to(dev)
+    # many queries, so that the products' roundings fall both ways
+    p.q.view(new, 4, hd)[:, :, 5] = (
+        peak * (1 + torch.rand(new, 4, generator=g)) / 2).to(p.q.dtype).to(dev)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    got = vlasr.paged_attention(p.q, p.kc, p.vc, p.q_start, p.kv_len, p.table, max_q_len=new,
+                                scale=1.0, status=status)
+    torch.cuda.synchronize()
+    want = p.vc[ids[best // 16], best % 16, 0].expand(new, 4, hd).reshape(new, -1)
+    assert int(status) == 0 and torch.isfinite(got).all()
+    # the weight's rounding and the output's
+    assert ((got - want).float().abs() <=
+            2 * paged_ref.HALF_STEP[name] * want.float().abs() * 1.01 + 2.0 ** -24).all()

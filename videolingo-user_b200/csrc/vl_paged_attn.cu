@@ -487,9 +487,9 @@ __device__ __forceinline__ void few_body(const PagedAttnArgs& a, const CUtensorM
             alpha[nt][e] = m_new == -INFINITY ? 1.0f : exp2f(m_run[nt][e] - m_new);
             rescale |= alpha[nt][e] != 1.0f;
             m_run[nt][e] = m_new;
-            const float about = m_new - kFewLift<T>;
-            sv[e] = sv[e] == -INFINITY ? 0.0f : exp2f(sv[e] - about);
-            sv[e + 2] = sv[e + 2] == -INFINITY ? 0.0f : exp2f(sv[e + 2] - about);
+            // (lifted after the difference: scores past 2^24 have no room for it)
+            sv[e] = sv[e] == -INFINITY ? 0.0f : exp2f(sv[e] - m_new + kFewLift<T>);
+            sv[e + 2] = sv[e + 2] == -INFINITY ? 0.0f : exp2f(sv[e + 2] - m_new + kFewLift<T>);
             l_run[nt][e] = fmaf(l_run[nt][e], alpha[nt][e], sv[e] + sv[e + 2]);
           }
           // P rounds to the storage type, as its tensor-core operand: half a

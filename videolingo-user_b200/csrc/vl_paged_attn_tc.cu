@@ -942,8 +942,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           my = fmaxf(my, fmaxf(mz, mw));
         }
         mx = fmaxf(mx, my);
-        mx *= scale;
-        if (__any_sync(0xffffffffu, mine && mx > m + kRescaleLog2<T>)) {
+        // Rounded so that no weight passes 2^(kLift + kRescaleLog2), however large
+        // the scores (past 2^24 a rounding is more than 1).
+        mx = __fmul_ru(mx, scale);
+        if (__any_sync(0xffffffffu, mine && mx > __fadd_rd(m, kRescaleLog2<T>))) {
           const float m_new = fmaxf(m, mx);
           const float f = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
           l *= f;
@@ -962,7 +964,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float off = m == -INFINITY ? 0.0f : kLift<T> - m;
+        const float off = m == -INFINITY ? 0.0f : __fsub_rd(kLift<T>, m);
         const uint64_t scale2 = pair_of(scale, scale), off2 = pair_of(off, off);
         // P rounds to the storage type, as its tensor-core operand: half a
         // step per weight, against a sum that stays in fp32
