@@ -453,3 +453,14 @@ def test_wrappers_tell_their_own_errors_from_wrong_arguments(monkeypatch):
         vlasr.beam_select(x, torch.zeros(2, 2))
     with pytest.raises(AttributeError, match="no such helper"):
         vlasr.paged_rope_append(None, x, x, x, x, x, x, x)
+
+
+def test_beams_below_one_are_refused():
+    """Not taken for greedy decoding."""
+    from vlasr.engine import AsrEngine, transcribe_ids_sharded
+    engine = object.__new__(AsrEngine)
+    for beams in (0, -2):
+        with pytest.raises(vlasr.VlasrInputError, match="beams"):
+            engine.transcribe_ids(np.zeros(16, np.float32), [1], beams=beams)
+        with pytest.raises(vlasr.VlasrInputError, match="beams"):
+            transcribe_ids_sharded(engine, np.zeros((1, 16), np.float32), [1], beams=beams)

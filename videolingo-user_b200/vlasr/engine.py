@@ -22,6 +22,7 @@ from ._lib import VlasrInputError
 from .checkpoint import load_weights
 from .decoder import TextDecoder
 from .encoder import AudioEncoder
+from .paged import BEAM_MAX
 from .synth import CHUNK_SAMPLES
 
 MAX_CHUNKS = 128   # the reference engine's limit per call (native.py:155-157)
@@ -74,6 +75,7 @@ class AsrEngine:
         """pcm: [samples] or [chunks, 480000] f32 (numpy or torch, host or
         device) -> generated ids per chunk: greedy decoding, or with beams > 1
         the best hypothesis of a beam search."""
+        _check_beams(beams)
         if isinstance(pcm, torch.Tensor) and pcm.dim() == 2:
             chunks_t = pcm.to(self.device, torch.float32).contiguous()
         else:
@@ -104,6 +106,11 @@ class AsrEngine:
         return result.per_chunk_ids
 
 
+def _check_beams(beams: int) -> None:
+    if not 1 <= beams <= BEAM_MAX:
+        raise VlasrInputError(f"beams must be in [1, {BEAM_MAX}], got {beams}")
+
+
 def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int = 256,
                            group=None, beams: int = 1) -> list[list[int]]:
     """Multi-GPU engine call: one process per GPU, chunks sharded by
@@ -115,6 +122,7 @@ def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int =
     per-chunk decode), so the ids equal a single-GPU call's."""
     import torch.distributed as dist
     from .pipeline import shard_range
+    _check_beams(beams)
     chunks_np = pcm_chunks if np.asarray(pcm_chunks).ndim == 2 else pad_to_chunks(pcm_chunks)
     chunks = chunks_np.shape[0]
     world = dist.get_world_size(group)
