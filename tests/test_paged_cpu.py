@@ -464,3 +464,27 @@ def test_beams_below_one_are_refused():
             engine.transcribe_ids(np.zeros(16, np.float32), [1], beams=beams)
         with pytest.raises(vlasr.VlasrInputError, match="beams"):
             transcribe_ids_sharded(engine, np.zeros((1, 16), np.float32), [1], beams=beams)
+
+
+def test_backend_does_not_take_no_beams_for_greedy():
+    from vlasr.backend import VlasrAsrBackend
+
+    class Engine:
+        def transcribe_ids(self, pcm, prompt_ids, max_new_tokens=256, beams=1):
+            if beams < 1:
+                raise vlasr.VlasrInputError("beams")
+            return [[1]] * len(pcm)
+
+    class Processor:
+        class tokenizer:
+            @staticmethod
+            def decode(ids, skip_special_tokens=True):
+                return "word"
+
+        def apply_transcription_request(self, arrays):
+            return type("R", (), {"input_ids": [[1, 2]]})
+
+    backend = VlasrAsrBackend(engine=Engine(), processor=Processor(), beams=0,
+                              audio_loader=lambda path: np.ones(16000, np.float32))
+    with pytest.raises(Exception, match="beams"):
+        backend.transcribe("x", "en")

@@ -182,7 +182,7 @@ class VlasrAsrBackend:
 
         processor = self._processor()
         prompt_ids = list(processor.apply_transcription_request([arrays[0]]).input_ids[0])
-        search = {"beams": self.beams} if self.beams > 1 else {}
+        search = {"beams": self.beams} if self.beams != 1 else {}
         try:
             if self.group is not None:
                 from .engine import transcribe_ids_sharded
