@@ -232,3 +232,56 @@ def test_peer_gather_maps_every_other_rank_once(world):
     for p in procs:
         p.join(timeout=60)
     assert all(ok for _, ok, _ in results), results
+
+
+# ---------------------------------------------------------------------------
+# A shard that fails: every rank learns of it in the gather.
+# ---------------------------------------------------------------------------
+
+class _FailingEngine:
+    """Chunk 3 has no hypothesis, as a beam search over logits that are not
+    finite finds."""
+
+    def transcribe_ids(self, chunks, prompt_ids, max_new_tokens=256):
+        from vlasr import VlasrExecutionError
+        if any(int(round(float(c[0]))) == 3 for c in chunks):
+            raise VlasrExecutionError("chunks [1] have no hypothesis")
+        return [[1] for _ in chunks]
+
+
+def _failing_worker(rank, world, port, q):
+    import time
+    try:
+        import numpy as np
+        from vlasr import VlasrExecutionError
+        from vlasr.engine import transcribe_ids_sharded
+        dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank,
+                                world_size=world, timeout=datetime.timedelta(seconds=20))
+        pcm = np.repeat(np.arange(4, dtype=np.float32)[:, None], 480000, axis=1)
+        began = time.monotonic()
+        try:
+            transcribe_ids_sharded(_FailingEngine(), pcm, [1, 2, 3], 8)
+            said = "nothing"
+        except VlasrExecutionError as exc:
+            said = str(exc)
+        took = time.monotonic() - began
+        dist.barrier()                        # the group is still usable
+        dist.destroy_process_group()
+        q.put((rank, said, took))
+    except Exception as exc:  # noqa: BLE001
+        q.put((rank, repr(exc), 1e9))
+
+
+def test_a_failing_shard_is_an_error_on_every_rank():
+    world, port = 2, _free_port()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_failing_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    results = sorted(q.get(timeout=120) for _ in range(world))
+    for p in procs:
+        p.join(timeout=60)
+    assert "rank 1" in results[0][1] and "no hypothesis" in results[0][1], results
+    assert results[1][1] == "chunks [1] have no hypothesis", results
+    assert all(took < 15 for _, _, took in results), results

@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import ops
-from ._lib import VlasrInputError
+from ._lib import VlasrExecutionError, VlasrInputError
 from .checkpoint import load_weights
 from .decoder import TextDecoder
 from .encoder import AudioEncoder
@@ -119,7 +119,8 @@ def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int =
     on its own engine and the id lists are all-gathered, so every rank
     returns the ids of all chunks in chunk order.  Chunks are independent
     (per-chunk mel normalisation, unmasked per-chunk encoder attention,
-    per-chunk decode), so the ids equal a single-GPU call's."""
+    per-chunk decode), so the ids equal a single-GPU call's.  A shard that
+    fails raises on every rank, after the gather."""
     import torch.distributed as dist
     from .pipeline import shard_range
     _check_beams(beams)
@@ -128,13 +129,23 @@ def transcribe_ids_sharded(engine, pcm_chunks, prompt_ids, max_new_tokens: int =
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)
     c0, c1 = shard_range(chunks, rank, world)
-    more = {"beams": beams} if beams > 1 else {}
-    mine = engine.transcribe_ids(chunks_np[c0:c1], prompt_ids, max_new_tokens=max_new_tokens,
-                                 **more) if c1 > c0 else []
+    more = {"beams": beams} if beams != 1 else {}
+    mine, failure = [], None
+    try:
+        if c1 > c0:
+            mine = engine.transcribe_ids(chunks_np[c0:c1], prompt_ids,
+                                         max_new_tokens=max_new_tokens, **more)
+    except Exception as exc:  # noqa: BLE001 - told to the others, then raised
+        failure = exc
     gathered: list = [None] * world
-    dist.all_gather_object(gathered, mine, group=group)
+    dist.all_gather_object(gathered, (mine, None if failure is None else repr(failure)),
+                           group=group)
+    if failure is not None:
+        raise failure
     out: list[list[int]] = []
-    for part in gathered:
+    for r, (part, error) in enumerate(gathered):
+        if error is not None:
+            raise VlasrExecutionError(f"the shard of rank {r} failed: {error}")
         out.extend(part)
     if len(out) != chunks:
         raise VlasrInputError(f"sharded engine returned {len(out)} transcripts for {chunks} chunks")
