@@ -383,6 +383,7 @@ def _stub_decoder(monkeypatch, layers=2):
     dec.shape = SimpleNamespace(heads=2, kv_heads=1, head_dim=64, hidden=64, eps=1e-5, layers=layers,
                                 rope_base=1e4)
     dec.fused, dec.device, dec.eos_ids, dec.embed = False, torch.device("cpu"), (3,), None
+    dec.dtype, dec._states = torch.float32, {}
     dec.layer_w = [{"ln1": None, "qkv_t": torch.zeros(64, 256), "o_t": torch.zeros(128, 64)}
                    for _ in range(layers)]
     dec._mlp = lambda lw, h, a: a
@@ -488,3 +489,16 @@ def test_backend_does_not_take_no_beams_for_greedy():
                               audio_loader=lambda path: np.ones(16000, np.float32))
     with pytest.raises(Exception, match="beams"):
         backend.transcribe("x", "en")
+
+
+def test_sizes_of_zero_are_input_errors(monkeypatch):
+    from vlasr import paged
+    empty = torch.zeros(2, 16, 1, 0)
+    with pytest.raises(vlasr.VlasrInputError, match="head_dim"):
+        paged._cache_pages(empty, empty)
+    dec, _ = _stub_decoder(monkeypatch)
+    dec.max_seq_len = 64
+    for page_size in (0, -16, 8, 48, 512):
+        with pytest.raises(vlasr.VlasrInputError, match="page_size"):
+            dec.generate_beam(torch.zeros(1, 375, 64), [1, 2], beams=2, max_new_tokens=4,
+                              page_size=page_size)

@@ -555,6 +555,9 @@ class TextDecoder:
         chunks = audio.shape[0]
         if not 1 <= beams <= paged.BEAM_MAX:
             raise VlasrInputError(f"beams must be in [1, {paged.BEAM_MAX}]")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise VlasrInputError("page_size must be a power of two in [16, 256], got "
+                                  f"{page_size}")
         if chunks < 1 or L < 1 or max_new_tokens < 1:
             raise VlasrInputError("at least one chunk, prompt id and new token are required")
         if L + max_new_tokens > self.max_seq_len:

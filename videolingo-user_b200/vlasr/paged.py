@@ -144,6 +144,8 @@ def _cache_pages(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int
         raise VlasrInputError("k_cache and v_cache must be [num_pages, page_size, kv_heads, "
                               "head_dim] of the same shape and strides")
     num_pages, page_size, heads, hd = shape
+    if hd == 0:
+        raise VlasrInputError("the caches' head_dim must be positive")
     if stride[3] != 1 or (stride[2] != hd and heads != 1) or stride[1] != heads * hd:
         raise VlasrInputError("the rows of a cache page must be contiguous")
     return num_pages, page_size, heads, hd, stride[0] if num_pages > 1 else max(
