@@ -502,3 +502,21 @@ def test_sizes_of_zero_are_input_errors(monkeypatch):
         with pytest.raises(vlasr.VlasrInputError, match="page_size"):
             dec.generate_beam(torch.zeros(1, 375, 64), [1, 2], beams=2, max_new_tokens=4,
                               page_size=page_size)
+
+
+def test_exponential_polynomial():
+    """2^f on [-1/2, 1/2] by the coefficients that the kernel holds, in fp32 with
+    fused steps as there: within the 2.2e-7 that its comment states."""
+    import re
+
+    from conftest import PKG
+    text = (PKG / "csrc" / "vl_paged_attn_tc.cu").read_text()
+    body = text[text.index("float2 ex2_pair"):text.index("halves_of(p)")]
+    cf = [np.float32(x) for x in re.findall(r"pair_of\((0\.\d+|1\.\d+)f, \1f\)", body)]
+    assert len(cf) == 6
+    f = np.linspace(-0.5, 0.5, 400001).astype(np.float32)
+    p = np.full_like(f, cf[0])
+    for c in cf[1:]:
+        p = (p.astype(np.float64) * f + np.float64(c)).astype(np.float32)
+    off = np.abs(p.astype(np.float64) / np.exp2(f.astype(np.float64)) - 1)
+    assert off.max() <= 2.2e-7

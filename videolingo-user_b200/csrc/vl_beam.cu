@@ -10,7 +10,7 @@
 // entry.  It is bound by the read of the logits (about eight instructions an
 // element keep up with it) and by what a piece costs by itself, or for one
 // entry by two launches' latency: 64 x 5 f32 rows of 51865, some finished
-// (53 MB), 20.9 us, 1 x 4 bf16 rows of 59264 9.9 us.
+// (53 MB), 20.9 us, 64 x 5 bf16 rows of 59264 (38 MB) 24.6, 1 x 4 of them 10.4.
 //   * The K-th largest of the lanes' maxima of the first round bounds the K-th
 //     largest value from below and lets few values through (a few dozen of
 //     50,000, as what gets through raises the bound again): these go to a
@@ -33,8 +33,8 @@
 // CTA of an entry works the small plan out for itself (a bitmap of the
 // entry's range in shared memory), so one launch does tables and copies and
 // nothing waits for another CTA.  Bound by the copies: 32 x 5 rows over 28
-// layers (119 MB moved) 25.6 us, 0.70 of the measured copy rate; 4 x 4 rows
-// 6.2 us, the plan's chain of look-ups.
+// layers (119 MB moved) 23.6 us, 0.77 of the measured copy rate; 4 x 4 rows
+// 6.0 us, the plan's chain of look-ups.
 #include <atomic>
 #include <cmath>
 
@@ -780,8 +780,8 @@ cudaError_t launch_beam_select(const BeamSelectArgs& a, int dtype, void* workspa
 
 cudaError_t launch_beam_reorder(const BeamReorderArgs& a, cudaStream_t stream) {
   if (a.batch == 0) return cudaSuccess;
-  // about eight CTAs per SM over the entries (32 x 5 rows, 28 layers: 25.0 us,
-  // with four 27.0), and no more than there are segments when half the rows
+  // about eight CTAs per SM over the entries (32 x 5 rows, 28 layers: 23.6 us,
+  // with four 26.2), and no more than there are segments when half the rows
   // copy
   int64_t per = (static_cast<int64_t>(sm_count()) * 8 + a.batch - 1) / a.batch;
   const int64_t most = 2 * a.layers * (a.beams > 1 ? a.beams / 2 : 1);

@@ -16,9 +16,9 @@
 // then move 16-byte vectors: a task is the two vectors of a head that turn
 // together (one, when interleaved), or one that is only copied.
 //
-// 16 x 383 tokens, 16 / 4 heads of 128, bf16 (75 MB): 18.6 us, 0.62 of the
+// 16 x 383 tokens, 16 / 4 heads of 128, bf16 (75 MB): 18.3 us, 0.63 of the
 // measured copy rate; issue slots are 0.57 busy, the rest is what the short
-// blocks wait for (lookup, sincosf, first vectors).  16 x 1: 3.4 us.
+// blocks wait for (lookup, sincosf, first vectors).  16 x 1: 3.1 us.
 #include <cmath>
 
 #include "vl_common.cuh"
@@ -32,8 +32,8 @@ namespace {
 constexpr int kAppendThreads = 256;
 // Tasks of a thread in flight: a task that turns two vectors holds twice the
 // registers.  With three of those five blocks fit on an SM (16 x 383 tokens:
-// 18.6 us, with four and four blocks 19.2).  Interleaved ones fit six with four
-// as they come (37 ragged sequences: 53.4 us, 62.8 with three; held to six
+// 18.3 us, with four and four blocks 0.6 more).  Interleaved ones fit six with four
+// as they come (37 ragged sequences: 53.2 us, 62.8 with three; held to six
 // blocks 55.1).
 constexpr int append_ahead(bool interleaved) { return interleaved ? 4 : 3; }
 constexpr int kAppendTokens = 4;  // of a block, at most

@@ -25,10 +25,12 @@
 //   * A consumer warp owns 16 positions of a stage and keeps its own running
 //     maximum and sums; warps are joined once per pair.
 // 64 sequences of up to 4096 positions (269 MB), 16 / 4 heads of 128: 53.5 us,
-// 5.0 TB/s, 0.77 of the measured copy rate (0.82 when all are equally long);
-// what is left is the ring's start and the join.  4 sequences of 500: 6.7 us,
-// the latency of a launch, of lengths, pages and rows one after the other, and of
-// the join.
+// 5.0 TB/s, 0.77 of the measured copy rate (90 us and 0.91 when all are that
+// long); what is left is the ring's start and the join.  4 sequences of 500:
+// 6.7 us, the latency of a launch, of lengths, pages and rows one after the
+// other, and of the join.  Pages that beams share are read once per beam; most
+// of that comes from L2 (16 x 4 beams of 421 positions 12.9 us, 16.9 with pages
+// of their own; 32 x 5: 28.0 and 34.5).
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -783,10 +785,10 @@ __global__ void __launch_bounds__(kJoinThreads)
 }
 
 // Few pairs and tables of at most 1024 positions: one launch of clusters,
-// instead of the line and its join.  4 sequences of 500, G = 4: 6.6 us against
-// 7.9 (4 tokens each 9.0 against 12.2); of 1000: 8.0 against 8.6; of 2000 the
-// line is better, 9.5 against 10.9.  Clusters of eight: 6.5 us at 500, 6.3
-// against 5.8 at 200, and fewer of them fit.
+// instead of the line and its join.  4 sequences of 500, G = 4: 6.7 us against
+// 8.0 (4 tokens each 9.0 against 12.2); of 200: 5.6 against 7.6; of 1000: 8.1
+// against 8.8; of 2000 the line is better, 9.6 against 10.9.  Clusters of eight
+// gain 0.1 us at 500, lose 0.5 at 200, and fewer of them fit.
 bool few_by_cluster(const PagedAttnArgs& a) {
   const int64_t pairs = static_cast<int64_t>(a.batch) * a.n_kv_heads;
   const int64_t tiles = (static_cast<int64_t>(a.max_pages) * a.page_size + kFewTile - 1) / kFewTile;
@@ -951,8 +953,9 @@ enum class Kind { kFew, kChunk, kAny };
 
 // Up to 16 rows per kv head (two 8-wide MMA columns) the few-token kernel
 // streams the cache; from there on the tcgen05 kernel's 128-row blocks re-read
-// it less often.  64 x 4 tokens over 2048 positions, G = 4 (16 rows): 57 us
-// against 71; 16 x 4 over 1000: 16 against 28; 4 x 1 over 500: 8 against 16.
+// it less often.  64 x 4 tokens over 2048 positions, G = 4 (16 rows): 57.6
+// us against 71.4; 16 x 4 over 1000: 16.8 against 29.0; 4 x 1 over 500: 6.7
+// against 16.2.
 Kind paged_kind(int64_t max_q_len, int n_q_heads, int n_kv_heads, int head_dim, int dtype) {
   if (dtype == kDtypeF32 || (head_dim != 64 && head_dim != 128)) return Kind::kAny;
   return max_q_len * (n_q_heads / n_kv_heads) <= kFewRows ? Kind::kFew : Kind::kChunk;

@@ -29,8 +29,9 @@
 // long cell is cut where a share ends, and a second launch joins the partial
 // sums of its pieces.
 //
-// 2048 tokens after 14336, 16 / 4 heads of 128, bf16: 225 us, 1140 TFLOP/s, 0.69
-// of cuBLAS's rate.  What bounds it is the chain of a block's tile (maximum,
+// 2048 tokens after 14336, 16 / 4 heads of 128, bf16: 226 us at 1.9 GHz, 1140
+// TFLOP/s, 0.69 of cuBLAS's burst rate; 265 where long runs settle under the
+// power cap, 0.70 of its sustained rate.  What bounds it is the chain of a block's tile (maximum,
 // exponentials, two products: some 4000 cycles for two blocks side by side,
 // 2050 of them tensor cores' and 1940 the exponentials').  Short cells add what
 // they cost by themselves (16 x 383 tokens, 33 us: 9000 cycles until the first
@@ -412,8 +413,9 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   return y;
 }
 // 2^x of two values on the multiply-add pipe, beside the exponential unit:
-// x = n + f with |f| <= 1/2, a degree-5 polynomial of f fitted to the least
-// relative error (2.2e-7), n added to the exponent.  Values below -126 give
+// x = n + f with |f| <= 1/2, a degree-5 polynomial of f (least squares of the
+// relative error, reweighted until it is level: 2.2e-7 in fp32), n added to the
+// exponent.  Values below -126 give
 // about 1e-38 (a row all of -inf is told by its maximum), NaN gives what rounds
 // to infinity in either type.
 __device__ __forceinline__ float2 ex2_pair(float2 z) {
