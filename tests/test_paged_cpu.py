@@ -520,3 +520,27 @@ def test_exponential_polynomial():
         p = (p.astype(np.float64) * f + np.float64(c)).astype(np.float32)
     off = np.abs(p.astype(np.float64) / np.exp2(f.astype(np.float64)) - 1)
     assert off.max() <= 2.2e-7
+
+
+def test_wrong_arguments_on_another_device_are_input_errors(monkeypatch):
+    """The call is made again under the tensors' device; its checks are the same."""
+    import contextlib
+
+    from vlasr import paged
+    under = []
+
+    @contextlib.contextmanager
+    def device(index):
+        under.append(index)
+        yield
+        under.pop()
+
+    def lead(t, name):
+        if not under:
+            raise paged._OtherDevice(3)
+        return 0, t.dtype, t.get_device()
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(paged, "_lead", lead)
+    with pytest.raises(vlasr.VlasrInputError, match="scores is not a torch.Tensor"):
+        vlasr.beam_select(torch.zeros(2, 8), [[0.0, 0.0]])

@@ -65,10 +65,11 @@ def _operator(fn):
     @functools.wraps(fn)
     def call(*args, **kwargs):
         try:
-            return fn(*args, **kwargs)
-        except _OtherDevice as e:
-            with torch.cuda.device(e.device):
+            try:
                 return fn(*args, **kwargs)
+            except _OtherDevice as e:
+                with torch.cuda.device(e.device):
+                    return fn(*args, **kwargs)
         except AttributeError:
             for name, value in signature.bind(*args, **kwargs).arguments.items():
                 if name in tensors and not isinstance(value, torch.Tensor) and (
