@@ -946,3 +946,25 @@ def test_attention_of_enormous_scores(dev, name, hd, new, past, wide, peak):
     # the weight's rounding and the output's
     assert ((got - want).float().abs() <=
             2 * paged_ref.HALF_STEP[name] * want.float().abs() * 1.01 + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("seqs,share", [(12, 0.5), (300, 0.1), (1500, 0.05), (1500, 0.5)])
+@pytest.mark.parametrize("name,hd", [("bf16", 128), ("f16", 64)])
+def test_attention_chunks_among_sequences_that_see_nothing(dev, name, hd, seqs, share):
+    """Rows of sequences without positions, many in a row, between chunks that
+    end inside a tile: every block's run has pieces without tiles behind one
+    that has some."""
+    rng = np.random.default_rng(seqs)
+    new = rng.integers(1, 4, seqs)
+    past = rng.integers(0, 60, seqs)
+    new[seqs // 3] = 20
+    p = Paged(dev, name, new.tolist(), past.tolist(), 2, 2, hd, 16, seed=103)
+    lens = p.kv_len.cpu().numpy()
+    gone = rng.random(seqs) > share
+    gone[seqs // 3] = False
+    lens[gone] = 0
+    p.kv_len.copy_(torch.from_numpy(lens))
+    got = run_attention(p, 20)
+    starts = p.q_start.cpu().numpy()
+    for b in np.nonzero(gone)[0][:50]:
+        assert int(got[starts[b]:starts[b + 1]].count_nonzero()) == 0

@@ -34,7 +34,7 @@
 // power cap, 0.70 of its sustained rate.  What bounds it is the chain of a block's tile (maximum,
 // exponentials, two products: some 4000 cycles for two blocks side by side,
 // 2050 of them tensor cores' and 1940 the exponentials').  Short cells add what
-// they cost by themselves (16 x 383 tokens, 33 us: 9000 cycles until the first
+// they cost by themselves (16 x 383 tokens, 33.4 us: 9000 cycles until the first
 // scores, 3000 for a cell's last product and its rows, runs of 2 or 3 cells).
 #include <cuda.h>
 
@@ -675,6 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           clear_stage = st;
         }
       }
+      // a piece without tiles: the plan behind it may wait for the last one's rows
+      if (ok && p.j0 == p.j1) clear_tail();
     }
     if (ok) clear_tail();
     if (*reinterpret_cast<volatile int*>(&bars.bad)) {
@@ -738,65 +740,69 @@ __global__ void __launch_bounds__(kThreads, 1)
       struct Count {
         int all, of[2], apart;
       };
-      auto next_piece = [&](Count& c) {
-        for (;;) {
-          wait(bars.plan_full[piece % kPlans], piece / kPlans);
-          if (!ok) return false;
-          const Plan& p = bars.plan[piece % kPlans];
-          const bool over = p.last != 0;
-          c.all = p.j1 - p.j0;
-          c.apart = p.apart;
-          c.of[0] = p.count[0];
-          c.of[1] = p.count[1];
-          mbarrier_arrive(&bars.plan_empty[piece % kPlans]);
-          ++piece;
-          if (over) return false;
-          if (c.all > 0) return true;
-        }
+      auto next_piece = [&](Count& c) {                    // false: the run is over
+        wait(bars.plan_full[piece % kPlans], piece / kPlans);
+        if (!ok) return false;
+        const Plan& p = bars.plan[piece % kPlans];
+        const bool over = p.last != 0;
+        c.all = p.j1 - p.j0;
+        c.apart = p.apart;
+        c.of[0] = p.count[0];
+        c.of[1] = p.count[1];
+        mbarrier_arrive(&bars.plan_empty[piece % kPlans]);
+        ++piece;
+        return !over;
       };
       Count now, then;
-      bool more = next_piece(now);
-      if (more) {
+      bool more = true;
+      while (ok && more) {                // pieces with tiles, one behind the other
+        more = next_piece(now);
+        if (!more || now.all == 0) continue;
         if (now.of[0] > 0) {
-          ask(0, 0, true, now.of[0] == 1);
+          ask(0, tile, true, now.of[0] == 1);
           // in a long run the second block starts half a tile later, and stays
           // there: one's products run under the other's exponentials
-          if (now.apart) wait(bars.p_half[0], 0);
+          if (tile == 0 && now.apart) wait(bars.p_half[0], 0);
         }
-        if (now.of[1] > 0) ask(1, 0, true, now.of[1] == 1);
-        commit(&bars.k_empty[0]);
-      }
-      int jj = 0;
-      while (ok && more) {
-        const bool ends = jj + 1 == now.all;
-        int jn = jj + 1;
-        then = now;
-        if (ends) {
-          more = next_piece(then);
-          jn = 0;
-          if (!more) then.of[0] = then.of[1] = 0;
-        }
-        wait(bars.v_full[tile % kStages], tile / kStages);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (jj < now.of[i]) {
-            // O of the block's last cell has been read
-            if (jj == 0 && begun[i]++ > 0) wait(bars.o_free[i], begun[i]);
-            wait(bars.p_half[i], used[i]);
-            if (ok) values(i, 0, jj == 0);
-            wait(bars.p_ready[i], used[i]++);
-            if (ok) {
-              values(i, 1, false);
-              if (jj + 1 == now.of[i]) commit(&bars.o_done[i]);
-            }
+        if (now.of[1] > 0) ask(1, tile, true, now.of[1] == 1);
+        commit(&bars.k_empty[tile % kStages]);
+        int jj = 0;
+        bool linked = true;               // the next tile's scores are asked for
+        while (ok && linked) {
+          const bool ends = jj + 1 == now.all;
+          int jn = jj + 1;
+          then = now;
+          if (ends) {
+            // One piece is looked ahead.  Where its rows see nothing, one with
+            // tiles is looked for when this one's products are issued: plans are
+            // handed out as far as kPlans ahead of the rows being finished.
+            more = next_piece(then);
+            linked = more && then.all > 0;
+            jn = 0;
+            if (!linked) then.of[0] = then.of[1] = 0;
           }
-          if (jn < then.of[i]) ask(i, tile + 1, ends, jn + 1 == then.of[i]);
+          wait(bars.v_full[tile % kStages], tile / kStages);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (jj < now.of[i]) {
+              // O of the block's last cell has been read
+              if (jj == 0 && begun[i]++ > 0) wait(bars.o_free[i], begun[i]);
+              wait(bars.p_half[i], used[i]);
+              if (ok) values(i, 0, jj == 0);
+              wait(bars.p_ready[i], used[i]++);
+              if (ok) {
+                values(i, 1, false);
+                if (jj + 1 == now.of[i]) commit(&bars.o_done[i]);
+              }
+            }
+            if (jn < then.of[i]) ask(i, tile + 1, ends, jn + 1 == then.of[i]);
+          }
+          commit(&bars.v_empty[tile % kStages]);
+          if (linked) commit(&bars.k_empty[(tile + 1) % kStages]);
+          ++tile;
+          now = then;
+          jj = jn;
         }
-        commit(&bars.v_empty[tile % kStages]);
-        if (more) commit(&bars.k_empty[(tile + 1) % kStages]);
-        ++tile;
-        now = then;
-        jj = jn;
       }
       // every MMA has ended, and with it the arrivals that it owes
       commit(&bars.end);
