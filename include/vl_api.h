@@ -691,8 +691,8 @@ VL_EXPORT size_t vl_beam_select_workspace_bytes(int64_t batch, int beams, int64_
  * -inf, ...).  Places without a candidate get value -inf and are finished.
  * scores_out may be scores and finished_out may be finished; finished_out may
  * be NULL.  Sums in fp32 over 64 values of a thread and fp64 above, values in
- * fp64 (within 1e-5 at any vocab), rounded to f32 once.  beams <= 32, vocab <= 2^24, f32 / f16 / bf16; any
- * vocab and row_stride.  workspace as in vl_paged_attention.
+ * fp64 (within 1e-5 at any vocab), rounded to f32 once.  beams <= 32, vocab
+ * <= 2^24, f32 / f16 / bf16; any vocab and row_stride.  workspace as in vl_paged_attention.
  * vl_beam_select_status does the same and takes a status word (or NULL): a
  * bounded wait that runs out inside the kernel makes its beam offer nothing,
  * and VL_STATUS_TIMEOUT tells that from a masked row.

@@ -31,11 +31,12 @@
 //
 // 2048 tokens after 14336, 16 / 4 heads of 128, bf16: 226 us at 1.9 GHz, 1140
 // TFLOP/s, 0.69 of cuBLAS's burst rate; 265 where long runs settle under the
-// power cap, 0.70 of its sustained rate.  What bounds it is the chain of a block's tile (maximum,
-// exponentials, two products: some 4000 cycles for two blocks side by side,
-// 2050 of them tensor cores' and 1940 the exponentials').  Short cells add what
-// they cost by themselves (16 x 383 tokens, 33.4 us: 9000 cycles until the first
-// scores, 3000 for a cell's last product and its rows, runs of 2 or 3 cells).
+// power cap, 0.70 of its sustained rate.  What bounds it is the chain of a
+// block's tile (maximum, exponentials, two products: some 4000 cycles for two
+// blocks side by side, 2050 of them tensor cores' and 1940 the exponentials').
+// Short cells add what they cost by themselves (16 x 383 tokens, 33.4 us: 9000
+// cycles until the first scores, 3000 for a cell's last product and its rows,
+// runs of 2 or 3 cells).
 #include <cuda.h>
 
 #include <atomic>

@@ -20,8 +20,9 @@ page_table int32 [batch, max_pages] (rows may be strided).  Sequence b's new
 tokens are the packed rows q_start[b] .. q_start[b + 1] - 1, the last of its
 kv_len[b] positions; position p lies in row p % page_size of page
 page_table[b, p // page_size].  Packed rows behind the last sequence are left
-as they were, and what they hold does not matter (they may be read).  What is out of range on the device is skipped and sets
-VL_STATUS_BAD_PAGE in `status` (an int32 tensor), if given.
+as they were, and what they hold does not matter (they may be read).  What is
+out of range on the device is skipped and sets VL_STATUS_BAD_PAGE in `status`
+(an int32 tensor), if given.
 """
 
 from __future__ import annotations
